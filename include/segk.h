@@ -289,6 +289,77 @@ int segk_dot(const void* a, int lda, const void* b, int ldb, int dtype, long lon
              float* result, segk_stream_t stream);
 int segk_dot_partial_rows(long long M);
 
+/* ---- multi-head attention -------------------------------------------------------------------- */
+/* The multi-head form of the position attention (modeling/damm_cam_pam.py:22-48 is its single-head form), fused: no
+ * [Lq][Lk] matrix is stored.  For image n, token i, head h (which reads key / value head h / (Hq / Hk)):
+ *   s_j = scale * q_i . k_j over the open keys j,  out_i = sum_j softmax(s)_j v_j,  lse_i = log sum_j exp(s_j).
+ * Key j is open to token i when mask and key_mask (bytes, non-zero = open; NULL = all) say so and, with causal != 0,
+ * j <= i + Lk - Lq.  A row without an open key gives out = 0, lse = -inf and no gradient.  A key that key_mask closes is
+ * not read; a pair that only `mask` closes has probability zero, its key and value are read.
+ * Operands: [N][L][heads][D] by element strides with unit stride over D, 16-byte aligned, strides multiples of 16 bytes
+ * (0: broadcast); D a multiple of 8 up to 128.  bf16 operands: fp32 scores, statistics and sums, probabilities rounded to
+ * bf16 for their products; fp32 operands: exact-fp32 products throughout. */
+typedef struct {
+  void* p;
+  long long n, l, h; /* elements between images, tokens, heads */
+} segk_attention_view;
+typedef struct {
+  int N, Lq, Lk, Hq, Hk, D;
+  int dtype;   /* of every operand, result and gradient */
+  int causal;
+  float scale; /* > 0 */
+  segk_attention_view q, k, v;
+  segk_attention_view out;
+  float* lse;  /* [N][Hq][Lq]; NULL in a forward pass that needs none */
+  const void* mask;
+  long long mask_n, mask_h, mask_q, mask_k; /* byte strides of `mask` over images, query heads, tokens, keys */
+  const void* key_mask;
+  long long key_mask_n, key_mask_k;
+  /* backward only */
+  segk_attention_view dout;
+  void* dq;    /* [N][Lq][Hq][D], or NULL: not wanted */
+  void* dk;    /* [N][Lk][Hk][D], dk and dv both or neither */
+  void* dv;
+  void* workspace; /* segk_attention_workspace(args, backward) bytes, 16-byte aligned, used by this call only */
+  long long workspace_bytes;
+} segk_attention_args;
+int segk_attention_fwd(const segk_attention_args* a, segk_stream_t stream);
+/* Gradients from q, k, v, out, lse and dout: the probabilities are computed again.  Every sum has a fixed order. */
+int segk_attention_bwd(const segk_attention_args* a, segk_stream_t stream);
+/* Bytes of workspace, 0 if none; negative status on bad arguments.  The same fields as for the call, workspace aside. */
+long long segk_attention_workspace(const segk_attention_args* a, int backward);
+
+/* Norm and position rotation of queries and keys in front of the attention, one pass: every head x of every token is
+ * scaled to y = w * x * (mean x^2 + eps)^-1/2 (norm != 0; w NULL = 1) and its channel pairs are turned by the angle
+ * position * inv_freq.  The first sum(section) pairs rotate, section[a] of them by position axis a (time, height, width,
+ * ...), channels past them pass through; pair c is channels (c, c + sum(section)), or (2c, 2c + 1) with interleaved != 0.
+ * positions: int32 (pos_dtype 0), int64 (1) or fp32 (2), element strides over images (0: shared), tokens, axes.
+ * D a multiple of 8 up to 256, sum(section) a multiple of 4 up to D / 2; q, k as segk_attention_args (Hk = 0: queries
+ * alone); results contiguous [N][L][heads][D]. */
+typedef struct {
+  int N, L, Hq, Hk, D;
+  int dtype;
+  segk_attention_view q, k;
+  void *q_out, *k_out;   /* backward: the gradients of q and k */
+  const float *q_weight, *k_weight; /* [D] or NULL */
+  const void* positions;
+  int pos_dtype;
+  long long pos_n, pos_l, pos_a;
+  int axes;              /* 1 .. 4 */
+  int section[4];
+  const float* inv_freq; /* [sum of section] */
+  int norm, interleaved;
+  float eps;
+  /* backward only */
+  segk_attention_view dq, dk;       /* gradients of the results */
+  float *dq_weight, *dk_weight;     /* [D] or NULL: not wanted */
+  void* workspace;                  /* segk_qk_norm_rotary_bwd_workspace(args) bytes */
+  long long workspace_bytes;
+} segk_qk_norm_rotary_args;
+int segk_qk_norm_rotary(const segk_qk_norm_rotary_args* a, segk_stream_t stream);
+int segk_qk_norm_rotary_bwd(const segk_qk_norm_rotary_args* a, segk_stream_t stream);
+long long segk_qk_norm_rotary_bwd_workspace(const segk_qk_norm_rotary_args* a);
+
 /* ---- batch normalisation (synchronized) ----------------------------------------------------- */
 /* Layouts for the BN entry points. */
 typedef enum { SEGK_PM = 0 /* [M][ld], channels contiguous */, SEGK_NCHW = 1 /* [N][C][HW] */ } segk_layout;

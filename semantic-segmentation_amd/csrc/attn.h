@@ -1,0 +1,290 @@
+// Shared pieces of the multi-head attention kernels (attn_fwd.hip, attn_dkv.hip, attn_dq.hip).
+//
+// Everything is built from 32 x 32 MFMA tiles whose contraction runs over 16 elements ("k-step"):
+//   operand fragment  lane l holds row (or column) l & 31 and 8 of the 16 contracted elements; h = l >> 5 picks which
+//   result tile       lane l holds column l & 31 and the 16 rows 8 * (i / 4) + 4 * h + i % 4, i = 0 .. 15
+// The contracted elements may be dealt to the (h, e) slots in any order as long as both operands use the same one.  A
+// result tile therefore IS the operand of the next product without any exchange between lanes: registers 8 s .. 8 s + 7
+// of a tile of scores hold rows 16 s + 8 (e / 4) + 4 h + e % 4, and the other operand is read from LDS in that order
+// (AttnRead::cols below).  So the probabilities never leave the registers of the lane that computed them.
+//   bf16: v_mfma_f32_32x32x16_bf16; fp32: eight v_mfma_f32_32x32x2_f32 on the same fragments.
+//
+// Shared heads: the G = Hq / Hk query heads that read one key / value head are packed into the rows of one problem,
+// row r = token r / G, head r % G of the group.  Keys and values are then read once for the group, and the gradient of a
+// shared head is a sum over rows inside one workgroup.
+#pragma once
+#include "common.h"
+
+namespace segk {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 attn_bf16x8;
+typedef __attribute__((ext_vector_type(4))) short attn_s16x4;
+typedef __attribute__((address_space(3))) void* attn_lds_ptr;
+
+constexpr int ATTN_THREADS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr unsigned ATTN_OOB = 0xfffffff0u;   // buffer offsets at or past this read as zeros and touch no memory
+
+struct AttnView {   // element strides of a [N][L][heads][D] operand, unit stride over D
+  const char* p;
+  long long n, l, h;
+};
+
+struct AttnDev {
+  AttnView q, k, v, o, dout;
+  char *out, *dq, *dk, *dv;       // out: strides of `o`; gradients contiguous [N][L][heads][D]
+  float* lse;                     // [N][Hq][Lq] natural log, or NULL
+  const unsigned char* mask;      // element strides below; NULL = all open
+  long long m_n, m_h, m_q, m_k;
+  const unsigned char* kmask;     // [N][Lk]
+  long long km_n, km_k;
+  int N, Lq, Lk, Hq, Hk, G, D;
+  int R;                          // rows of one problem: Lq * G
+  int Rp;                         // R rounded up to 64 (row statistics of the backward pass)
+  unsigned g_magic;               // r / G = umulhi(r, g_magic) for G > 1
+  int causal, off;                // key j is open to token i when j <= i + off, off = Lk - Lq
+  float scale, scale_log2;
+  int tiles, splits;              // workgroup tiles of one problem, parts of the looped axis
+  float* part;                    // partial results of the splits
+  float* part_ml;
+  float *row_lse2, *row_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and rowsum(dout * out)
+};
+
+__device__ __forceinline__ int div_g(const AttnDev& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.g_magic); }
+
+// Workgroup -> piece of work such that the workgroups of one XCD (blockIdx % 8 in launch order) take neighbouring
+// pieces: the tiles of one head share its keys and values in that XCD's L2.  Returns -1 for the grid's padding.
+__device__ __forceinline__ int xcd_contiguous(int total) {
+  const int per = (int)(gridDim.x >> 3);
+  const int w = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  return w < total ? w : -1;
+}
+
+template <typename T>
+struct AttnFrag;
+template <>
+struct AttnFrag<bf16_t> {
+  u32x4 v;
+};
+template <>
+struct AttnFrag<float> {
+  f32x8 v;
+};
+
+__device__ __forceinline__ void mma32(f32x16& c, const AttnFrag<bf16_t>& a, const AttnFrag<bf16_t>& b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(attn_bf16x8, a.v), __builtin_bit_cast(attn_bf16x8, b.v), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma32(f32x16& c, const AttnFrag<float>& a, const AttnFrag<float>& b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// registers 8 s .. 8 s + 7 of a result tile as an operand.  bf16: probabilities (and the score gradients) are rounded to
+// the operand type here, as every bf16 product of the framework rounds its operands; sums and statistics stay fp32.
+template <typename T>
+__device__ __forceinline__ AttnFrag<T> pack_frag(const f32x16& s, int half);
+template <>
+__device__ __forceinline__ AttnFrag<bf16_t> pack_frag<bf16_t>(const f32x16& s, int half) {
+  f32x8 x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = s[8 * half + j];
+  AttnFrag<bf16_t> f;
+  f.v = __builtin_bit_cast(u32x4, __builtin_convertvector(x, attn_bf16x8));   // (four v_cvt_pk_bf16_f32)
+  return f;
+}
+template <>
+__device__ __forceinline__ AttnFrag<float> pack_frag<float>(const f32x16& s, int half) {
+  AttnFrag<float> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = s[8 * half + j];
+  return f;
+}
+
+// ---- tiles in LDS -------------------------------------------------------------------------------
+// Rows of DP elements at a pitch of a power of two; the 16-byte chunks of a row are permuted by XOR with a function of
+// the row chosen so that (a) eight lanes that read the same chunk of eight neighbouring rows (AttnRead::rows) and (b) sixteen
+// lanes that read a 32-byte piece of four neighbouring rows (cols, bf16) meet distinct LDS banks.
+template <typename T, int DP>
+struct AttnTile {
+  static constexpr int ES = sizeof(T);
+  static constexpr int PITCH = DP * ES <= 64 ? 64 : DP * ES <= 128 ? 128 : DP * ES <= 256 ? 256 : 512;
+  static constexpr int CPR = PITCH / 16;     // chunks per row
+  static constexpr int ROWS_1K = 1024 / PITCH;
+  static __device__ __forceinline__ int swz(int row) {
+    if (PITCH == 64) return (row >> 2) & 3;
+    if (PITCH == 128) return (((row >> 1) & 1) << 1) | ((row >> 2) & 1) | (((row >> 3) & 1) << 2);
+    if (PITCH == 256) return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8);
+    return ((row & 3) << 1) | ((row >> 2) & 1);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * PITCH + ((chunk ^ swz(row)) << 4); }
+};
+
+// rows(): operand fragment contracted along the tile's rows in memory: lane (l & 31, h) reads elements 16 ks + 8 h .. + 7
+// of row row0 + (l & 31).
+// cols(): operand fragment contracted over the tile's rows: lane (l & 31, h) gets column d0 + (l & 31) of rows
+// row0 + 8 (e / 4) + 4 h + e % 4, the order in which a result tile holds them.
+template <typename T, int DP>
+struct AttnRead;
+template <int DP>
+struct AttnRead<bf16_t, DP> {
+  typedef AttnTile<bf16_t, DP> Tile;
+  static __device__ __forceinline__ AttnFrag<bf16_t> rows(const char* tile, int row0, int ks, int lane) {
+    AttnFrag<bf16_t> f;
+    f.v = *reinterpret_cast<const u32x4*>(tile + Tile::at(row0 + (lane & 31), 2 * ks + (lane >> 5)));
+    return f;
+  }
+  static __device__ __forceinline__ AttnFrag<bf16_t> cols(const char* tile, int row0, int d0, int lane) {
+    // a group of 16 lanes reads a block of 4 rows x 16 columns, 8 bytes a lane, and receives it transposed
+    const int c0 = (d0 >> 3) + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    AttnFrag<bf16_t> f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = row0 + 8 * j + 4 * (lane >> 5) + ((lane & 15) >> 2);
+      const attn_s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) attn_s16x4*)(__attribute__((address_space(3))) char*)(tile + Tile::at(row, c0) +
+                                                                                                (lane & 1) * 8));
+      const u32x2 u = __builtin_bit_cast(u32x2, t);
+      f.v[2 * j] = u[0];
+      f.v[2 * j + 1] = u[1];
+    }
+    return f;
+  }
+};
+template <int DP>
+struct AttnRead<float, DP> {
+  typedef AttnTile<float, DP> Tile;
+  static __device__ __forceinline__ AttnFrag<float> rows(const char* tile, int row0, int ks, int lane) {
+    AttnFrag<float> f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(tile + Tile::at(row0 + (lane & 31), 4 * ks + 2 * (lane >> 5) + j));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[4 * j + e] = t[e];
+    }
+    return f;
+  }
+  static __device__ __forceinline__ AttnFrag<float> cols(const char* tile, int row0, int d0, int lane) {
+    const int d = d0 + (lane & 31);
+    AttnFrag<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = row0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+      f.v[e] = *reinterpret_cast<const float*>(tile + Tile::at(row, d >> 2) + (d & 3) * 4);
+    }
+    return f;
+  }
+};
+
+// Operand fragment straight from global memory: 8 elements from channel 16 ks + 8 h of one row (zeros past D and for
+// ok == false).  D is a multiple of 8, so a fragment is whole or absent.
+template <typename T>
+__device__ __forceinline__ AttnFrag<T> load_frag(const char* row, int ks, int h, int D, bool ok);
+template <>
+__device__ __forceinline__ AttnFrag<bf16_t> load_frag<bf16_t>(const char* row, int ks, int h, int D, bool ok) {
+  AttnFrag<bf16_t> f;
+  f.v = u32x4{0, 0, 0, 0};
+  const int d = 16 * ks + 8 * h;
+  if (ok && d < D) f.v = *reinterpret_cast<const u32x4*>(row + d * 2);
+  return f;
+}
+template <>
+__device__ __forceinline__ AttnFrag<float> load_frag<float>(const char* row, int ks, int h, int D, bool ok) {
+  AttnFrag<float> f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.v[e] = 0.f;
+  const int d = 16 * ks + 8 * h;
+  if (ok && d < D) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(row + d * 4), b = *reinterpret_cast<const f32x4*>(row + d * 4 + 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f.v[e] = a[e];
+      f.v[4 + e] = b[e];
+    }
+  }
+  return f;
+}
+
+// 4 consecutive channels of one row
+template <typename T>
+__device__ __forceinline__ void store4(char* row, int d, float a, float b, float c, float e);
+template <>
+__device__ __forceinline__ void store4<bf16_t>(char* row, int d, float a, float b, float c, float e) {
+  *reinterpret_cast<u32x2*>(row + d * 2) = u32x2{pack_bf16x2(a, b), pack_bf16x2(c, e)};
+}
+template <>
+__device__ __forceinline__ void store4<float>(char* row, int d, float a, float b, float c, float e) {
+  *reinterpret_cast<f32x4*>(row + d * 4) = f32x4{a, b, c, e};
+}
+
+// ---- LDS-DMA ------------------------------------------------------------------------------------
+// One 1-KiB piece: lane l's 16 bytes at buffer offset voff land at lds + 16 l; offsets from ATTN_OOB on write zeros.  In
+// assembly because the compiler puts a wait for every LDS-DMA in flight before the next LDS read, which would empty the
+// prefetch; the loops below wait themselves.  It has no register output.  s_nop 4: the resource may come from a
+// v_readfirstlane, which needs five wait states before a buffer instruction reads it (s_mov_b32 is one of them).
+__device__ __forceinline__ void dma_1k(const u32x4& rsrc, unsigned lds, unsigned voff) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(voff), "s"(rsrc)
+      : "memory");
+}
+// the same with 4 bytes a lane (256 B)
+__device__ __forceinline__ void dma_256(const u32x4& rsrc, unsigned lds, unsigned voff) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(voff), "s"(rsrc)
+      : "memory");
+}
+
+__device__ __forceinline__ u32x4 buffer_of(const char* base) {
+  const unsigned long long a = (unsigned long long)base;
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+  r[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu);
+  r[2] = ATTN_OOB;
+  r[3] = 0x00020000u;
+  return r;
+}
+
+__device__ __forceinline__ unsigned lds_addr(const char* p) {
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(attn_lds_ptr)p);
+}
+
+// Every LDS-DMA of this wavefront has landed and every LDS read has returned; then all wavefronts meet.  (The bare
+// barrier: the compiler's own would be the same here, the counts are spelled out because the DMA is in assembly.)
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// max over the two lanes that share a result column
+__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// host side, attn_fwd.hip
+int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);
+int launch_attn_dkv(AttnDev p, int dtype, hipStream_t st);   // attn_dkv.hip
+int launch_attn_dq(AttnDev p, int dtype, hipStream_t st);    // attn_dq.hip
+int launch_attn_sum(const float* part, long long part_stride, int parts, float scale, char* out, long long count, int dtype,
+                    hipStream_t st);
+int attn_dkv_splits(const AttnDev& p, int dtype);
+int attn_dq_splits(const AttnDev& p, int dtype);
+
+}  // namespace segk

@@ -1,0 +1,428 @@
+// Root-mean-square norm of every query and key head and the rotation of its channel pairs by position angles, in one
+// pass over the heads (several position axes: time, height, width), and its backward pass.
+//   r = (mean_d x_d^2 + eps)^-1/2,  y = w x r,  pair c turned by t = position[axis of c] * inv_freq[c]:
+//   (a, b) -> (a cos t - b sin t, a sin t + b cos t)
+// Memory-bound: every head is read once and written once (backward: x and dy read, dx written).
+#include "common.h"
+
+namespace segk {
+
+constexpr int ROT_THREADS = 256;
+constexpr int ROT_UNROLL = 4;        // heads in flight per group of lanes
+constexpr int ROT_MAX_BLOCKS = 2048; // of the backward pass: rows of weight-gradient partials
+
+struct RotSide {   // queries or keys
+  const char* x;
+  long long xn, xl, xh;     // byte strides
+  const char* dy;
+  long long dn, dl, dh;
+  char* y;                  // forward result / backward dx, contiguous
+  const float* w;
+  int heads;
+};
+
+struct RotDev {
+  RotSide s[2];
+  const char* pos;
+  long long pn, pl, pa;     // element strides
+  int pos_dtype, axes;
+  int first[4];             // first pair of each axis
+  const float* inv_freq;
+  float eps;
+  int norm, interleaved, pairs;
+  int N, L, D;
+  int heads_per, chunks;    // heads of one piece of work, pieces per token
+  float* part;              // [2 * D][blocks] weight-gradient partials
+  int blocks;
+};
+
+template <typename T>
+__device__ __forceinline__ void rot_load4(const char* p, float* v);
+template <>
+__device__ __forceinline__ void rot_load4<bf16_t>(const char* p, float* v) {
+  const u32x2 a = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    v[2 * e] = __uint_as_float(a[e] << 16);
+    v[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void rot_load4<float>(const char* p, float* v) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = a[e];
+}
+template <typename T>
+__device__ __forceinline__ void rot_store4(char* p, const float* v);
+template <>
+__device__ __forceinline__ void rot_store4<bf16_t>(char* p, const float* v) {
+  *reinterpret_cast<u32x2*>(p) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+template <>
+__device__ __forceinline__ void rot_store4<float>(char* p, const float* v) {
+  *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+}
+
+// A lane owns 4 pairs = 8 channels of a head: two runs of 4 channels at lo and hi.  Pairs of distant channels
+// (i, i + pairs): v[0..3] are the first, v[4..7] the second members; pairs of neighbours: runs of (a, b, a, b).
+// Channels past the rotated ones travel in neighbouring runs too, turned by nothing.
+struct RotLane {
+  int lo, hi;
+  bool live, split;
+  float c[4], s[4];
+};
+
+__device__ __forceinline__ RotLane rot_lane(const RotDev& p, int j) {
+  RotLane t;
+  t.live = j * 8 < p.D;
+  t.split = !p.interleaved && 4 * j < p.pairs;
+  t.lo = t.split ? 4 * j : 8 * j;
+  t.hi = t.split ? p.pairs + 4 * j : 8 * j + 4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t.c[e] = 1.f, t.s[e] = 0.f;
+  return t;
+}
+
+// cos and sin of this lane's 4 pairs.  The angle is formed and reduced to half turns in fp64 (a position in the hundred
+// thousands times a frequency loses its fraction in fp32), the rest in fp32.
+__device__ __forceinline__ void rot_angles(const RotDev& p, int j, int n, int l, RotLane& t) {
+  if (4 * j >= p.pairs) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = 4 * j + e;
+    int axis = 0;
+#pragma unroll
+    for (int a = 1; a < 4; ++a) axis = a < p.axes && c >= p.first[a] ? a : axis;
+    const long long at = n * p.pn + l * p.pl + axis * p.pa;
+    double x;
+    if (p.pos_dtype == 0) x = ((const int*)p.pos)[at];
+    else if (p.pos_dtype == 1) x = (double)((const long long*)p.pos)[at];
+    else x = ((const float*)p.pos)[at];
+    const double half_turns = x * (double)p.inv_freq[c] * 0.31830988618379067154;
+    const float f = (float)(half_turns - 2.0 * rint(half_turns * 0.5));
+    sincospif(f, &t.s[e], &t.c[e]);
+  }
+}
+
+// forward turn (sign +1) or its inverse (-1)
+__device__ __forceinline__ void rot_turn(const RotLane& t, float sign, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = t.split ? v[e] : v[2 * e], b = t.split ? v[4 + e] : v[2 * e + 1];
+    const float s = sign * t.s[e];
+    const float x = a * t.c[e] - b * s, y = a * s + b * t.c[e];
+    // (a lane is of one kind throughout; both forms are written by selects)
+    if (t.split) {
+      v[e] = x;
+      v[4 + e] = y;
+    } else {
+      v[2 * e] = x;
+      v[2 * e + 1] = y;
+    }
+  }
+}
+
+template <int LPH>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LPH >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// A group of LPH lanes (D / 8 rounded up to a power of two) takes one token and `heads_per` of its heads: the angles are
+// computed once for all of them.
+template <typename T, int LPH>
+__global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_kernel(const RotDev p) {
+  const int j = threadIdx.x % LPH;
+  const long long work = (long long)blockIdx.x * (ROT_THREADS / LPH) + threadIdx.x / LPH;
+  const long long tokens = (long long)p.N * p.L;
+  if (work >= tokens * p.chunks) return;
+  const long long nl = work / p.chunks;
+  const int chunk = (int)(work - nl * p.chunks);
+  const int n = (int)(nl / p.L), l = (int)(nl - (long long)n * p.L);
+  RotLane t = rot_lane(p, j);
+  rot_angles(p, j, n, l, t);
+  float w[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[q][e] = t.live && p.s[q].w ? p.s[q].w[(e < 4 ? t.lo : t.hi - 4) + e] : 1.f;
+  const int total = p.s[0].heads + p.s[1].heads;
+  const int h0 = chunk * p.heads_per, h1 = min(h0 + p.heads_per, total);
+  const float inv_d = 1.f / (float)p.D;
+  for (int hb = h0; hb < h1; hb += ROT_UNROLL) {
+    float v[ROT_UNROLL][8];
+#pragma unroll
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      const int hh = hb + u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+      if (hh < h1 && t.live) {
+        const bool key = hh >= p.s[0].heads;
+        const RotSide& sd = p.s[key ? 1 : 0];
+        const char* src = sd.x + n * sd.xn + l * sd.xl + (hh - (key ? p.s[0].heads : 0)) * sd.xh;
+        rot_load4<T>(src + t.lo * (int)sizeof(T), v[u]);
+        rot_load4<T>(src + t.hi * (int)sizeof(T), v[u] + 4);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      const int hh = hb + u;
+      if (hh >= h1) break;
+      const bool key = hh >= p.s[0].heads;
+      const RotSide& sd = p.s[key ? 1 : 0];
+      if (p.norm) {
+        float q = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q = fmaf(v[u][e], v[u][e], q);
+        const float r = rsqrtf(fmaf(group_sum<LPH>(q), inv_d, p.eps));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[u][e] *= r * (key ? w[1][e] : w[0][e]);
+      }
+      rot_turn(t, 1.f, v[u]);
+      if (t.live) {
+        char* dst = sd.y + ((nl * sd.heads + (hh - (key ? p.s[0].heads : 0))) * p.D) * (int)sizeof(T);
+        rot_store4<T>(dst + t.lo * (int)sizeof(T), v[u]);
+        rot_store4<T>(dst + t.hi * (int)sizeof(T), v[u] + 4);
+      }
+    }
+  }
+}
+
+// Backward.  dn = dy turned back; dw = sum dn x r; g = w dn; dx = r (g - x r mean(g x r)).  Weight gradients: each lane
+// sums its channels over its work in fp32, the groups of a workgroup are joined in LDS in order, one partial per
+// workgroup and channel, joined in fp64 by the second kernel: no atomics, a fixed order.
+template <typename T, int LPH>
+__global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const RotDev p) {
+  __shared__ float red[ROT_THREADS][17];   // (17: a column walk meets distinct banks)
+  constexpr int GROUPS = ROT_THREADS / LPH;
+  const int j = threadIdx.x % LPH;
+  const long long tokens = (long long)p.N * p.L;
+  RotLane t = rot_lane(p, j);
+  float w[2][8], dw[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[q][e] = t.live && p.s[q].w ? p.s[q].w[(e < 4 ? t.lo : t.hi - 4) + e] : 1.f;
+      dw[q][e] = 0.f;
+    }
+  const int total = p.s[0].heads + p.s[1].heads;
+  const float inv_d = 1.f / (float)p.D;
+  for (long long work = (long long)blockIdx.x * GROUPS + threadIdx.x / LPH; work < tokens * p.chunks;
+       work += (long long)gridDim.x * GROUPS) {
+    const long long nl = work / p.chunks;
+    const int chunk = (int)(work - nl * p.chunks);
+    const int n = (int)(nl / p.L), l = (int)(nl - (long long)n * p.L);
+    rot_angles(p, j, n, l, t);
+    const int h0 = chunk * p.heads_per, h1 = min(h0 + p.heads_per, total);
+    for (int hb = h0; hb < h1; hb += 2) {
+      float v[2][8], g[2][8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int hh = hb + u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] = 0.f;
+        if (hh < h1 && t.live) {
+          const bool key = hh >= p.s[0].heads;
+          const RotSide& sd = p.s[key ? 1 : 0];
+          const int hl = hh - (key ? p.s[0].heads : 0);
+          const char* dy = sd.dy + n * sd.dn + l * sd.dl + hl * sd.dh;
+          rot_load4<T>(dy + t.lo * (int)sizeof(T), g[u]);
+          rot_load4<T>(dy + t.hi * (int)sizeof(T), g[u] + 4);
+          if (p.norm) {
+            const char* src = sd.x + n * sd.xn + l * sd.xl + hl * sd.xh;
+            rot_load4<T>(src + t.lo * (int)sizeof(T), v[u]);
+            rot_load4<T>(src + t.hi * (int)sizeof(T), v[u] + 4);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int hh = hb + u;
+        if (hh >= h1) break;
+        const bool key = hh >= p.s[0].heads;
+        const RotSide& sd = p.s[key ? 1 : 0];
+        rot_turn(t, -1.f, g[u]);
+        if (p.norm) {
+          float q = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q = fmaf(v[u][e], v[u][e], q);
+          const float r = rsqrtf(fmaf(group_sum<LPH>(q), inv_d, p.eps));
+          float dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[u][e] *= r;
+            const float add = g[u][e] * v[u][e];
+            dw[0][e] += key ? 0.f : add;
+            dw[1][e] += key ? add : 0.f;
+            g[u][e] *= key ? w[1][e] : w[0][e];
+            dot = fmaf(g[u][e], v[u][e], dot);
+          }
+          dot = group_sum<LPH>(dot) * inv_d;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[u][e] = r * (g[u][e] - v[u][e] * dot);
+        }
+        if (t.live) {
+          char* dst = sd.y + ((nl * sd.heads + (hh - (key ? p.s[0].heads : 0))) * p.D) * (int)sizeof(T);
+          rot_store4<T>(dst + t.lo * (int)sizeof(T), g[u]);
+          rot_store4<T>(dst + t.hi * (int)sizeof(T), g[u] + 4);
+        }
+      }
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[threadIdx.x][q * 8 + e] = dw[q][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < LPH * 16; i += ROT_THREADS) {
+    const int jj = i % LPH, slot = i / LPH;
+    float s = 0.f;
+    for (int g = 0; g < GROUPS; ++g) s += red[g * LPH + jj][slot];
+    const RotLane o = rot_lane(p, jj);
+    const int e = slot & 7;
+    const int ch = (e < 4 ? o.lo : o.hi - 4) + e;
+    if (o.live) p.part[((long long)(slot >> 3) * p.D + ch) * p.blocks + blockIdx.x] = s;
+  }
+}
+
+// one wavefront per channel: dq_weight[0 .. D), dk_weight[0 .. D)
+__global__ __launch_bounds__(64) void qk_norm_weight_grad_kernel(const float* __restrict__ part, int blocks, int D, float* __restrict__ dqw,
+                                                                 float* __restrict__ dkw) {
+  const int ch = blockIdx.x;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < blocks; i += 64) s += (double)part[(long long)ch * blocks + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  float* dst = ch < D ? dqw : dkw;
+  if (threadIdx.x == 0 && dst) dst[ch < D ? ch : ch - D] = (float)s;
+}
+
+static int rot_lanes(int D) {
+  int l = 1;
+  while (l * 8 < D) l *= 2;
+  return l;
+}
+
+static int rot_fill(const segk_qk_norm_rotary_args* a, RotDev* p, bool backward) {
+  SEGK_REQUIRE(a && valid_dtype(a->dtype), "qk_norm_rotary: null arguments or bad dtype");
+  SEGK_REQUIRE(a->N > 0 && a->L > 0 && a->Hq > 0 && a->Hk >= 0 && (long long)a->N * a->L < 0x7fffffffLL,
+               "qk_norm_rotary: bad shape N=%d L=%d Hq=%d Hk=%d", a->N, a->L, a->Hq, a->Hk);
+  SEGK_UNSUPPORTED(a->D > 0 && a->D % 8 == 0 && a->D <= 256, "qk_norm_rotary: head size %d is not a multiple of 8 up to 256", a->D);
+  SEGK_REQUIRE(a->axes >= 1 && a->axes <= 4 && a->positions && a->inv_freq && a->pos_dtype >= 0 && a->pos_dtype <= 2,
+               "qk_norm_rotary: positions of 1 to 4 axes and their frequencies are needed");
+  int pairs = 0;
+  for (int i = 0; i < 4; ++i) {
+    p->first[i] = pairs;
+    if (i < a->axes) {
+      SEGK_REQUIRE(a->section[i] >= 0 && a->section[i] <= 128, "qk_norm_rotary: section of %d pairs", a->section[i]);
+      pairs += a->section[i];
+    }
+  }
+  SEGK_UNSUPPORTED(pairs > 0 && pairs % 4 == 0 && 2 * pairs <= a->D,
+                   "qk_norm_rotary: %d rotated pairs for a head size of %d (a multiple of 4 up to half of it)", pairs, a->D);
+  SEGK_REQUIRE(!a->norm || a->eps >= 0.f, "qk_norm_rotary: negative eps");
+  SEGK_REQUIRE(a->norm || (!a->q_weight && !a->k_weight), "qk_norm_rotary: weights belong to the norm");
+  const int es = dtype_size(a->dtype), e8 = 16 / es;
+  for (int i = 0; i < 2; ++i) {
+    RotSide& s = p->s[i];
+    const segk_attention_view& x = i ? a->k : a->q;
+    const segk_attention_view& g = i ? a->dk : a->dq;
+    s.heads = i ? a->Hk : a->Hq;
+    s.x = (const char*)x.p, s.xn = x.n * es, s.xl = x.l * es, s.xh = x.h * es;
+    s.dy = (const char*)g.p, s.dn = g.n * es, s.dl = g.l * es, s.dh = g.h * es;
+    s.y = (char*)(i ? a->k_out : a->q_out);
+    s.w = i ? a->k_weight : a->q_weight;
+    if (s.heads == 0) continue;
+    SEGK_REQUIRE(s.x && s.y && (!backward || s.dy), "qk_norm_rotary: null operand");
+    SEGK_REQUIRE((((uintptr_t)s.x | (uintptr_t)s.y | (backward ? (uintptr_t)s.dy : 0)) & 15) == 0 && x.n % e8 == 0 && x.l % e8 == 0 &&
+                     x.h % e8 == 0 && (!backward || (g.n % e8 == 0 && g.l % e8 == 0 && g.h % e8 == 0)),
+                 "qk_norm_rotary: operands need 16-byte aligned pointers and strides that are multiples of 16 bytes");
+  }
+  p->pos = (const char*)a->positions, p->pn = a->pos_n, p->pl = a->pos_l, p->pa = a->pos_a;
+  p->pos_dtype = a->pos_dtype, p->axes = a->axes, p->inv_freq = a->inv_freq;
+  p->eps = a->eps, p->norm = a->norm != 0, p->interleaved = a->interleaved != 0, p->pairs = pairs;
+  p->N = a->N, p->L = a->L, p->D = a->D;
+  // Heads of a token that one group of lanes takes: all of them (the angles are computed once) as long as that leaves
+  // 1024 threads for every CU, else fewer, down to one: a single token then spreads over 20 groups, not one.
+  const int lanes = rot_lanes(a->D), total = a->Hq + a->Hk;
+  const long long threads = (long long)a->N * a->L * total * lanes;
+  long long per = threads / (256 * 1024);
+  per = per < 1 ? 1 : per > total ? total : per;
+  if (per > 4) per = (per + 3) / 4 * 4;
+  p->heads_per = (int)per;
+  p->chunks = ceil_div(total, p->heads_per);
+  p->part = nullptr;
+  p->blocks = 0;
+  return SEGK_OK;
+}
+
+static long long rot_blocks(const RotDev& p) {
+  const int per = ROT_THREADS / rot_lanes(p.D);
+  return ((long long)p.N * p.L * p.chunks + per - 1) / per;
+}
+static int rot_bwd_blocks(const RotDev& p) {
+  const long long b = rot_blocks(p);
+  return (int)(b < ROT_MAX_BLOCKS ? b : ROT_MAX_BLOCKS);
+}
+
+}  // namespace segk
+
+using namespace segk;
+
+#define ROT_LAUNCH(kernel, grid)                                                            \
+  switch (rot_lanes(p.D)) {                                                                 \
+    case 1: kernel<T, 1><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
+    case 2: kernel<T, 2><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
+    case 4: kernel<T, 4><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
+    case 8: kernel<T, 8><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
+    case 16: kernel<T, 16><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;             \
+    default: kernel<T, 32><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;             \
+  }
+
+extern "C" int segk_qk_norm_rotary(const segk_qk_norm_rotary_args* a, segk_stream_t stream) {
+  RotDev p;
+  const int rc = rot_fill(a, &p, false);
+  if (rc != SEGK_OK) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  const long long grid = rot_blocks(p);
+  SEGK_UNSUPPORTED(grid < 0x7fffffffLL, "qk_norm_rotary: too many heads");
+  SEGK_DISPATCH_DTYPE(a->dtype, T, ROT_LAUNCH(qk_norm_rotary_kernel, grid));
+  SEGK_CHECK_LAUNCH("qk_norm_rotary");
+  return SEGK_OK;
+}
+
+extern "C" long long segk_qk_norm_rotary_bwd_workspace(const segk_qk_norm_rotary_args* a) {
+  RotDev p;
+  const int rc = rot_fill(a, &p, true);
+  if (rc != SEGK_OK) return rc;
+  return a->dq_weight || a->dk_weight ? (long long)rot_bwd_blocks(p) * 2 * p.D * 4 : 0;
+}
+
+extern "C" int segk_qk_norm_rotary_bwd(const segk_qk_norm_rotary_args* a, segk_stream_t stream) {
+  RotDev p;
+  const int rc = rot_fill(a, &p, true);
+  if (rc != SEGK_OK) return rc;
+  SEGK_REQUIRE(p.norm || (!a->dq_weight && !a->dk_weight), "qk_norm_rotary_bwd: weights belong to the norm");
+  hipStream_t st = (hipStream_t)stream;
+  p.blocks = rot_bwd_blocks(p);
+  if (a->dq_weight || a->dk_weight) {
+    SEGK_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0, "qk_norm_rotary_bwd: workspace missing or not 16-byte aligned");
+    const long long need = (long long)p.blocks * 2 * p.D * 4;
+    if (a->workspace_bytes < need) {
+      set_error("qk_norm_rotary_bwd: workspace of %lld bytes, needs %lld", a->workspace_bytes, need);
+      return SEGK_WORKSPACE_TOO_SMALL;
+    }
+    p.part = (float*)a->workspace;
+  }
+  SEGK_DISPATCH_DTYPE(a->dtype, T, ROT_LAUNCH(qk_norm_rotary_bwd_kernel, p.blocks));
+  SEGK_CHECK_LAUNCH("qk_norm_rotary_bwd");
+  if (p.part) {
+    qk_norm_weight_grad_kernel<<<2 * p.D, 64, 0, st>>>(p.part, p.blocks, p.D, a->dq_weight, a->dk_weight);
+    SEGK_CHECK_LAUNCH("qk_norm_rotary_bwd weights");
+  }
+  return SEGK_OK;
+}

@@ -1314,3 +1314,114 @@ class CAMFunction(torch.autograd.Function):
             ops.lincomb(dxp, [(dxa, 1.0, None), (gp, 1.0, None)])
             dx = grad_like(x, dxp, N, H, W)
         return dx, dgamma
+
+
+# ------------------------------------------------------ multi-head attention ----
+def _attention_operand(t):
+    """The tensor itself where the kernels can read it, else a contiguous copy."""
+    return t if ops.attention_operand_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+class AttentionFunction(torch.autograd.Function):
+    """Multi-head attention with fused softmax; the backward pass computes the probabilities again from lse."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, key_mask, causal, scale):
+        q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, mask, key_mask)
+        ctx.how = (causal, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse, mask, key_mask = ctx.saved_tensors
+        causal, scale = ctx.how
+        need = ctx.needs_input_grad
+        dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, _attention_operand(g), scale, causal, mask, key_mask,
+                                       need_dq=need[0], need_dkv=need[1] or need[2])
+        return dq, (dk if need[1] else None), (dv if need[2] else None), None, None, None, None
+
+
+def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
+    """Multi-head attention, the many-headed form of PAMFunction's single-head one (modeling/damm_cam_pam.py:22-48), in
+    one pass over the keys: no [Lq, Lk] matrix is stored.
+
+    q [N, Lq, Hq, D]; k, v [N, Lk, Hk, D] (float32 or bfloat16, D a multiple of 8 up to 128; query head h reads
+    key / value head h // (Hq // Hk)) -> [N, Lq, Hq, D].  Views are read in place when their channels are contiguous and
+    their rows 16-byte aligned (slices of one projection's output are), copied otherwise.
+      mask      bool, broadcastable to [N, Hq, Lq, Lk], True = open.  A closed pair has probability zero; its key and value
+                are still read and must be finite.
+      key_mask  bool [N, Lk], True = open (e.g. the pixels that are not padding).  A closed key is not read.
+      causal    key j is open to token i for j <= i + Lk - Lq
+      scale     of the scores, positive; default D ** -0.5
+    A query without an open key gives zeros, and no gradient.  Differentiable once with respect to q, k and v."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("attention takes [N, L, heads, D] tensors, got %s, %s, %s"
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    scale = float(q.shape[3]) ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return AttentionFunction.apply(q, k, v, mask, key_mask, bool(causal), scale)
+    q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask)
+    return out
+
+
+class QkNormRotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved):
+        q, k = _attention_operand(q), (None if k is None else _attention_operand(k))
+        wq, wk = _fp32_weight(q_weight), _fp32_weight(k_weight)
+        res = ops.qk_norm_rotary_fwd(q, k, wq, wk, positions, inv_freq, sections, eps, interleaved)
+        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
+        ctx.how = (sections, eps, interleaved)
+        ctx.weight_dtypes = (None if q_weight is None else q_weight.dtype, None if k_weight is None else k_weight.dtype)
+        return res if k is not None else res[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk=None):
+        q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gq = _attention_operand(gq)
+        gk = None if k is None else _attention_operand(gk)
+        dq, dk, dwq, dwk = ops.qk_norm_rotary_bwd(gq, gk, q, k, wq, wk, positions, inv_freq, *ctx.how,
+                                                  need_weights=need[2:4])
+        dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.weight_dtypes))
+        return (dq if need[0] else None), (dk if need[1] else None), dwq, dwk, None, None, None, None, None
+
+
+def _fp32_weight(w):
+    return None if w is None else w.detach().float().contiguous()
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, interleaved=False):
+    """What stands between the projections and `attention`: every head of the queries and keys is normalised and turned
+    by its token's position, in one pass.
+
+    q [N, L, Hq, D], k [N, L, Hk, D] or None (queries alone), float32 or bfloat16, D a multiple of 8 up to 256 -> (q', k')
+    contiguous (q' alone without k).  For every head x:
+        y = weight * x * (mean(x^2) + eps)^-1/2        weight [D] or None; eps None: no norm and no weights
+        pair c of y turned by the angle positions[..., axis of c] * inv_freq[c]: (a, b) -> (a cos - b sin, a sin + b cos)
+      positions    [L, axes] or [N, L, axes], int32, int64 or float32, 1 to 4 axes (row and column of a pixel; time, height
+                   and width of a clip)
+      inv_freq     float32, one frequency per rotated pair; a multiple of 4 pairs, at most D / 2
+      sections     how many of the pairs, in order, turn by each axis; default: equal shares
+      interleaved  pairs are channels (2c, 2c + 1) instead of (c, c + pairs); channels past the pairs stay as normalised
+    Angles are formed in 64 bits.  Differentiable once with respect to q, k and the weights."""
+    args = (positions, inv_freq, None if sections is None else tuple(int(z) for z in sections),
+            None if eps is None else float(eps), bool(interleaved))
+    tensors = (q, k, q_weight, k_weight)
+    if positions.requires_grad or inv_freq.requires_grad:
+        raise ValueError("positions and inv_freq get no gradient here")
+    for t, name in ((q, "q"), (k, "k")):
+        if t is not None and t.dim() != 4:
+            raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return QkNormRotaryFunction.apply(*tensors, *args)
+    res = ops.qk_norm_rotary_fwd(_attention_operand(q), None if k is None else _attention_operand(k),
+                                 _fp32_weight(q_weight), _fp32_weight(k_weight), *args)
+    return res if k is not None else res[0]
