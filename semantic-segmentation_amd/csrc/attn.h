@@ -272,6 +272,107 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Stages tiles of KT keys and their values: piece i of a wavefront is rows st_row + i * (4096 / PITCH) of a tile.
+template <typename T, int DP>
+struct AttnStage {
+  typedef AttnTile<T, DP> Tile;
+  int row, chunk;
+  bool ok;
+  unsigned k_step, v_step, lds0;
+  const char *kbase, *vbase;
+  __device__ __forceinline__ AttnStage(const AttnDev& p, int n, int hk, int wave, int lane, const char* smem) {
+    const int lin = wave * 1024 + lane * 16;
+    row = lin / Tile::PITCH;
+    chunk = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(row);     // (4096 / PITCH is a period of swz)
+    ok = chunk * 16 < p.D * (int)sizeof(T);
+    k_step = (unsigned)(p.k.l * (int)sizeof(T)), v_step = (unsigned)(p.v.l * (int)sizeof(T));
+    kbase = p.k.p + ((long long)n * p.k.n + (long long)hk * p.k.h) * (int)sizeof(T);
+    vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
+    lds0 = lds_addr(smem) + wave * 1024;
+  }
+  // bits: the tile's open keys (MASKED).  A closed key is not read: whatever its memory holds, zeros arrive.
+  template <int KT, bool MASKED>
+  __device__ __forceinline__ void keys(const AttnDev& p, int key0, int buf, const unsigned long long* bits) const {
+    constexpr int TILE_B = KT * Tile::PITCH;
+    const u32x4 kr = buffer_of(kbase + (long long)key0 * k_step), vr = buffer_of(vbase + (long long)key0 * v_step);
+#pragma unroll
+    for (int i = 0; i < TILE_B / 4096; ++i) {
+      const int x = row + i * (4096 / Tile::PITCH);
+      bool in = ok && key0 + x < p.Lk;
+      if (MASKED) in = in && ((bits[i * (4096 / Tile::PITCH) >> 6] >> (x & 63)) & 1);
+      const unsigned lds = lds0 + buf * (2 * TILE_B) + i * 4096;
+      dma_1k(kr, lds, in ? x * k_step + chunk * 16 : ATTN_OOB);
+      dma_1k(vr, lds + TILE_B, in ? x * v_step + chunk * 16 : ATTN_OOB);
+    }
+  }
+};
+
+// Key mask of a tile of KT keys as one bit per key, the same in every wavefront: load() asks for a tile's bytes, next()
+// turns the bytes asked for last into bits.  Without a mask all bits are set.
+template <int KT>
+struct AttnKeyMask {
+  const unsigned char* mask;
+  long long step;
+  int Lk, lane;
+  unsigned char raw[KT / 64];
+  unsigned long long bits[KT / 64];
+  __device__ __forceinline__ AttnKeyMask(const unsigned char* m, long long s, int lk, int ln) : mask(m), step(s), Lk(lk), lane(ln) {
+#pragma unroll
+    for (int i = 0; i < KT / 64; ++i) {
+      raw[i] = 1;
+      bits[i] = ~0ULL;
+    }
+  }
+  __device__ __forceinline__ void load(int key0) {
+    if (!mask) return;
+#pragma unroll
+    for (int i = 0; i < KT / 64; ++i) {
+      const int j = key0 + i * 64 + lane;
+      raw[i] = j < Lk ? mask[j * step] : 0;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (!mask) return;
+#pragma unroll
+    for (int i = 0; i < KT / 64; ++i) bits[i] = __ballot(raw[i] != 0);
+  }
+  __device__ __forceinline__ unsigned word(int key) const { return (unsigned)(bits[KT == 64 ? 0 : key >> 6] >> (key & 63)); }
+};
+
+// Pair mask of one row against 32 * NKB keys: byte e of w[kb][g] belongs to key first + kb * 32 + 8 g + e of the tile, the
+// order of a result tile's registers.
+template <int NKB>
+struct AttnPairMask {
+  const unsigned char* row;
+  long long step;
+  int Lk, first;
+  unsigned w[NKB][4];
+  __device__ __forceinline__ AttnPairMask(const unsigned char* m, long long s, int lk, int f) : row(m), step(s), Lk(lk), first(f) {}
+  __device__ __forceinline__ void load(int key0) {
+    if (!row) return;
+    const int j0 = key0 + first;
+    if (step == 1 && key0 + (NKB == 1 ? 128 : 64) <= Lk) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[kb][g], row + j0 + kb * 32 + 8 * g, 4);
+      return;
+    }
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        unsigned x = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + kb * 32 + 8 * g + e;
+          if (j < Lk && row[j * step]) x |= 0xffu << (8 * e);
+        }
+        w[kb][g] = x;
+      }
+  }
+};
+
 // max over the two lanes that share a result column
 __device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 __device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32, 64); }
@@ -280,6 +381,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // host side, attn_fwd.hip
 int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);
+bool attn_few(const AttnDev& p, int dtype);
 int launch_attn_dkv(AttnDev p, int dtype, hipStream_t st);   // attn_dkv.hip
 int launch_attn_dq(AttnDev p, int dtype, hipStream_t st);    // attn_dq.hip
 int launch_attn_sum(const float* part, long long part_stride, int parts, float scale, char* out, long long count, int dtype,

@@ -103,6 +103,16 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       const int row0 = t * QT + rb * 32;
+      if (row0 >= p.R) break;
+      unsigned char open[16];
+      if (MASKED && mkey) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = min(row0 + 8 * (i >> 2) + 4 * h + (i & 3), p.R - 1);
+          const int tok = div_g(p, r);
+          open[i] = mkey[(long long)(r - tok * p.G) * p.m_h + (long long)tok * p.m_q];
+        }
+      }
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(qt, rb * 32, ks, lane), kf[ks]);
@@ -121,18 +131,17 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = exp2_fast(fmaf(s[i], p.scale_log2, -ls[i]));
-      const bool diagonal = p.causal && key_wg + 127 > div_g(p, min(row0, p.R - 1)) + p.off;
-      if (MASKED || diagonal) {
+      // closed pairs (a closed key's products are those of zeros; the padding rows' lse is +inf)
+      if (p.causal && key_wg + 127 > div_g(p, row0) + p.off) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int r = row0 + 8 * (i >> 2) + 4 * h + (i & 3);
-          bool open = key_ok && r < p.R;
-          const int tok = div_g(p, r);
-          if (p.causal) open = open && key <= tok + p.off;
-          if (MASKED && mkey && open) open = mkey[(long long)(r - tok * p.G) * p.m_h + (long long)tok * p.m_q] != 0;
-          s[i] = open ? s[i] : 0.f;
-          dp[i] = open ? dp[i] : 0.f;
+          s[i] = key <= div_g(p, r) + p.off ? s[i] : 0.f;
         }
+      }
+      if (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = key_ok && (!mkey || open[i] != 0) ? s[i] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - dl[i]);

@@ -5,17 +5,15 @@
 
 namespace segk {
 
-constexpr int DQ_KT = 64;
-
-// As the forward kernel: 4 wavefronts of 32 packed rows, tiles of 64 keys, a lane owns one query.
+// As the forward kernel (attn_fwd.hip), FEW and MASKED included: a lane owns one query,
 //   S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
-template <typename T, int DP, bool MASKED>
+template <typename T, int DP, bool FEW, bool MASKED>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2)) void attn_dq_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
+  constexpr int KT = FEW ? 128 : 64, NKB = FEW ? 1 : 2;
   constexpr int KS = DP / 16, DB = DP / 32;
-  constexpr int TILE_B = DQ_KT * Tile::PITCH;
-  constexpr int NP = TILE_B / 4096;
+  constexpr int TILE_B = KT * Tile::PITCH;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -27,16 +25,17 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
   const int tile = w % p.tiles;
   w /= p.tiles;
   const int hk = w % p.Hk, n = w / p.Hk;
-  const int row0 = tile * 128;
+  const int row0 = FEW ? 0 : tile * 128 + wave * 32;
+  const bool idle = row0 >= p.R;
 
-  const int last_row = min(row0 + 128, p.R) - 1;
+  const int last_row = min(FEW ? 32 : tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
-  const int all_steps = (k_end + DQ_KT - 1) / DQ_KT;
+  const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + p.splits - 1) / p.splits;
   const int t0 = min(split * per, all_steps), t1 = min(t0 + per, all_steps);
 
-  const int r = row0 + wave * 32 + l31;
+  const int r = row0 + l31;
   const bool row_in = r < p.R;
   const int rr = row_in ? r : 0;
   const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
@@ -54,50 +53,64 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       gf[ks] = load_frag<T>(gs, ks, h, p.D, row_ok);
     }
   }
-  const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0 + wave * 32, p.R - 1)));
-  const unsigned char* const mrow =
-      MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr;
+  const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0, p.R - 1)));
 
-  const int lin = wave * 1024 + lane * 16;
-  const int st_row = lin / Tile::PITCH;
-  const int st_chunk = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(st_row);
-  const bool st_ok = st_chunk * 16 < p.D * (int)sizeof(T);
-  const unsigned k_step_b = (unsigned)(p.k.l * (int)sizeof(T)), v_step_b = (unsigned)(p.v.l * (int)sizeof(T));
-  const char* const kbase = p.k.p + ((long long)n * p.k.n + (long long)hk * p.k.h) * (int)sizeof(T);
-  const char* const vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
-  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
-  const unsigned lds0 = lds_addr(smem) + wave * 1024;
-  auto stage = [&](int t, int buf) {
-    const int key0 = t * DQ_KT;
-    const u32x4 kr = buffer_of(kbase + (long long)key0 * k_step_b);
-    const u32x4 vr = buffer_of(vbase + (long long)key0 * v_step_b);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int row = st_row + i * (4096 / Tile::PITCH);
-      bool ok = st_ok && key0 + row < p.Lk;
-      if (MASKED && kmask && ok) ok = kmask[(long long)(key0 + row) * p.km_k] != 0;
-      const unsigned lds = lds0 + buf * (2 * TILE_B) + i * 4096;
-      dma_1k(kr, lds, ok ? row * k_step_b + st_chunk * 16 : ATTN_OOB);
-      dma_1k(vr, lds + TILE_B, ok ? row * v_step_b + st_chunk * 16 : ATTN_OOB);
-    }
-  };
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
+  AttnPairMask<NKB> pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k,
+                       p.Lk, (FEW ? wave * 32 : 0) + 4 * h);
 
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = zero16();
 
-  if (t0 < t1) stage(t0, 0);
+  if (t0 < t1) {
+    if (MASKED) {
+      km.load(t0 * KT);
+      km.next();
+      km.load((t0 + 1) * KT);
+      pm.load(t0 * KT);
+    }
+    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     tile_barrier();
-    if (t + 1 < t1) stage(t + 1, buf ^ 1);
-    const char* kt = smem + buf * (2 * TILE_B);
-    const char* vt = kt + TILE_B;
-    const int key0 = t * DQ_KT;
-    const bool ragged = key0 + DQ_KT > p.Lk || (p.causal && key0 + DQ_KT - 1 > wave_tok0 + p.off);
-    const int lim = p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1;
+    const int key0 = t * KT + (FEW ? wave * 32 : 0);
+    unsigned kw[NKB], pw[NKB][4];
+    bool dead = idle;
+    if (MASKED) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < NKB; ++kb) {
+        kw[kb] = km.word((FEW ? wave * 32 : 0) + kb * 32);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) pw[kb][g] = pm.w[kb][g];
+      }
+      dead = dead || !(NKB == 2 ? kw[0] | kw[NKB - 1] : kw[0]);
+      if (pm.row && !dead) {
+        unsigned some = 0;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) some |= pw[kb][g];
+        dead = !__any(row_ok && some != 0);
+      }
+    }
+    if (t + 1 < t1) {
+      if (MASKED) {
+        km.next();
+        km.load((t + 2) * KT);
+        pm.load((t + 1) * KT);
+      }
+      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    }
+    if (dead) continue;
+    const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
+    const char* vt = kt + TILE_B;
+    const bool ragged = key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off);
+    const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
@@ -105,16 +118,19 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(vt, kb * 32, ks, lane), gf[ks]);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
-      if (MASKED || ragged) {
+      if (ragged) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = key0 + kb * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-          bool open = j <= lim;
-          if (MASKED && open) {
-            if (kmask) open = kmask[(long long)j * p.km_k] != 0;
-            if (mrow && open) open = mrow[(long long)j * p.m_k] != 0;
-          }
-          dp[i] = open ? dp[i] : 0.f;
+        for (int i = 0; i < 16; ++i) dp[i] = kb * 32 + 8 * (i >> 2) + (i & 3) <= lim ? dp[i] : 0.f;
+      }
+      if (MASKED) {
+        if (km.mask) {
+          const unsigned x = kw[kb] >> (4 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? dp[i] : 0.f;
+        }
+        if (pm.row) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = pw[kb][i >> 2] & (0xffu << (8 * (i & 3))) ? dp[i] : 0.f;
         }
       }
 #pragma unroll
@@ -126,6 +142,34 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
     }
   }
 
+  if constexpr (FEW) {
+    constexpr int LD = DP + 4;
+    float* const so = reinterpret_cast<float*>(smem);
+    tile_barrier();
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
+            f32x4{dq[db][i], dq[db][i + 1], dq[db][i + 2], dq[db][i + 3]};
+    tile_barrier();
+    for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
+      const int row = x / (DP / 4), d = x % (DP / 4) * 4;
+      if (row >= p.R || d >= p.D) continue;
+      f32x4 v = *reinterpret_cast<const f32x4*>(so + row * LD + d);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + row) * LD + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += y[e];
+      }
+      const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
+      const long long at = (((long long)n * p.Lq + tk) * p.Hq + hd) * p.D;
+      if (p.splits == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
+      else store4<float>((char*)(p.part + (long long)split * p.N * p.Lq * p.Hq * p.D + at), d, v[0], v[1], v[2], v[3]);
+    }
+    return;
+  }
   if (!row_in) return;
   const long long at = (((long long)n * p.Lq + tok) * p.Hq + head) * p.D;
   if (p.splits == 1) {
@@ -150,20 +194,21 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
 }
 
 int attn_dq_splits(const AttnDev& p, int dtype) {
-  const long long blocks = (long long)ceil_div(p.R, 128) * p.N * p.Hk;
-  const int steps = ceil_div(p.Lk, DQ_KT);
-  if (blocks >= 256 || steps < 4) return 1;
-  long long s = (512 + blocks - 1) / blocks;
-  if (s > steps / 2) s = steps / 2;
-  return s < 1 ? 1 : (int)s;
+  const bool few = attn_few(p, dtype);
+  const long long blocks = (long long)(few ? 1 : ceil_div(p.R, 128)) * p.N * p.Hk;
+  const int steps = ceil_div(p.Lk, few ? 128 : 64);
+  if (blocks >= 256 || steps < 2) return 1;
+  long long per = (steps * blocks + 511) / 512;
+  if (!few && per < 2) per = 2;
+  return (int)((steps + per - 1) / per);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool FEW>
 static int launch(const AttnDev& p, hipStream_t st) {
-  const int lds = 4 * DQ_KT * AttnTile<T, DP>::PITCH;
+  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
   const long long blocks = (long long)p.tiles * p.splits * p.N * p.Hk;
   SEGK_UNSUPPORTED(blocks < 0x7ffffff0LL, "attention_bwd: too many workgroups");
-  auto kern = p.mask || p.kmask ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>;
+  auto kern = p.mask || p.kmask ? attn_dq_kernel<T, DP, FEW, true> : attn_dq_kernel<T, DP, FEW, false>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
@@ -177,17 +222,20 @@ static int launch(const AttnDev& p, hipStream_t st) {
 }
 
 template <typename T>
-static int dispatch(const AttnDev& p, hipStream_t st) {
-  if (p.D <= 32) return launch<T, 32>(p, st);
-  if (p.D <= 64) return launch<T, 64>(p, st);
-  if (p.D <= 96) return launch<T, 96>(p, st);
-  return launch<T, 128>(p, st);
+static int dispatch(const AttnDev& p, bool few, hipStream_t st) {
+  if (p.D <= 32) return few ? launch<T, 32, true>(p, st) : launch<T, 32, false>(p, st);
+  if (p.D <= 64) return few ? launch<T, 64, true>(p, st) : launch<T, 64, false>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (few) return p.D <= 96 ? launch<T, 96, true>(p, st) : launch<T, 128, true>(p, st);
+  }
+  return p.D <= 96 ? launch<T, 96, false>(p, st) : launch<T, 128, false>(p, st);
 }
 
 int launch_attn_dq(AttnDev p, int dtype, hipStream_t st) {
-  p.tiles = ceil_div(p.R, 128);
+  const bool few = attn_few(p, dtype);
+  p.tiles = few ? 1 : ceil_div(p.R, 128);
   p.splits = attn_dq_splits(p, dtype);
-  const int rc = dtype == SEGK_BF16 ? dispatch<bf16_t>(p, st) : dispatch<float>(p, st);
+  const int rc = dtype == SEGK_BF16 ? dispatch<bf16_t>(p, few, st) : dispatch<float>(p, few, st);
   if (rc != SEGK_OK || p.splits == 1) return rc;
   const long long all = (long long)p.N * p.Lq * p.Hq * p.D;
   return launch_attn_sum(p.part, all, p.splits, p.scale, p.dq, all, dtype, st);

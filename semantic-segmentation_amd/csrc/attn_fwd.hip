@@ -6,20 +6,20 @@
 
 namespace segk {
 
-constexpr int KT = 64;   // keys per step
-
-// One workgroup: 4 wavefronts of 32 * QB rows each; a loop over tiles of 64 keys.  Scores are computed transposed
-// (S^T = K Q^T, a lane owns one query), so the row maximum is an in-lane reduction plus one exchange, the running
-// statistics are one register, and S^T is the operand of O^T = V^T P^T as it lies (attn.h).
-// MASKED: a pair mask and / or a key mask is read.
-template <typename T, int DP, int QB, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * QB * (int)sizeof(T) >= 512 ? 1 : 2)) void attn_fwd_kernel(const AttnDev p) {
+// One workgroup: 4 wavefronts and a loop over tiles of keys.  Scores are computed transposed (S^T = K Q^T, a lane owns one
+// query), so the row maximum is an in-lane reduction plus one exchange, the running statistics are one register, and S^T is
+// the operand of O^T = V^T P^T as it lies (attn.h).
+//   FEW = false  128 rows, 32 to a wavefront; tiles of 64 keys that every wavefront reads
+//   FEW = true   at most 32 rows (a query token, class queries): all wavefronts take the same rows and each its own 32 keys
+//                of a tile of 128; their parts are joined in LDS at the end
+// MASKED: a pair mask and / or a key mask is read, one tile ahead of its use.
+template <typename T, int DP, bool FEW, bool MASKED>
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
+  constexpr int KT = FEW ? 128 : 64, NKB = FEW ? 1 : 2;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
-  constexpr int NP = TILE_B / 4096;       // 1-KiB pieces per wavefront and operand
-  constexpr int RPW = 32 * QB, RPB = 4 * RPW;
   extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -31,224 +31,280 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * QB * (int)sizeof(T) >= 512 ? 1 
   const int tile = w % p.tiles;
   w /= p.tiles;
   const int hk = w % p.Hk, n = w / p.Hk;
-  const int row0 = tile * RPB;
+  const int row0 = FEW ? 0 : tile * 128 + wave * 32;      // of this wavefront
+  const bool idle = row0 >= p.R;                          // it then only helps to stage the tiles
 
   // keys that some row of the workgroup may use
-  const int last_row = min(row0 + RPB, p.R) - 1;
+  const int last_row = min(FEW ? 32 : tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
   const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + p.splits - 1) / p.splits;
   const int t0 = min(split * per, all_steps), t1 = min(t0 + per, all_steps);
 
-  AttnFrag<T> qf[QB][KS];
-  int tok[QB], head[QB];
-  bool row_ok[QB];
+  const int r = row0 + l31;
+  const bool row_ok = r < p.R;
+  const int rr = row_ok ? r : 0;
+  const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
+  AttnFrag<T> qf[KS];
+  {
+    const char* src = p.q.p + ((long long)n * p.q.n + (long long)tok * p.q.l + (long long)head * p.q.h) * (int)sizeof(T);
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int r = row0 + wave * RPW + qb * 32 + l31;
-    row_ok[qb] = r < p.R;
-    const int rr = row_ok[qb] ? r : 0;
-    tok[qb] = div_g(p, rr);
-    head[qb] = hk * p.G + rr - tok[qb] * p.G;
-    const char* src = p.q.p + ((long long)n * p.q.n + (long long)tok[qb] * p.q.l + (long long)head[qb] * p.q.h) * (int)sizeof(T);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[qb][ks] = load_frag<T>(src, ks, h, p.D, row_ok[qb]);
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<T>(src, ks, h, p.D, row_ok);
   }
-  const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0 + wave * RPW, p.R - 1)));
-  const unsigned char* mrow[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb)
-    mrow[qb] = MASKED && p.mask ? p.mask + n * p.m_n + (long long)head[qb] * p.m_h + (long long)tok[qb] * p.m_q : nullptr;
+  const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0, p.R - 1)));
 
-  // staging: this lane's place in the pieces it loads
-  const int lin = wave * 1024 + lane * 16;
-  const int st_row = lin / Tile::PITCH;
-  const int st_chunk = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(st_row);     // (4096 / PITCH is a period of swz)
-  const bool st_ok = st_chunk * 16 < p.D * (int)sizeof(T);
-  const unsigned k_step_b = (unsigned)(p.k.l * (int)sizeof(T)), v_step_b = (unsigned)(p.v.l * (int)sizeof(T));
-  const char* const kbase = p.k.p + ((long long)n * p.k.n + (long long)hk * p.k.h) * (int)sizeof(T);
-  const char* const vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
-  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
-  const unsigned lds0 = lds_addr(smem) + wave * 1024;
-  auto stage = [&](int t, int buf) {
-    const int key0 = t * KT;
-    const u32x4 kr = buffer_of(kbase + (long long)key0 * k_step_b);
-    const u32x4 vr = buffer_of(vbase + (long long)key0 * v_step_b);
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
+  AttnPairMask<NKB> pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k,
+                       p.Lk, (FEW ? wave * 32 : 0) + 4 * h);
+
+  f32x16 o[DB];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int row = st_row + i * (4096 / Tile::PITCH);
-      bool ok = st_ok && key0 + row < p.Lk;
-      // a key that its mask closes is not read: whatever its memory holds, zeros arrive
-      if (MASKED && kmask && ok) ok = kmask[(long long)(key0 + row) * p.km_k] != 0;
-      const unsigned lds = lds0 + buf * (2 * TILE_B) + i * 4096;
-      dma_1k(kr, lds, ok ? row * k_step_b + st_chunk * 16 : ATTN_OOB);
-      dma_1k(vr, lds + TILE_B, ok ? row * v_step_b + st_chunk * 16 : ATTN_OOB);
+  for (int db = 0; db < DB; ++db) o[db] = zero16();
+
+  if (t0 < t1) {
+    if (MASKED) {
+      km.load(t0 * KT);
+      km.next();
+      km.load((t0 + 1) * KT);
+      pm.load(t0 * KT);
     }
-  };
-
-  f32x16 o[QB][DB];
-  float m[QB], l[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    m[qb] = -INFINITY;
-    l[qb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[qb][db] = zero16();
+    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
   }
-
-  if (t0 < t1) stage(t0, 0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     tile_barrier();                       // tile t is here; every wavefront has left tile t - 1
-    if (t + 1 < t1) stage(t + 1, buf ^ 1);
-    const char* kt = smem + buf * (2 * TILE_B);
+    const int key0 = t * KT + (FEW ? wave * 32 : 0);
+    unsigned kw[NKB], pw[NKB][4];
+    bool dead = idle;
+    if (MASKED) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        kw[kb] = km.word((FEW ? wave * 32 : 0) + kb * 32);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) pw[kb][g] = pm.w[kb][g];
+      }
+      dead = dead || !(NKB == 2 ? kw[0] | kw[NKB - 1] : kw[0]);
+      if (pm.row && !dead) {
+        unsigned some = 0;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) some |= pw[kb][g];
+        dead = !__any(row_ok && some != 0);
+      }
+    }
+    if (t + 1 < t1) {
+      if (MASKED) {
+        km.next();
+        km.load((t + 2) * KT);
+        pm.load((t + 1) * KT);
+      }
+      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    }
+    if (dead) continue;                   // nothing of this tile is open to this wavefront's rows
+    const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
     const char* vt = kt + TILE_B;
-    const int key0 = t * KT;
 
-    f32x16 s[QB][2];
+    f32x16 s[NKB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) s[qb][kb] = zero16();
+    for (int kb = 0; kb < NKB; ++kb) s[kb] = zero16();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const AttnFrag<T> a = Rd::rows(kt, kb * 32, ks, lane);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) mma32(s[qb][kb], a, qf[qb][ks]);
-      }
+      for (int kb = 0; kb < NKB; ++kb) mma32(s[kb], Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
 
     // closed pairs: past the last key, above the diagonal, masked
-    const bool ragged = key0 + KT > p.Lk || (p.causal && key0 + KT - 1 > wave_tok0 + p.off);
-    if (MASKED || ragged) {
+    if (key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off)) {
+      const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const int lim = p.causal ? min(p.Lk - 1, tok[qb] + p.off) : p.Lk - 1;
+      for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = key0 + kb * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-            bool open = j <= lim;
-            if (MASKED && open) {
-              if (kmask) open = kmask[(long long)j * p.km_k] != 0;
-              if (mrow[qb] && open) open = mrow[qb][(long long)j * p.m_k] != 0;
-            }
-            s[qb][kb][i] = open ? s[qb][kb][i] : -INFINITY;
-          }
-      }
+        for (int i = 0; i < 16; ++i) s[kb][i] = kb * 32 + 8 * (i >> 2) + (i & 3) <= lim ? s[kb][i] : -INFINITY;
     }
-
-    AttnFrag<T> pf[QB][4];
+    if (MASKED) {
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      float mx = s[qb][0][0];
+      for (int kb = 0; kb < NKB; ++kb) {
+        if (km.mask) {
+          const unsigned x = kw[kb] >> (4 * h);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[qb][kb][i]);
-      mx = pair_max(mx) * p.scale_log2;
-      // The maximum in use may lag the true one by up to 8 (probabilities up to 2^8, harmless in fp32 and in the relative
-      // precision of bf16): the accumulators are then rescaled a few times per row instead of once per tile.
-      if (__any(mx > m[qb] + 8.f)) {
-        const float nm = fmaxf(m[qb], mx);
-        const float safe = nm == -INFINITY ? 0.f : nm;
-        const float alpha = exp2_fast(m[qb] - safe);
-        m[qb] = nm;
-        l[qb] *= alpha;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[qb][db][i] *= alpha;
-      }
-      const float ms = m[qb] == -INFINITY ? 0.f : m[qb];
-      float sum = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = exp2_fast(fmaf(s[qb][kb][i], p.scale_log2, -ms));
-          s[qb][kb][i] = e;
-          sum += e;
+          for (int i = 0; i < 16; ++i) s[kb][i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[kb][i] : -INFINITY;
         }
-      l[qb] += sum;
+        if (pm.row) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pf[qb][j] = pack_frag<T>(s[qb][j >> 1], j & 1);
+          for (int i = 0; i < 16; ++i) s[kb][i] = pw[kb][i >> 2] & (0xffu << (8 * (i & 3))) ? s[kb][i] : -INFINITY;
+        }
+      }
     }
 
+    float mx = s[0][0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const AttnFrag<T> a = Rd::cols(vt, j * 16, db * 32, lane);
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = pair_max(mx) * p.scale_log2;
+    // The maximum in use may lag the true one by up to 8 (probabilities up to 2^8, harmless in fp32 and in the relative
+    // precision of bf16): the accumulators are then rescaled a few times per row instead of once per tile.
+    if (__any(mx > m + 8.f)) {
+      const float nm = fmaxf(m, mx);
+      const float alpha = exp2_fast(m - (nm == -INFINITY ? 0.f : nm));
+      m = nm;
+      l *= alpha;
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) mma32(o[qb][db], a, pf[qb][j]);
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_fast(fmaf(s[kb][i], p.scale_log2, -ms));
+        s[kb][i] = e;
+        sum += e;
       }
+    l += sum;
+#pragma unroll
+    for (int j = 0; j < 2 * NKB; ++j) {
+      const AttnFrag<T> pf = pack_frag<T>(s[j >> 1], j & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) mma32(o[db], Rd::cols(vt, j * 16, db * 32, lane), pf);
+    }
   }
 
+  float lt = pair_sum(l);
+  if constexpr (FEW) {
+    // join the four wavefronts' parts: [wave][row][DP + 4] sums, then 4 x 32 maxima and sums
+    constexpr int LD = DP + 4;
+    float* const so = reinterpret_cast<float*>(smem);
+    float* const sm = so + 4 * 32 * LD;
+    tile_barrier();
+    if (h == 0) sm[wave * 32 + l31] = m;
+    tile_barrier();
+    float all = sm[l31];
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const float lt = pair_sum(l[qb]);
-    if (!row_ok[qb]) continue;
-    if (p.splits == 1) {
-      const float inv = lt == 0.f ? 0.f : 1.f / lt;
-      char* dst = p.out + ((long long)n * p.o.n + (long long)tok[qb] * p.o.l + (long long)head[qb] * p.o.h) * (int)sizeof(T);
+    for (int i = 1; i < 4; ++i) all = fmaxf(all, sm[i * 32 + l31]);
+    const float a = exp2_fast(m - (all == -INFINITY ? 0.f : all));
+    if (h == 0) sm[128 + wave * 32 + l31] = lt * a;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int d = db * 32 + 2 * i + 4 * h;
-          if (d < p.D) store4<T>(dst, d, o[qb][db][i] * inv, o[qb][db][i + 1] * inv, o[qb][db][i + 2] * inv, o[qb][db][i + 3] * inv);
-        }
-      if (p.lse && h == 0)
-        p.lse[((long long)n * p.Hq + head[qb]) * p.Lq + tok[qb]] = lt == 0.f ? -INFINITY : (m[qb] + log2f(lt)) * 0.6931471805599453f;
-    } else {
-      const long long r = ((long long)split * p.N * p.Hk + (long long)n * p.Hk + hk) * p.R + row0 + wave * RPW + qb * 32 + l31;
-      float* dst = p.part + r * p.D;
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
+            f32x4{o[db][i] * a, o[db][i + 1] * a, o[db][i + 2] * a, o[db][i + 3] * a};
+    tile_barrier();
+    for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
+      const int row = x / (DP / 4), d = x % (DP / 4) * 4;
+      if (row >= p.R || d >= p.D) continue;
+      f32x4 v = *reinterpret_cast<const f32x4*>(so + row * LD + d);
+      float sum = sm[128 + row], top = sm[row];
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int i = 1; i < 4; ++i) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + row) * LD + d);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int d = db * 32 + 2 * i + 4 * h;
-          if (d < p.D) store4<float>((char*)dst, d, o[qb][db][i], o[qb][db][i + 1], o[qb][db][i + 2], o[qb][db][i + 3]);
-        }
-      if (h == 0) {
-        p.part_ml[2 * r] = m[qb];
-        p.part_ml[2 * r + 1] = lt;
+        for (int e = 0; e < 4; ++e) v[e] += y[e];
+        sum += sm[128 + i * 32 + row];
+        top = fmaxf(top, sm[i * 32 + row]);
       }
+      if (p.splits == 1) {
+        const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store4<T>(p.out + ((long long)n * p.o.n + (long long)tk * p.o.l + (long long)hd * p.o.h) * (int)sizeof(T), d, v[0] * inv, v[1] * inv,
+                  v[2] * inv, v[3] * inv);
+        if (p.lse && d == 0)
+          p.lse[((long long)n * p.Hq + hd) * p.Lq + tk] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+      } else {
+        const long long at = ((long long)split * p.N * p.Hk + (long long)n * p.Hk + hk) * p.R + row;
+        store4<float>((char*)(p.part + at * p.D), d, v[0], v[1], v[2], v[3]);
+        if (d == 0) {
+          p.part_ml[2 * at] = top;
+          p.part_ml[2 * at + 1] = sum;
+        }
+      }
+    }
+    return;
+  }
+  if (!row_ok) return;
+  if (p.splits == 1) {
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    char* dst = p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = db * 32 + 2 * i + 4 * h;
+        if (d < p.D) store4<T>(dst, d, o[db][i] * inv, o[db][i + 1] * inv, o[db][i + 2] * inv, o[db][i + 3] * inv);
+      }
+    if (p.lse && h == 0)
+      p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.6931471805599453f;
+  } else {
+    const long long at = ((long long)split * p.N * p.Hk + (long long)n * p.Hk + hk) * p.R + r;
+    char* dst = (char*)(p.part + at * p.D);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = db * 32 + 2 * i + 4 * h;
+        if (d < p.D) store4<float>(dst, d, o[db][i], o[db][i + 1], o[db][i + 2], o[db][i + 3]);
+      }
+    if (h == 0) {
+      p.part_ml[2 * at] = m;
+      p.part_ml[2 * at + 1] = lt;
     }
   }
 }
 
-// Joins the parts of a split key axis, in part order: one wavefront per row.
+// Joins the parts of a split key axis: one workgroup per row; D / 4 (rounded up to a power of two) threads walk the
+// channels of every GROUPS-th part, the groups are joined in LDS in order.
 template <typename T>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p) {
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes) {
+  __shared__ f32x4 so[ATTN_THREADS];
+  __shared__ float sl[ATTN_THREADS], sm[4];
   const long long rows = (long long)p.N * p.Hk * p.R;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
+  const long long r = blockIdx.x;
+  const int c = threadIdx.x % lanes, g = threadIdx.x / lanes, groups = ATTN_THREADS / lanes;
   float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * rows + r)]);
+  for (int s = threadIdx.x; s < p.splits; s += ATTN_THREADS) m = fmaxf(m, p.part_ml[2 * (s * rows + r)]);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   const float ms = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = g; s < p.splits; s += groups) {
     const long long at = s * rows + r;
     const float a = exp2_fast(p.part_ml[2 * at] - ms);
     l = fmaf(p.part_ml[2 * at + 1], a, l);
-    if (lane < p.D) o0 = fmaf(p.part[at * p.D + lane], a, o0);
-    if (lane + 64 < p.D) o1 = fmaf(p.part[at * p.D + lane + 64], a, o1);
+    if (c * 4 < p.D) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * p.D + c * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], a, o[e]);
+    }
+  }
+  so[threadIdx.x] = o;
+  sl[threadIdx.x] = l;
+  __syncthreads();
+  if (g != 0 || c * 4 >= p.D) return;
+  for (int i = 1; i < groups; ++i) {
+    const f32x4 x = so[i * lanes + c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += x[e];
+    l += sl[i * lanes + c];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int rr = (int)(r % p.R);
   const long long nh = r / p.R;
   const int hk = (int)(nh % p.Hk), n = (int)(nh / p.Hk);
   const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
-  T* dst = (T*)p.out + (long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h;
-  if (lane < p.D) Elem<T>::store(dst + lane, o0 * inv);
-  if (lane + 64 < p.D) Elem<T>::store(dst + lane + 64, o1 * inv);
-  if (p.lse && lane == 0)
+  store4<T>(p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T), c * 4, o[0] * inv, o[1] * inv,
+            o[2] * inv, o[3] * inv);
+  if (p.lse && c == 0)
     p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
@@ -300,17 +356,22 @@ static int attn_pitch(int D, int dtype) {
   return b <= 64 ? 64 : b <= 128 ? 128 : b <= 256 ? 256 : 512;
 }
 
-static int fwd_rows_per_block(const AttnDev& p, int dtype) { return 128; }
+// The wavefronts divide the keys instead of the rows where 32 rows hold the whole problem, except for fp32 heads over 64
+// channels, whose tiles of 128 keys do not fit into LDS twice, and for keys so far apart that 128 pass a buffer's range.
+bool attn_few(const AttnDev& p, int dtype) {
+  const long long far = (p.k.l > p.v.l ? p.k.l : p.v.l) * 128 * dtype_size(dtype);
+  return p.R <= 32 && attn_pitch(p.D, dtype) <= 256 && far < 0xf0000000LL;
+}
 
 static int fwd_splits(const AttnDev& p, int dtype) {
-  const int rpb = fwd_rows_per_block(p, dtype);
-  const long long blocks = (long long)ceil_div(p.R, rpb) * p.N * p.Hk;
-  const int steps = ceil_div(p.Lk, KT);
-  // Too few workgroups for 256 CUs: cut the key axis, at least 2 steps a part.
-  if (blocks >= 256 || steps < 4) return 1;
-  long long s = (512 + blocks - 1) / blocks;
-  if (s > steps / 2) s = steps / 2;
-  return s < 1 ? 1 : (int)s;
+  const bool few = attn_few(p, dtype);
+  const long long blocks = (long long)(few ? 1 : ceil_div(p.R, 128)) * p.N * p.Hk;
+  const int steps = ceil_div(p.Lk, few ? 128 : 64);
+  // Too few workgroups for 256 CUs: cut the key axis into parts of `per` steps.
+  if (blocks >= 256 || steps < 2) return 1;
+  long long per = (steps * blocks + 511) / 512;
+  if (!few && per < 2) per = 2;
+  return (int)((steps + per - 1) / per);
 }
 
 #define CHK_VIEW(v, name, L, H)                                                                                                   \
@@ -372,14 +433,14 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   return SEGK_OK;
 }
 
-template <typename T, int DP, int QB>
+template <typename T, int DP, bool FEW>
 static int launch_fwd(const AttnDev& p, hipStream_t st) {
-  const int lds = 4 * KT * AttnTile<T, DP>::PITCH;
+  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
   const long long blocks = (long long)p.tiles * p.splits * p.N * p.Hk;
   SEGK_UNSUPPORTED(blocks < 0x7ffffff0LL, "attention: too many workgroups");
   const unsigned grid = (unsigned)((blocks + 7) / 8 * 8);
   const bool masked = p.mask || p.kmask;
-  auto kern = masked ? attn_fwd_kernel<T, DP, QB, true> : attn_fwd_kernel<T, DP, QB, false>;
+  auto kern = masked ? attn_fwd_kernel<T, DP, FEW, true> : attn_fwd_kernel<T, DP, FEW, false>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
@@ -393,12 +454,18 @@ static int launch_fwd(const AttnDev& p, hipStream_t st) {
 }
 
 template <typename T>
-static int dispatch_fwd(const AttnDev& p, hipStream_t st) {
+static int dispatch_fwd(const AttnDev& p, bool few, hipStream_t st) {
   switch (attn_dp(p.D)) {
-    case 32: return launch_fwd<T, 32, 1>(p, st);
-    case 64: return launch_fwd<T, 64, 1>(p, st);
-    case 96: return launch_fwd<T, 96, 1>(p, st);
-    default: return launch_fwd<T, 128, 1>(p, st);
+    case 32: return few ? launch_fwd<T, 32, true>(p, st) : launch_fwd<T, 32, false>(p, st);
+    case 64: return few ? launch_fwd<T, 64, true>(p, st) : launch_fwd<T, 64, false>(p, st);
+    case 96:
+      if constexpr (sizeof(T) == 2)
+        if (few) return launch_fwd<T, 96, true>(p, st);
+      return launch_fwd<T, 96, false>(p, st);
+    default:
+      if constexpr (sizeof(T) == 2)
+        if (few) return launch_fwd<T, 128, true>(p, st);
+      return launch_fwd<T, 128, false>(p, st);
   }
 }
 
@@ -434,7 +501,8 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
   const int rc = attn_check(a, &p, false);
   if (rc != SEGK_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
-  p.tiles = ceil_div(p.R, fwd_rows_per_block(p, a->dtype));
+  const bool few = attn_few(p, a->dtype);
+  p.tiles = few ? 1 : ceil_div(p.R, 128);
   p.splits = fwd_splits(p, a->dtype);
   const long long need = fwd_part_floats(p, p.splits) * 4;
   if (need > 0) {
@@ -446,10 +514,11 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
     p.part = (float*)a->workspace;
     p.part_ml = p.part + (long long)p.splits * p.N * p.Hk * p.R * p.D;
   }
-  const int rc2 = a->dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, st) : dispatch_fwd<float>(p, st);
+  const int rc2 = a->dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, few, st) : dispatch_fwd<float>(p, few, st);
   if (rc2 != SEGK_OK || p.splits == 1) return rc2;
-  const unsigned grid = (unsigned)(((long long)p.N * p.Hk * p.R + 3) / 4);
-  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p)));
+  const int lanes = p.D <= 8 ? 2 : p.D <= 16 ? 4 : p.D <= 32 ? 8 : p.D <= 64 ? 16 : 32;
+  const unsigned grid = (unsigned)((long long)p.N * p.Hk * p.R);   // (splits only where workgroups are few: small)
+  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes)));
   SEGK_CHECK_LAUNCH("attention_fwd join");
   return SEGK_OK;
 }

@@ -31,7 +31,9 @@ struct RotDev {
   float eps;
   int norm, interleaved, pairs;
   int N, L, D;
+  float inv_d;
   int heads_per, chunks;    // heads of one piece of work, pieces per token
+  int work;                 // pieces in all
   float* part;              // [2 * D][blocks] weight-gradient partials
   int blocks;
 };
@@ -64,128 +66,128 @@ __device__ __forceinline__ void rot_store4<float>(char* p, const float* v) {
   *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-// A lane owns 4 pairs = 8 channels of a head: two runs of 4 channels at lo and hi.  Pairs of distant channels
-// (i, i + pairs): v[0..3] are the first, v[4..7] the second members; pairs of neighbours: runs of (a, b, a, b).
-// Channels past the rotated ones travel in neighbouring runs too, turned by nothing.
+// A lane owns 4 pairs = 8 channels of a head, v[0 .. 3] and v[4 .. 7] from the runs of 4 channels at lo and hi.  INTER
+// (neighbours are paired): one run of 8, pairs (v[2c], v[2c + 1]).  Else pairs (v[c], v[4 + c]): channel c of the first
+// half and of the second half of the rotated channels, and then of the channels past them (which turn by nothing).
+template <bool INTER>
 struct RotLane {
   int lo, hi;
-  bool live, split;
+  bool live;
   float c[4], s[4];
-};
-
-__device__ __forceinline__ RotLane rot_lane(const RotDev& p, int j) {
-  RotLane t;
-  t.live = j * 8 < p.D;
-  t.split = !p.interleaved && 4 * j < p.pairs;
-  t.lo = t.split ? 4 * j : 8 * j;
-  t.hi = t.split ? p.pairs + 4 * j : 8 * j + 4;
+  __device__ __forceinline__ RotLane(const RotDev& p, int j) {
+    live = j * 8 < p.D;
+    const bool turned = 4 * j < p.pairs;
+    lo = INTER ? 8 * j : turned ? 4 * j : p.pairs + 4 * j;
+    hi = INTER ? 8 * j + 4 : turned ? p.pairs + 4 * j : p.D / 2 + 4 * j;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) t.c[e] = 1.f, t.s[e] = 0.f;
-  return t;
-}
-
-// cos and sin of this lane's 4 pairs.  The angle is formed and reduced to half turns in fp64 (a position in the hundred
-// thousands times a frequency loses its fraction in fp32), the rest in fp32.
-__device__ __forceinline__ void rot_angles(const RotDev& p, int j, int n, int l, RotLane& t) {
-  if (4 * j >= p.pairs) return;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int c = 4 * j + e;
-    int axis = 0;
-#pragma unroll
-    for (int a = 1; a < 4; ++a) axis = a < p.axes && c >= p.first[a] ? a : axis;
-    const long long at = n * p.pn + l * p.pl + axis * p.pa;
-    double x;
-    if (p.pos_dtype == 0) x = ((const int*)p.pos)[at];
-    else if (p.pos_dtype == 1) x = (double)((const long long*)p.pos)[at];
-    else x = ((const float*)p.pos)[at];
-    const double half_turns = x * (double)p.inv_freq[c] * 0.31830988618379067154;
-    const float f = (float)(half_turns - 2.0 * rint(half_turns * 0.5));
-    sincospif(f, &t.s[e], &t.c[e]);
+    for (int e = 0; e < 4; ++e) c[e] = 1.f, s[e] = 0.f;
   }
-}
-
-// forward turn (sign +1) or its inverse (-1)
-__device__ __forceinline__ void rot_turn(const RotLane& t, float sign, float* v) {
+  __device__ __forceinline__ int channel(int e) const { return e < 4 ? lo + e : hi + e - 4; }
+  // cos and sin of this lane's pairs.  The angle is formed and reduced to half turns in fp64 (a position in the hundred
+  // thousands times a frequency loses its fraction in fp32), the rest in fp32.
+  __device__ __forceinline__ void angles(const RotDev& p, int j, int n, int l) {
+    if (4 * j >= p.pairs) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = t.split ? v[e] : v[2 * e], b = t.split ? v[4 + e] : v[2 * e + 1];
-    const float s = sign * t.s[e];
-    const float x = a * t.c[e] - b * s, y = a * s + b * t.c[e];
-    // (a lane is of one kind throughout; both forms are written by selects)
-    if (t.split) {
-      v[e] = x;
-      v[4 + e] = y;
-    } else {
-      v[2 * e] = x;
-      v[2 * e + 1] = y;
+    for (int e = 0; e < 4; ++e) {
+      const int k = 4 * j + e;
+      int axis = 0;
+#pragma unroll
+      for (int a = 1; a < 4; ++a) axis = a < p.axes && k >= p.first[a] ? a : axis;
+      const long long at = n * p.pn + l * p.pl + axis * p.pa;
+      double x;
+      if (p.pos_dtype == 0) x = ((const int*)p.pos)[at];
+      else if (p.pos_dtype == 1) x = (double)((const long long*)p.pos)[at];
+      else x = ((const float*)p.pos)[at];
+      const double half_turns = x * (double)p.inv_freq[k] * 0.31830988618379067154;
+      const float f = (float)(half_turns - 2.0 * rint(half_turns * 0.5));
+      sincospif(f, &s[e], &c[e]);
     }
   }
-}
+  // forward turn (sign +1) or its inverse (-1)
+  __device__ __forceinline__ void turn(float sign, float* v) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float &a = v[INTER ? 2 * e : e], &b = v[INTER ? 2 * e + 1 : 4 + e];
+      const float z = sign * s[e];
+      const float x = a * c[e] - b * z, y = a * z + b * c[e];
+      a = x;
+      b = y;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const char* row, float* v) const {
+    rot_load4<T>(row + lo * (int)sizeof(T), v);
+    rot_load4<T>(row + hi * (int)sizeof(T), v + 4);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(char* row, const float* v) const {
+    rot_store4<T>(row + lo * (int)sizeof(T), v);
+    rot_store4<T>(row + hi * (int)sizeof(T), v + 4);
+  }
+};
 
+// Sum over a group of LPH neighbouring lanes, to every lane: exchanges inside 16 lanes are DPP operands.
 template <int LPH>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = LPH >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+#define ROT_DPP(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
+  if (LPH >= 2) ROT_DPP(0xb1);    // lanes 1 0 3 2 of a quad
+  if (LPH >= 4) ROT_DPP(0x4e);    // lanes 2 3 0 1 of a quad
+  if (LPH >= 8) ROT_DPP(0x141);   // mirror of 8 lanes: the other quad
+  if (LPH >= 16) ROT_DPP(0x140);  // mirror of 16 lanes: the other eight
+#undef ROT_DPP
+  if (LPH >= 32) v += __shfl_xor(v, 16, 64);
   return v;
 }
 
-// A group of LPH lanes (D / 8 rounded up to a power of two) takes one token and `heads_per` of its heads: the angles are
-// computed once for all of them.
-template <typename T, int LPH>
+// one head of the forward pass, from registers
+template <typename T, int LPH, bool INTER>
+__device__ __forceinline__ void rot_head(const RotDev& p, const RotLane<INTER>& t, const float* w, float* v, char* dst) {
+  if (p.norm) {
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q = fmaf(v[e], v[e], q);
+    const float r = rsqrtf(fmaf(group_sum<LPH>(q), p.inv_d, p.eps));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= r * w[e];
+  }
+  t.turn(1.f, v);
+  if (t.live) t.template store<T>(dst, v);
+}
+
+// A group of LPH lanes (D / 8 rounded up to a power of two) takes one token and `heads_per` of its heads (queries, then
+// keys): the angles are computed once for all of them.
+template <typename T, int LPH, bool INTER>
 __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_kernel(const RotDev p) {
   const int j = threadIdx.x % LPH;
-  const long long work = (long long)blockIdx.x * (ROT_THREADS / LPH) + threadIdx.x / LPH;
-  const long long tokens = (long long)p.N * p.L;
-  if (work >= tokens * p.chunks) return;
-  const long long nl = work / p.chunks;
-  const int chunk = (int)(work - nl * p.chunks);
-  const int n = (int)(nl / p.L), l = (int)(nl - (long long)n * p.L);
-  RotLane t = rot_lane(p, j);
-  rot_angles(p, j, n, l, t);
-  float w[2][8];
+  const unsigned work = blockIdx.x * (ROT_THREADS / LPH) + threadIdx.x / LPH;
+  if (work >= (unsigned)p.work) return;
+  const unsigned nl = work / (unsigned)p.chunks;
+  const int h0 = (int)(work - nl * (unsigned)p.chunks) * p.heads_per;
+  const int n = (int)(nl / (unsigned)p.L), l = (int)(nl - (unsigned)n * (unsigned)p.L);
+  RotLane<INTER> t(p, j);
+  t.angles(p, j, n, l);
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
+  for (int q = 0; q < 2; ++q) {
+    const RotSide& sd = p.s[q];
+    const int shift = q ? p.s[0].heads : 0;
+    const int a = max(h0 - shift, 0), b = min(h0 + p.heads_per - shift, sd.heads);
+    if (a >= b) continue;
+    float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[q][e] = t.live && p.s[q].w ? p.s[q].w[(e < 4 ? t.lo : t.hi - 4) + e] : 1.f;
-  const int total = p.s[0].heads + p.s[1].heads;
-  const int h0 = chunk * p.heads_per, h1 = min(h0 + p.heads_per, total);
-  const float inv_d = 1.f / (float)p.D;
-  for (int hb = h0; hb < h1; hb += ROT_UNROLL) {
-    float v[ROT_UNROLL][8];
+    for (int e = 0; e < 8; ++e) w[e] = t.live && sd.w ? sd.w[t.channel(e)] : 1.f;
+    const char* src = sd.x + n * sd.xn + l * sd.xl;
+    char* dst = sd.y + (long long)nl * sd.heads * p.D * (int)sizeof(T);
+    for (int hb = a; hb < b; hb += ROT_UNROLL) {
+      float v[ROT_UNROLL][8];
 #pragma unroll
-    for (int u = 0; u < ROT_UNROLL; ++u) {
-      const int hh = hb + u;
+      for (int u = 0; u < ROT_UNROLL; ++u) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-      if (hh < h1 && t.live) {
-        const bool key = hh >= p.s[0].heads;
-        const RotSide& sd = p.s[key ? 1 : 0];
-        const char* src = sd.x + n * sd.xn + l * sd.xl + (hh - (key ? p.s[0].heads : 0)) * sd.xh;
-        rot_load4<T>(src + t.lo * (int)sizeof(T), v[u]);
-        rot_load4<T>(src + t.hi * (int)sizeof(T), v[u] + 4);
+        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+        if (hb + u < b && t.live) t.template load<T>(src + (hb + u) * sd.xh, v[u]);
       }
-    }
 #pragma unroll
-    for (int u = 0; u < ROT_UNROLL; ++u) {
-      const int hh = hb + u;
-      if (hh >= h1) break;
-      const bool key = hh >= p.s[0].heads;
-      const RotSide& sd = p.s[key ? 1 : 0];
-      if (p.norm) {
-        float q = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q = fmaf(v[u][e], v[u][e], q);
-        const float r = rsqrtf(fmaf(group_sum<LPH>(q), inv_d, p.eps));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] *= r * (key ? w[1][e] : w[0][e]);
-      }
-      rot_turn(t, 1.f, v[u]);
-      if (t.live) {
-        char* dst = sd.y + ((nl * sd.heads + (hh - (key ? p.s[0].heads : 0))) * p.D) * (int)sizeof(T);
-        rot_store4<T>(dst + t.lo * (int)sizeof(T), v[u]);
-        rot_store4<T>(dst + t.hi * (int)sizeof(T), v[u] + 4);
-      }
+      for (int u = 0; u < ROT_UNROLL; ++u)
+        if (hb + u < b) rot_head<T, LPH, INTER>(p, t, w, v[u], dst + (long long)(hb + u) * p.D * (int)sizeof(T));
     }
   }
 }
@@ -193,81 +195,67 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_kernel(const RotDe
 // Backward.  dn = dy turned back; dw = sum dn x r; g = w dn; dx = r (g - x r mean(g x r)).  Weight gradients: each lane
 // sums its channels over its work in fp32, the groups of a workgroup are joined in LDS in order, one partial per
 // workgroup and channel, joined in fp64 by the second kernel: no atomics, a fixed order.
-template <typename T, int LPH>
+template <typename T, int LPH, bool INTER>
 __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const RotDev p) {
   __shared__ float red[ROT_THREADS][17];   // (17: a column walk meets distinct banks)
   constexpr int GROUPS = ROT_THREADS / LPH;
   const int j = threadIdx.x % LPH;
-  const long long tokens = (long long)p.N * p.L;
-  RotLane t = rot_lane(p, j);
+  RotLane<INTER> t(p, j);
   float w[2][8], dw[2][8];
 #pragma unroll
   for (int q = 0; q < 2; ++q)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[q][e] = t.live && p.s[q].w ? p.s[q].w[(e < 4 ? t.lo : t.hi - 4) + e] : 1.f;
+      w[q][e] = t.live && p.s[q].w ? p.s[q].w[t.channel(e)] : 1.f;
       dw[q][e] = 0.f;
     }
-  const int total = p.s[0].heads + p.s[1].heads;
-  const float inv_d = 1.f / (float)p.D;
-  for (long long work = (long long)blockIdx.x * GROUPS + threadIdx.x / LPH; work < tokens * p.chunks;
-       work += (long long)gridDim.x * GROUPS) {
-    const long long nl = work / p.chunks;
-    const int chunk = (int)(work - nl * p.chunks);
-    const int n = (int)(nl / p.L), l = (int)(nl - (long long)n * p.L);
-    rot_angles(p, j, n, l, t);
-    const int h0 = chunk * p.heads_per, h1 = min(h0 + p.heads_per, total);
-    for (int hb = h0; hb < h1; hb += 2) {
-      float v[2][8], g[2][8];
+  for (unsigned work = blockIdx.x * GROUPS + threadIdx.x / LPH; work < (unsigned)p.work; work += gridDim.x * GROUPS) {
+    const unsigned nl = work / (unsigned)p.chunks;
+    const int h0 = (int)(work - nl * (unsigned)p.chunks) * p.heads_per;
+    const int n = (int)(nl / (unsigned)p.L), l = (int)(nl - (unsigned)n * (unsigned)p.L);
+    t.angles(p, j, n, l);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int hh = hb + u;
+    for (int q = 0; q < 2; ++q) {
+      const RotSide& sd = p.s[q];
+      const int shift = q ? p.s[0].heads : 0;
+      const int a = max(h0 - shift, 0), b = min(h0 + p.heads_per - shift, sd.heads);
+      if (a >= b) continue;
+      const char* src = sd.x + n * sd.xn + l * sd.xl;
+      const char* dys = sd.dy + n * sd.dn + l * sd.dl;
+      char* dst = sd.y + (long long)nl * sd.heads * p.D * (int)sizeof(T);
+      for (int hb = a; hb < b; hb += 2) {
+        float v[2][8], g[2][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] = 0.f;
-        if (hh < h1 && t.live) {
-          const bool key = hh >= p.s[0].heads;
-          const RotSide& sd = p.s[key ? 1 : 0];
-          const int hl = hh - (key ? p.s[0].heads : 0);
-          const char* dy = sd.dy + n * sd.dn + l * sd.dl + hl * sd.dh;
-          rot_load4<T>(dy + t.lo * (int)sizeof(T), g[u]);
-          rot_load4<T>(dy + t.hi * (int)sizeof(T), g[u] + 4);
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] = 0.f;
+          if (hb + u < b && t.live) {
+            t.template load<T>(dys + (hb + u) * sd.dh, g[u]);
+            if (p.norm) t.template load<T>(src + (hb + u) * sd.xh, v[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (hb + u >= b) break;
+          t.turn(-1.f, g[u]);
           if (p.norm) {
-            const char* src = sd.x + n * sd.xn + l * sd.xl + hl * sd.xh;
-            rot_load4<T>(src + t.lo * (int)sizeof(T), v[u]);
-            rot_load4<T>(src + t.hi * (int)sizeof(T), v[u] + 4);
+            float z = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z = fmaf(v[u][e], v[u][e], z);
+            const float r = rsqrtf(fmaf(group_sum<LPH>(z), p.inv_d, p.eps));
+            float dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              v[u][e] *= r;
+              dw[q][e] = fmaf(g[u][e], v[u][e], dw[q][e]);
+              g[u][e] *= w[q][e];
+              dot = fmaf(g[u][e], v[u][e], dot);
+            }
+            dot = group_sum<LPH>(dot) * p.inv_d;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[u][e] = r * (g[u][e] - v[u][e] * dot);
           }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int hh = hb + u;
-        if (hh >= h1) break;
-        const bool key = hh >= p.s[0].heads;
-        const RotSide& sd = p.s[key ? 1 : 0];
-        rot_turn(t, -1.f, g[u]);
-        if (p.norm) {
-          float q = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q = fmaf(v[u][e], v[u][e], q);
-          const float r = rsqrtf(fmaf(group_sum<LPH>(q), inv_d, p.eps));
-          float dot = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[u][e] *= r;
-            const float add = g[u][e] * v[u][e];
-            dw[0][e] += key ? 0.f : add;
-            dw[1][e] += key ? add : 0.f;
-            g[u][e] *= key ? w[1][e] : w[0][e];
-            dot = fmaf(g[u][e], v[u][e], dot);
-          }
-          dot = group_sum<LPH>(dot) * inv_d;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[u][e] = r * (g[u][e] - v[u][e] * dot);
-        }
-        if (t.live) {
-          char* dst = sd.y + ((nl * sd.heads + (hh - (key ? p.s[0].heads : 0))) * p.D) * (int)sizeof(T);
-          rot_store4<T>(dst + t.lo * (int)sizeof(T), g[u]);
-          rot_store4<T>(dst + t.hi * (int)sizeof(T), g[u] + 4);
+          if (t.live) t.template store<T>(dst + (long long)(hb + u) * p.D * (int)sizeof(T), g[u]);
         }
       }
     }
@@ -282,10 +270,8 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
     const int jj = i % LPH, slot = i / LPH;
     float s = 0.f;
     for (int g = 0; g < GROUPS; ++g) s += red[g * LPH + jj][slot];
-    const RotLane o = rot_lane(p, jj);
-    const int e = slot & 7;
-    const int ch = (e < 4 ? o.lo : o.hi - 4) + e;
-    if (o.live) p.part[((long long)(slot >> 3) * p.D + ch) * p.blocks + blockIdx.x] = s;
+    const RotLane<INTER> o(p, jj);
+    if (o.live) p.part[((long long)(slot >> 3) * p.D + o.channel(slot & 7)) * p.blocks + blockIdx.x] = s;
   }
 }
 
@@ -355,32 +341,31 @@ static int rot_fill(const segk_qk_norm_rotary_args* a, RotDev* p, bool backward)
   if (per > 4) per = (per + 3) / 4 * 4;
   p->heads_per = (int)per;
   p->chunks = ceil_div(total, p->heads_per);
+  const long long work = (long long)a->N * a->L * p->chunks;
+  SEGK_UNSUPPORTED(work < 0x7f000000LL, "qk_norm_rotary: too many heads");
+  p->work = (int)work;
+  p->inv_d = 1.f / (float)a->D;
   p->part = nullptr;
   p->blocks = 0;
   return SEGK_OK;
 }
 
-static long long rot_blocks(const RotDev& p) {
-  const int per = ROT_THREADS / rot_lanes(p.D);
-  return ((long long)p.N * p.L * p.chunks + per - 1) / per;
-}
-static int rot_bwd_blocks(const RotDev& p) {
-  const long long b = rot_blocks(p);
-  return (int)(b < ROT_MAX_BLOCKS ? b : ROT_MAX_BLOCKS);
-}
+static int rot_blocks(const RotDev& p) { return ceil_div(p.work, ROT_THREADS / rot_lanes(p.D)); }
+static int rot_bwd_blocks(const RotDev& p) { return rot_blocks(p) < ROT_MAX_BLOCKS ? rot_blocks(p) : ROT_MAX_BLOCKS; }
 
 }  // namespace segk
 
 using namespace segk;
 
-#define ROT_LAUNCH(kernel, grid)                                                            \
-  switch (rot_lanes(p.D)) {                                                                 \
-    case 1: kernel<T, 1><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
-    case 2: kernel<T, 2><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
-    case 4: kernel<T, 4><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
-    case 8: kernel<T, 8><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;               \
-    case 16: kernel<T, 16><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;             \
-    default: kernel<T, 32><<<(unsigned)(grid), ROT_THREADS, 0, st>>>(p); break;             \
+#define ROT_CASE(kernel, grid, LPH)                                              \
+  case LPH:                                                                      \
+    if (p.interleaved) kernel<T, LPH, true><<<(grid), ROT_THREADS, 0, st>>>(p);  \
+    else kernel<T, LPH, false><<<(grid), ROT_THREADS, 0, st>>>(p);               \
+    break;
+#define ROT_LAUNCH(kernel, grid)                                                                     \
+  switch (rot_lanes(p.D)) {                                                                          \
+    ROT_CASE(kernel, grid, 1) ROT_CASE(kernel, grid, 2) ROT_CASE(kernel, grid, 4)                    \
+    ROT_CASE(kernel, grid, 8) ROT_CASE(kernel, grid, 16) ROT_CASE(kernel, grid, 32)                  \
   }
 
 extern "C" int segk_qk_norm_rotary(const segk_qk_norm_rotary_args* a, segk_stream_t stream) {
@@ -388,9 +373,7 @@ extern "C" int segk_qk_norm_rotary(const segk_qk_norm_rotary_args* a, segk_strea
   const int rc = rot_fill(a, &p, false);
   if (rc != SEGK_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const long long grid = rot_blocks(p);
-  SEGK_UNSUPPORTED(grid < 0x7fffffffLL, "qk_norm_rotary: too many heads");
-  SEGK_DISPATCH_DTYPE(a->dtype, T, ROT_LAUNCH(qk_norm_rotary_kernel, grid));
+  SEGK_DISPATCH_DTYPE(a->dtype, T, ROT_LAUNCH(qk_norm_rotary_kernel, rot_blocks(p)));
   SEGK_CHECK_LAUNCH("qk_norm_rotary");
   return SEGK_OK;
 }
