@@ -6,6 +6,7 @@ caller gets an exception.  The library is built in-tree by
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsegk.so")
@@ -63,27 +64,11 @@ class GemmTnArgs(ctypes.Structure):
                 ("splits", c_int), ("slabs", c_void_p)]
 
 
-class AttentionView(ctypes.Structure):
-    _fields_ = [("p", c_void_p), ("n", c_ll), ("l", c_ll), ("h", c_ll)]
-
-
-class AttentionArgs(ctypes.Structure):
-    _fields_ = [("N", c_int), ("Lq", c_int), ("Lk", c_int), ("Hq", c_int), ("Hk", c_int), ("D", c_int), ("dtype", c_int),
-                ("causal", c_int), ("scale", c_float), ("q", AttentionView), ("k", AttentionView), ("v", AttentionView),
-                ("out", AttentionView), ("lse", c_void_p), ("mask", c_void_p), ("mask_n", c_ll), ("mask_h", c_ll),
-                ("mask_q", c_ll), ("mask_k", c_ll), ("key_mask", c_void_p), ("key_mask_n", c_ll), ("key_mask_k", c_ll),
-                ("dout", AttentionView), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("workspace", c_void_p),
-                ("workspace_bytes", c_ll)]
-
-
-class QkNormRotaryArgs(ctypes.Structure):
-    _fields_ = [("N", c_int), ("L", c_int), ("Hq", c_int), ("Hk", c_int), ("D", c_int), ("dtype", c_int),
-                ("q", AttentionView), ("k", AttentionView), ("q_out", c_void_p), ("k_out", c_void_p),
-                ("q_weight", c_void_p), ("k_weight", c_void_p), ("positions", c_void_p), ("pos_dtype", c_int),
-                ("pos_n", c_ll), ("pos_l", c_ll), ("pos_a", c_ll), ("axes", c_int), ("section", c_int * 4),
-                ("inv_freq", c_void_p), ("norm", c_int), ("interleaved", c_int), ("eps", c_float),
-                ("dq", AttentionView), ("dk", AttentionView), ("dq_weight", c_void_p), ("dk_weight", c_void_p),
-                ("workspace", c_void_p), ("workspace_bytes", c_ll)]
+# segk_attention_args and segk_qk_norm_rotary_args, packed in one go (native alignment; a view is pointer and 3 strides);
+# the workspace pointer and its size are the last two fields of both.
+ATTENTION_ARGS = struct.Struct("@8if" + "P3q" * 4 + "PP4qP2q" + "P3q" + "3P")
+QK_NORM_ROTARY_ARGS = struct.Struct("@6i" + "P3q" * 2 + "5Pi3q5iP2if" + "P3q" * 2 + "2P")
+WORKSPACE_ARGS = struct.Struct("@Pq")
 
 
 # name -> argument types (every function returns int unless listed in _RESTYPES)
@@ -118,12 +103,12 @@ SIGNATURES = {
                      c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_void_p],
     "segk_dot": [c_void_p, c_int, c_void_p, c_int, c_int, c_ll, c_int, c_void_p, c_void_p, c_void_p],
     "segk_dot_partial_rows": [c_ll],
-    "segk_attention_fwd": [ctypes.POINTER(AttentionArgs), c_void_p],
-    "segk_attention_bwd": [ctypes.POINTER(AttentionArgs), c_void_p],
-    "segk_attention_workspace": [ctypes.POINTER(AttentionArgs), c_int],
-    "segk_qk_norm_rotary": [ctypes.POINTER(QkNormRotaryArgs), c_void_p],
-    "segk_qk_norm_rotary_bwd": [ctypes.POINTER(QkNormRotaryArgs), c_void_p],
-    "segk_qk_norm_rotary_bwd_workspace": [ctypes.POINTER(QkNormRotaryArgs)],
+    "segk_attention_fwd": [c_void_p, c_void_p],
+    "segk_attention_bwd": [c_void_p, c_void_p],
+    "segk_attention_workspace": [c_void_p, c_int],
+    "segk_qk_norm_rotary": [c_void_p, c_void_p],
+    "segk_qk_norm_rotary_bwd": [c_void_p, c_void_p],
+    "segk_qk_norm_rotary_bwd_workspace": [c_void_p],
     "segk_bn_stats": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "segk_bn_stat_rows": [c_int, c_int, c_int, c_int],
     "segk_bn_reduce": [c_void_p, c_int, c_int, ctypes.c_double, c_void_p, c_void_p, c_void_p],

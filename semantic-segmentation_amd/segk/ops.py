@@ -11,8 +11,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, NCHW, PM, AttentionArgs, ConvArgs, GemmArgs, GemmTnArgs, QkNormRotaryArgs, WgradArgs, \
-    WgradGroupArgs, call
+from ._lib import ATTENTION_ARGS, BF16, F32, NCHW, PM, QK_NORM_ROTARY_ARGS, WORKSPACE_ARGS, ConvArgs, GemmArgs, GemmTnArgs, \
+    WgradArgs, WgradGroupArgs, call
 from ._tables import StagedTable
 
 
@@ -866,85 +866,80 @@ def dot(a, b):
 
 
 # ------------------------------------------------------ multi-head attention ----
-class _on_device:
-    """Makes the device of the operands current around a launch (a stream belongs to its device)."""
+def _launch_packed(name, args, t):
+    """call(name, packed arguments, stream) on the device of tensor t (a stream belongs to its device)."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        call(name, args, _stream())
+    else:
+        with torch.cuda.device(index):
+            call(name, args, _stream())
 
-    def __init__(self, t):
-        self.index = t.device.index
 
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.old != self.index:
-            torch.cuda.set_device(self.old)
+def _with_workspace(args, need, t):
+    """(packed arguments with `need` bytes of workspace, the tensor that owns them)."""
+    ws = torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
+    return args + WORKSPACE_ARGS.pack(ws.data_ptr() if need else 0, need), ws
 
 
 def attention_operand_ok(t):
     """Whether a [N, L, heads, D] tensor can be read where it lies: unit stride over D, 16-byte aligned rows."""
-    per = 16 // t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 != 0:
+    n, l, h, d = t.stride()
+    per = 4 if t.dtype == torch.float32 else 8
+    if d != 1 or t.data_ptr() % 16 != 0:
         return False
-    return all(t.stride(i) % per == 0 or t.shape[i] == 1 for i in range(3))
+    if n % per == 0 and l % per == 0 and h % per == 0:
+        return True
+    z = t.shape
+    return (n % per == 0 or z[0] == 1) and (l % per == 0 or z[1] == 1) and (h % per == 0 or z[2] == 1)
 
 
-def _attention_view(view, t, name):
+def _attention_view(t, name):
     if not attention_operand_ok(t):
         raise ValueError("%s needs unit stride over its channels and 16-byte aligned rows, got strides %s" % (name, t.stride()))
-    s, z = t.stride(), t.shape
-    view.p = t.data_ptr()
-    view.n, view.l, view.h = (s[0] if z[0] > 1 else 0), (s[1] if z[1] > 1 else 0), (s[2] if z[2] > 1 else 0)
+    (n, l, h, _), z = t.stride(), t.shape
+    return t.data_ptr(), (n if z[0] > 1 else 0), (l if z[1] > 1 else 0), (h if z[2] > 1 else 0)
+
+
+_NO_VIEW = (0, 0, 0, 0)
 
 
 def _attention_args(q, k, v, out, scale, causal, mask, key_mask):
+    """Checked arguments as far as key_mask_k: (tuple of fields, shape, lse and gradients to follow)."""
     _dev(q, k, v, out, mask, key_mask)
+    dtype, device = q.dtype, q.device
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         if t.dim() != 4:
             raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
-        if t.dtype != q.dtype or t.device != q.device:
+        if t.dtype != dtype or t.device != device:
             raise ValueError("attention operands share one dtype and device (q: %s on %s, %s: %s on %s)"
-                             % (q.dtype, q.device, name, t.dtype, t.device))
+                             % (dtype, device, name, t.dtype, t.device))
     N, Lq, Hq, D = q.shape
-    Lk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != N or k.shape[3] != D or out.shape != q.shape:
+    kn, Lk, Hk, kd = k.shape
+    if k.shape != v.shape or kn != N or kd != D or out.shape != q.shape:
         raise ValueError("attention shapes disagree: q %s k %s v %s out %s"
                          % (tuple(q.shape), tuple(k.shape), tuple(v.shape), tuple(out.shape)))
     if Hk == 0 or Hq % Hk != 0:
         raise ValueError("%d query heads cannot share %d key / value heads evenly" % (Hq, Hk))
-    a = AttentionArgs()
-    a.N, a.Lq, a.Lk, a.Hq, a.Hk, a.D = N, Lq, Lk, Hq, Hk, D
-    a.dtype, a.causal, a.scale = _dt(q), 1 if causal else 0, scale
-    _attention_view(a.q, q, "q")
-    _attention_view(a.out, out, "out")
-    if Lk > 0:
-        _attention_view(a.k, k, "k")
-        _attention_view(a.v, v, "v")
-    for t, name in ((mask, "mask"), (key_mask, "key_mask")):
-        if t is not None and (t.dtype != torch.bool or t.device != q.device):
-            raise ValueError("%s must be a bool tensor on %s, got %s on %s" % (name, q.device, t.dtype, t.device))
+    dt = _dt(q)
+    m, km = (0, 0, 0, 0, 0), (0, 0, 0)
     if mask is not None:
-        if mask.dim() != 4 or any(m != f and m != 1 for m, f in zip(mask.shape, (N, Hq, Lq, Lk))):
+        if mask.dtype != torch.bool or mask.device != device:
+            raise ValueError("mask must be a bool tensor on %s, got %s on %s" % (device, mask.dtype, mask.device))
+        if mask.dim() != 4 or any(z != f and z != 1 for z, f in zip(mask.shape, (N, Hq, Lq, Lk))):
             raise ValueError("mask of shape %s does not broadcast to [N, heads, Lq, Lk] = %s"
                              % (tuple(mask.shape), (N, Hq, Lq, Lk)))
-        a.mask = mask.data_ptr()
-        a.mask_n, a.mask_h, a.mask_q, a.mask_k = (0 if z == 1 else s for s, z in zip(mask.stride(), mask.shape))
+        m = (mask.data_ptr(),) + tuple(0 if z == 1 else s for s, z in zip(mask.stride(), mask.shape))
     if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.device != device:
+            raise ValueError("key_mask must be a bool tensor on %s, got %s on %s" % (device, key_mask.dtype, key_mask.device))
         if tuple(key_mask.shape) != (N, Lk):
             raise ValueError("key_mask of shape %s, expected [N, Lk] = %s" % (tuple(key_mask.shape), (N, Lk)))
-        a.key_mask = key_mask.data_ptr()
-        a.key_mask_n, a.key_mask_k = key_mask.stride()
-    return a
-
-
-def _attention_workspace(a, backward, device):
-    need = call("segk_attention_workspace", ctypes.byref(a), 1 if backward else 0)
-    if need == 0:
-        return None
-    ws = torch.empty((need,), dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    return ws
+        km = (key_mask.data_ptr(),) + key_mask.stride()
+    views = _attention_view(q, "q")
+    views += _attention_view(k, "k") + _attention_view(v, "v") if Lk > 0 else _NO_VIEW + _NO_VIEW
+    views += _attention_view(out, "out")
+    return (N, Lq, Lk, Hq, Hk, D, dt, 1 if causal else 0, ctypes.c_float(scale).value) + views, m + km
 
 
 def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, want_lse=False):
@@ -952,37 +947,36 @@ def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, w
     h // (Hq // Hk); any strides with unit stride over D and 16-byte aligned rows; D a multiple of 8 up to 128.
     mask: bool, broadcastable to [N, Hq, Lq, Lk], True = open; key_mask: bool [N, Lk]; causal: key j is open to token i
     for j <= i + Lk - Lq.  -> lse [N, Hq, Lq] float32 (None unless wanted)."""
-    a = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
-    lse = torch.empty((a.N, a.Hq, a.Lq), dtype=torch.float32, device=q.device) if want_lse else None
-    if a.N == 0 or a.Lq == 0:
+    head, masks = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
+    N, Lq, Hq = head[0], head[1], head[3]
+    lse = torch.empty((N, Hq, Lq), dtype=torch.float32, device=q.device) if want_lse else None
+    if N == 0 or Lq == 0:
         return lse
-    with _on_device(q):
-        a.lse = lse.data_ptr() if want_lse else None
-        ws = _attention_workspace(a, False, q.device)  # noqa: F841 (held until the launch)
-        call("segk_attention_fwd", ctypes.byref(a), _stream())
+    args = ATTENTION_ARGS.pack(*head, lse.data_ptr() if want_lse else 0, *masks, *_NO_VIEW, 0, 0, 0)
+    args, ws = _with_workspace(args, call("segk_attention_workspace", args + bytes(16), 0), q)
+    _launch_packed("segk_attention_fwd", args, q)
     return lse
 
 
 def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_mask=None, need_dq=True, need_dkv=True):
     """Gradients (dq, dk, dv) of attention_fwd, contiguous, of the operands' dtype; None where not wanted."""
-    a = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
+    head, masks = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
+    N, Lq, Lk, Hq = head[:4]
     if dout.shape != out.shape or dout.dtype != out.dtype or dout.device != out.device:
         raise ValueError("dout %s %s does not match out %s %s" % (tuple(dout.shape), dout.dtype, tuple(out.shape), out.dtype))
-    if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (a.N, a.Hq, a.Lq) or lse.device != q.device:
+    if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (N, Hq, Lq) or lse.device != q.device:
         raise ValueError("lse must be contiguous float32 [N, Hq, Lq]")
-    new = torch.empty if a.N > 0 and a.Lq > 0 and a.Lk > 0 else torch.zeros
+    some = N > 0 and Lq > 0 and Lk > 0
+    new = torch.empty if some else torch.zeros
     dq = new(q.shape, dtype=q.dtype, device=q.device) if need_dq else None
     dk = new(k.shape, dtype=q.dtype, device=q.device) if need_dkv else None
     dv = new(k.shape, dtype=q.dtype, device=q.device) if need_dkv else None
-    if new is torch.zeros or not (need_dq or need_dkv):
+    if not some or not (need_dq or need_dkv):
         return dq, dk, dv
-    _attention_view(a.dout, dout, "dout")
-    with _on_device(q):
-        a.lse = lse.data_ptr()
-        a.dq = dq.data_ptr() if need_dq else None
-        a.dk, a.dv = (dk.data_ptr(), dv.data_ptr()) if need_dkv else (None, None)
-        ws = _attention_workspace(a, True, q.device)  # noqa: F841 (held until the launch)
-        call("segk_attention_bwd", ctypes.byref(a), _stream())
+    args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), *masks, *_attention_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
+                               dk.data_ptr() if need_dkv else 0, dv.data_ptr() if need_dkv else 0)
+    args, ws = _with_workspace(args, call("segk_attention_workspace", args + bytes(16), 1), q)
+    _launch_packed("segk_attention_bwd", args, q)
     return dq, dk, dv
 
 
@@ -990,30 +984,31 @@ _POS_DTYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
 def _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved):
+    """Checked arguments: (N .. dtype and the views of q and k, the weights, positions .. eps)."""
     _dev(q, k, q_weight, k_weight, positions, inv_freq)
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None:
-            continue
-        if t.dim() != 4:
-            raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
-        if t.dtype != q.dtype or t.device != q.device or t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3]:
-            raise ValueError("queries %s %s and keys %s %s share images, tokens, head size, dtype and device"
-                             % (tuple(q.shape), q.dtype, tuple(t.shape), t.dtype))
+    device = q.device
+    if q.dim() != 4:
+        raise ValueError("q must be [N, L, heads, D], got shape %s" % (tuple(q.shape),))
     N, L, Hq, D = q.shape
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.device != device or k.shape[:2] != q.shape[:2]
+                          or k.shape[3] != D):
+        raise ValueError("queries %s %s and keys %s %s share images, tokens, head size, dtype and device"
+                         % (tuple(q.shape), q.dtype, tuple(k.shape), k.dtype))
     for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (D,) or not t.is_contiguous() or t.device != q.device):
-            raise ValueError("%s must be contiguous float32 [%d] on %s, got %s %s" % (name, D, q.device, tuple(t.shape), t.dtype))
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != D or not t.is_contiguous()
+                              or t.device != device):
+            raise ValueError("%s must be contiguous float32 [%d] on %s, got %s %s" % (name, D, device, tuple(t.shape), t.dtype))
     if eps is None and (q_weight is not None or k_weight is not None):
         raise ValueError("weights belong to the norm: none without eps")
     axes = positions.shape[-1] if positions.dim() in (2, 3) else 0
     if not 1 <= axes <= 4 or tuple(positions.shape[:-1]) not in ((L,), (N, L)):
         raise ValueError("positions must be [L, axes] or [N, L, axes] with 1 to 4 axes, got %s for N=%d L=%d"
                          % (tuple(positions.shape), N, L))
-    if positions.dtype not in _POS_DTYPES or positions.device != q.device:
+    if positions.dtype not in _POS_DTYPES or positions.device != device:
         raise ValueError("positions must be int32, int64 or float32 on %s, got %s on %s"
-                         % (q.device, positions.dtype, positions.device))
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != q.device:
-        raise ValueError("inv_freq must be contiguous float32 of one dimension on %s" % (q.device,))
+                         % (device, positions.dtype, positions.device))
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != device:
+        raise ValueError("inv_freq must be contiguous float32 of one dimension on %s" % (device,))
     pairs = inv_freq.shape[0]
     if sections is None:
         if pairs % axes != 0:
@@ -1021,67 +1016,51 @@ def _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, i
         sections = (pairs // axes,) * axes
     if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
         raise ValueError("sections %s: %d axes share %d pairs" % (tuple(sections), axes, pairs))
-    a = QkNormRotaryArgs()
-    a.N, a.L, a.Hq, a.Hk, a.D, a.dtype = N, L, Hq, (0 if k is None else k.shape[2]), D, _dt(q)
-    _attention_view(a.q, q, "q")
-    if k is not None:
-        _attention_view(a.k, k, "k")
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    a.positions, a.pos_dtype, a.axes = positions.data_ptr(), _POS_DTYPES[positions.dtype], axes
     s = positions.stride()
-    a.pos_n, a.pos_l, a.pos_a = (s[0] if positions.dim() == 3 else 0), s[-2], s[-1]
-    for i, z in enumerate(sections):
-        a.section[i] = z
-    a.inv_freq, a.interleaved = inv_freq.data_ptr(), 1 if interleaved else 0
-    a.norm, a.eps = (0, 0.0) if eps is None else (1, eps)
-    return a
+    head = (N, L, Hq, 0 if k is None else k.shape[2], D, _dt(q)) + _attention_view(q, "q") \
+        + (_NO_VIEW if k is None else _attention_view(k, "k"))
+    weights = (q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0)
+    rest = (positions.data_ptr(), _POS_DTYPES[positions.dtype], s[0] if len(s) == 3 else 0, s[-2], s[-1], axes) \
+        + tuple(sections) + (0,) * (4 - axes) \
+        + (inv_freq.data_ptr(), 0 if eps is None else 1, 1 if interleaved else 0, 0.0 if eps is None else ctypes.c_float(eps).value)
+    return head, weights, rest
 
 
 def qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, interleaved=False):
     """Norm and rotation of the heads of q [N, L, Hq, D] and k [N, L, Hk, D] (or None) in one pass -> contiguous
     (q', k').  Operands as attention_fwd, D up to 256; eps None: rotation only.  segk.functional.qk_norm_rotary has the
     formula."""
-    a = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
+    head, weights, rest = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k is not None else None
-    if a.N == 0 or a.L == 0:
-        return q_out, k_out
-    a.q_out = q_out.data_ptr()
-    a.k_out = k_out.data_ptr() if k is not None else None
-    with _on_device(q):
-        call("segk_qk_norm_rotary", ctypes.byref(a), _stream())
+    if q.shape[0] > 0 and q.shape[1] > 0:
+        args = QK_NORM_ROTARY_ARGS.pack(*head, q_out.data_ptr(), 0 if k is None else k_out.data_ptr(), *weights, *rest,
+                                        *_NO_VIEW, *_NO_VIEW, 0, 0)
+        _launch_packed("segk_qk_norm_rotary", args + bytes(16), q)
     return q_out, k_out
 
 
 def qk_norm_rotary_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6,
                        interleaved=False, need_weights=(True, True)):
     """Gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rotary_fwd; weight gradients (float32) where wanted."""
-    a = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
+    head, weights, rest = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
     for g, t in ((dq_out, q), (dk_out, k)):
         if t is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
             raise ValueError("gradient %s %s does not match %s %s" % (tuple(g.shape), g.dtype, tuple(t.shape), t.dtype))
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k is not None else None
-    none = a.N == 0 or a.L == 0
-    new = torch.zeros if none else torch.empty
-    dqw = new(a.D, dtype=torch.float32, device=q.device) if need_weights[0] and q_weight is not None else None
-    dkw = new(a.D, dtype=torch.float32, device=q.device) if need_weights[1] and k_weight is not None else None
-    if none:
+    some = q.shape[0] > 0 and q.shape[1] > 0
+    new = torch.empty if some else torch.zeros
+    dqw = new(q.shape[3], dtype=torch.float32, device=q.device) if need_weights[0] and q_weight is not None else None
+    dkw = new(q.shape[3], dtype=torch.float32, device=q.device) if need_weights[1] and k_weight is not None else None
+    if not some:
         return dq, dk, dqw, dkw
-    _attention_view(a.dq, dq_out, "dq")
-    a.q_out = dq.data_ptr()
-    if k is not None:
-        _attention_view(a.dk, dk_out, "dk")
-        a.k_out = dk.data_ptr()
-    a.dq_weight = dqw.data_ptr() if dqw is not None else None
-    a.dk_weight = dkw.data_ptr() if dkw is not None else None
-    with _on_device(q):
-        need = call("segk_qk_norm_rotary_bwd_workspace", ctypes.byref(a))
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        call("segk_qk_norm_rotary_bwd", ctypes.byref(a), _stream())
+    args = QK_NORM_ROTARY_ARGS.pack(*head, dq.data_ptr(), 0 if k is None else dk.data_ptr(), *weights, *rest,
+                                    *_attention_view(dq_out, "dq"), *(_NO_VIEW if k is None else _attention_view(dk_out, "dk")),
+                                    0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr())
+    need = call("segk_qk_norm_rotary_bwd_workspace", args + bytes(16))
+    args, ws = _with_workspace(args, need, q)
+    _launch_packed("segk_qk_norm_rotary_bwd", args, q)
     return dq, dk, dqw, dkw
 
 
