@@ -13,6 +13,8 @@
 // row r = token r / G, head r % G of the group.  Keys and values are then read once for the group, and the gradient of a
 // shared head is a sum over rows inside one workgroup.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 namespace segk {
@@ -46,20 +48,47 @@ struct AttnDev {
   unsigned g_magic;               // r / G = umulhi(r, g_magic) for G > 1
   int causal, off;                // key j is open to token i when j <= i + off, off = Lk - Lq
   float scale, scale_log2;
-  int tiles, splits;              // workgroup tiles of one problem, parts of the looped axis
-  float* part;                    // partial results of the splits
-  float* part_ml;
-  float *row_lse2, *row_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and rowsum(dout * out)
+  int tiles;                      // workgroup tiles of one problem
+  int whole, rest, parts, rest_x; // how the tiles are dealt out, see attn_deal
+  float* part;                    // partial results: [rest][parts][rows of a tile][D] (dk and dv: one after the other)
+  float* part_ml;                 // [rest][parts][rows of a tile][2]: maxima and sums of the forward pass
+  float *row_lse2, *minus_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and -rowsum(dout * out)
 };
 
 __device__ __forceinline__ int div_g(const AttnDev& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.g_magic); }
 
-// Workgroup -> piece of work such that the workgroups of one XCD (blockIdx % 8 in launch order) take neighbouring
-// pieces: the tiles of one head share its keys and values in that XCD's L2.  Returns -1 for the grid's padding.
-__device__ __forceinline__ int xcd_contiguous(int total) {
-  const int per = (int)(gridDim.x >> 3);
-  const int w = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-  return w < total ? w : -1;
+// What a workgroup does.  The tiles of all problems are numbered; the first `whole` of them (full rounds of the chip) go to
+// one workgroup each, the `rest` that would leave most of the chip idle for a round are cut along their loop into `parts`
+// parts, whose results another kernel joins in part order.  A problem with few tiles is all rest.  Workgroups of one XCD
+// (blockIdx % 8 in launch order) take neighbouring tiles, or the same part of neighbouring tiles: they share keys and
+// values (rows, in the backward pass over keys) in that XCD's L2.
+struct AttnWork {
+  int n, hk, tile;   // n < 0: nothing
+  int part, parts;
+  int slot;          // number among the tiles that are cut
+};
+__device__ __forceinline__ void attn_decode_tile(const AttnDev& p, int g, AttnWork* w) {
+  w->tile = g % p.tiles;
+  g /= p.tiles;
+  // (under the diagonal the last tiles are the longest: they start first)
+  if (p.causal) w->tile = p.tiles - 1 - w->tile;
+  w->hk = g % p.Hk;
+  w->n = g / p.Hk;
+}
+__device__ __forceinline__ AttnWork attn_work(const AttnDev& p) {
+  AttnWork w = {-1, 0, 0, 0, 1, 0};
+  const int x = (int)blockIdx.x & 7, i = (int)blockIdx.x >> 3, whole_x = p.whole >> 3;
+  if (i < whole_x) {
+    if (x * whole_x + i < p.tiles * p.N * p.Hk) attn_decode_tile(p, x * whole_x + i, &w);
+    return w;
+  }
+  const int u = x * p.rest_x + i - whole_x;
+  if (u >= p.rest * p.parts) return w;
+  w.part = u / p.rest;
+  w.parts = p.parts;
+  w.slot = u - w.part * p.rest;
+  attn_decode_tile(p, p.whole + w.slot, &w);
+  return w;
 }
 
 template <typename T>
@@ -109,23 +138,66 @@ __device__ __forceinline__ AttnFrag<float> pack_frag<float>(const f32x16& s, int
   return f;
 }
 
+// 8 probabilities as an operand, and their sum added to `sum` (unrounded: lse is an fp32 statistic).
+template <typename T>
+__device__ __forceinline__ AttnFrag<T> pack_sum(const float* x, float& sum);
+template <>
+__device__ __forceinline__ AttnFrag<bf16_t> pack_sum<bf16_t>(const float* x, float& sum) {
+  f32x8 y;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    y[j] = x[j];
+    sum += x[j];
+  }
+  AttnFrag<bf16_t> f;
+  f.v = __builtin_bit_cast(u32x4, __builtin_convertvector(y, attn_bf16x8));
+  return f;
+}
+template <>
+__device__ __forceinline__ AttnFrag<float> pack_sum<float>(const float* x, float& sum) {
+  AttnFrag<float> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f.v[j] = x[j];
+    sum += x[j];
+  }
+  return f;
+}
+
 // ---- tiles in LDS -------------------------------------------------------------------------------
 // Rows of DP elements at a pitch of a power of two; the 16-byte chunks of a row are permuted by XOR with a function of
-// the row chosen so that (a) eight lanes that read the same chunk of eight neighbouring rows (AttnRead::rows) and (b) sixteen
-// lanes that read a 32-byte piece of four neighbouring rows (cols, bf16) meet distinct LDS banks.
+// the row.  LDS serves 256 bytes a clock: 16 lanes of a 16-byte read (AttnRead::rows: the same chunk of 16 neighbouring
+// rows), 32 lanes of an 8-byte transposing read (cols in bf16: 64 bytes of four neighbouring rows) or 64 lanes of a 4-byte
+// read (cols in fp32: 128 bytes of two rows, four apart).  swz() gives each of these groups distinct banks (fp32 columns of
+// 128-byte rows excepted: both rows lie in the same half).
 template <typename T, int DP>
 struct AttnTile {
   static constexpr int ES = sizeof(T);
   static constexpr int PITCH = DP * ES <= 64 ? 64 : DP * ES <= 128 ? 128 : DP * ES <= 256 ? 256 : 512;
-  static constexpr int CPR = PITCH / 16;     // chunks per row
-  static constexpr int ROWS_1K = 1024 / PITCH;
   static __device__ __forceinline__ int swz(int row) {
     if (PITCH == 64) return (row >> 2) & 3;
-    if (PITCH == 128) return (((row >> 1) & 1) << 1) | ((row >> 2) & 1) | (((row >> 3) & 1) << 2);
-    if (PITCH == 256) return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8);
-    return ((row & 3) << 1) | ((row >> 2) & 1);
+    if (PITCH == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    if (ES == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+    return (((row >> 2) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1);
   }
   static __device__ __forceinline__ int at(int row, int chunk) { return row * PITCH + ((chunk ^ swz(row)) << 4); }
+};
+
+// One lane's share of staging a tile by LDS-DMA: the tile is cut into 1-KiB pieces, wavefront w takes pieces w, w + 4, ...;
+// piece i of a wavefront holds rows row + i * STEP, and the lane fetches chunk(i) of its row (the DMA writes lanes in
+// order, so the permutation is applied to what a lane reads).
+template <typename T, int DP>
+struct AttnPiece {
+  typedef AttnTile<T, DP> Tile;
+  static constexpr int STEP = 4096 / Tile::PITCH;
+  int row, chunk0;
+  __device__ __forceinline__ AttnPiece(int wave, int lane) {
+    const int lin = wave * 1024 + lane * 16;
+    row = lin / Tile::PITCH;
+    chunk0 = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(row);
+  }
+  // (STEP is a period of swz but for the 512-byte pitch, where every other piece flips its lowest bit)
+  __device__ __forceinline__ int chunk(int i) const { return Tile::PITCH == 512 ? chunk0 ^ (i & 1) : chunk0; }
 };
 
 // rows(): operand fragment contracted along the tile's rows in memory: lane (l & 31, h) reads elements 16 ks + 8 h .. + 7
@@ -141,6 +213,9 @@ struct AttnRead<bf16_t, DP> {
     AttnFrag<bf16_t> f;
     f.v = *reinterpret_cast<const u32x4*>(tile + Tile::at(row0 + (lane & 31), 2 * ks + (lane >> 5)));
     return f;
+  }
+  static __device__ __forceinline__ void write_rows(char* tile, int row0, int ks, int lane, const AttnFrag<bf16_t>& f) {
+    *reinterpret_cast<u32x4*>(tile + Tile::at(row0 + (lane & 31), 2 * ks + (lane >> 5))) = f.v;
   }
   static __device__ __forceinline__ AttnFrag<bf16_t> cols(const char* tile, int row0, int d0, int lane) {
     // a group of 16 lanes reads a block of 4 rows x 16 columns, 8 bytes a lane, and receives it transposed
@@ -171,6 +246,12 @@ struct AttnRead<float, DP> {
       for (int e = 0; e < 4; ++e) f.v[4 * j + e] = t[e];
     }
     return f;
+  }
+  static __device__ __forceinline__ void write_rows(char* tile, int row0, int ks, int lane, const AttnFrag<float>& f) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<f32x4*>(tile + Tile::at(row0 + (lane & 31), 4 * ks + 2 * (lane >> 5) + j)) =
+          f32x4{f.v[4 * j], f.v[4 * j + 1], f.v[4 * j + 2], f.v[4 * j + 3]};
   }
   static __device__ __forceinline__ AttnFrag<float> cols(const char* tile, int row0, int d0, int lane) {
     const int d = d0 + (lane & 31);
@@ -272,19 +353,17 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Stages tiles of KT keys and their values: piece i of a wavefront is rows st_row + i * (4096 / PITCH) of a tile.
+// Stages tiles of KT keys and their values.
 template <typename T, int DP>
 struct AttnStage {
   typedef AttnTile<T, DP> Tile;
-  int row, chunk;
-  bool ok;
+  typedef AttnPiece<T, DP> Piece;
+  Piece pc;
+  int row_b;               // bytes of a row that exist
   unsigned k_step, v_step, lds0;
   const char *kbase, *vbase;
-  __device__ __forceinline__ AttnStage(const AttnDev& p, int n, int hk, int wave, int lane, const char* smem) {
-    const int lin = wave * 1024 + lane * 16;
-    row = lin / Tile::PITCH;
-    chunk = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(row);     // (4096 / PITCH is a period of swz)
-    ok = chunk * 16 < p.D * (int)sizeof(T);
+  __device__ __forceinline__ AttnStage(const AttnDev& p, int n, int hk, int wave, int lane, const char* smem) : pc(wave, lane) {
+    row_b = p.D * (int)sizeof(T);
     k_step = (unsigned)(p.k.l * (int)sizeof(T)), v_step = (unsigned)(p.v.l * (int)sizeof(T));
     kbase = p.k.p + ((long long)n * p.k.n + (long long)hk * p.k.h) * (int)sizeof(T);
     vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
@@ -295,14 +374,22 @@ struct AttnStage {
   __device__ __forceinline__ void keys(const AttnDev& p, int key0, int buf, const unsigned long long* bits) const {
     constexpr int TILE_B = KT * Tile::PITCH;
     const u32x4 kr = buffer_of(kbase + (long long)key0 * k_step), vr = buffer_of(vbase + (long long)key0 * v_step);
+    const bool inside = !MASKED && key0 + KT <= p.Lk;
 #pragma unroll
     for (int i = 0; i < TILE_B / 4096; ++i) {
-      const int x = row + i * (4096 / Tile::PITCH);
-      bool in = ok && key0 + x < p.Lk;
-      if (MASKED) in = in && ((bits[i * (4096 / Tile::PITCH) >> 6] >> (x & 63)) & 1);
+      const int x = pc.row + i * Piece::STEP, c = pc.chunk(i) * 16;
       const unsigned lds = lds0 + buf * (2 * TILE_B) + i * 4096;
-      dma_1k(kr, lds, in ? x * k_step + chunk * 16 : ATTN_OOB);
-      dma_1k(vr, lds + TILE_B, in ? x * v_step + chunk * 16 : ATTN_OOB);
+      // (a row's missing chunks are the same in every tile)
+      const unsigned ko = c < row_b ? x * k_step + c : ATTN_OOB, vo = c < row_b ? x * v_step + c : ATTN_OOB;
+      if (inside) {
+        dma_1k(kr, lds, ko);
+        dma_1k(vr, lds + TILE_B, vo);
+      } else {
+        bool in = key0 + x < p.Lk;
+        if (MASKED) in = in && ((bits[i * Piece::STEP >> 6] >> (x & 63)) & 1);
+        dma_1k(kr, lds, in ? ko : ATTN_OOB);
+        dma_1k(vr, lds + TILE_B, in ? vo : ATTN_OOB);
+      }
     }
   }
 };
@@ -373,20 +460,36 @@ struct AttnPairMask {
   }
 };
 
-// max over the two lanes that share a result column
-__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+// maximum and sum over the two lanes that share a result column (l and l ^ 32)
+__device__ __forceinline__ float pair_max(float v) {
+  const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// Keeps a rarely taken uniform branch a branch (the compiler would compute both sides and select).
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// host side, attn_fwd.hip
-int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);
+// ---- host side ----------------------------------------------------------------------------------
+int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);                 // attn_fwd.hip
 bool attn_few(const AttnDev& p, int dtype);
-int launch_attn_dkv(AttnDev p, int dtype, hipStream_t st);   // attn_dkv.hip
-int launch_attn_dq(AttnDev p, int dtype, hipStream_t st);    // attn_dq.hip
-int launch_attn_sum(const float* part, long long part_stride, int parts, float scale, char* out, long long count, int dtype,
-                    hipStream_t st);
-int attn_dkv_splits(const AttnDev& p, int dtype);
-int attn_dq_splits(const AttnDev& p, int dtype);
+// Deals p->tiles of every problem out to workgroups of which `per_cu` share a CU; `steps`: length of a tile's loop, of
+// which a part takes at least min_steps.  Returns the grid.
+long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps);
+// Sets a kernel's LDS limit and returns how many of its workgroups share a CU (negative: status); `seen` keeps the answer
+// for each device.
+constexpr int ATTN_DEVICES = 64;
+int attn_occupancy(const void* kernel, int lds, std::atomic<int>* seen);
+// Each fills in the deal and, unless plan_only, launches.
+int attn_dkv(AttnDev* p, int dtype, bool plan_only, hipStream_t st);                     // attn_dkv.hip
+int attn_dq(AttnDev* p, int dtype, bool plan_only, hipStream_t st);                      // attn_dq.hip
+static inline long long attn_part_floats(const AttnDev& p, int tile_rows, int floats_per_row) {
+  return p.parts > 1 ? (long long)p.rest * p.parts * tile_rows * floats_per_row : 0;
+}
 
 }  // namespace segk

@@ -6,42 +6,49 @@
 
 namespace segk {
 
-constexpr int QT = 64;   // rows per step
+#ifndef DKV_W
+#define DKV_W 2
+#endif
+
+template <typename T, int DP>
+constexpr bool dkv_v_in_lds() { return DP * (int)sizeof(T) >= 192; }
+template <typename T, int DP>
+constexpr int dkv_rows() { return dkv_v_in_lds<T, DP>() ? 32 : 64; }
 
 // 4 wavefronts of 32 keys.  Scores are computed with queries as rows (a lane owns one key), so P and dS are the operands
-// of dV^T = dO^T P and dK^T = Q^T dS as they lie; K and V of the wavefront's keys stay in registers, Q and dO tiles of 64
-// rows are staged through LDS and read both along rows and along columns.
+// of dV^T = dO^T P and dK^T = Q^T dS as they lie.  K of the wavefront's keys stays in registers; Q and dO tiles of QT rows
+// are staged through LDS and read both along rows and along columns.
+// V stays in registers too where the heads are small; where they are not (VL) it lies in LDS: 32 registers less bring two
+// wavefronts to a SIMD, which cover each other's exponentials, for a quarter more LDS reads.
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2)) void attn_dkv_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : DKV_W)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
+  typedef AttnPiece<T, DP> Piece;
+  constexpr bool VL = dkv_v_in_lds<T, DP>();
+  constexpr int QT = dkv_rows<T, DP>();
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = QT * Tile::PITCH;
-  constexpr int NP = TILE_B / 4096;
-  constexpr int STAGE_B = 2 * TILE_B + 512;      // Q tile, dO tile, 64 lse, 64 delta
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int STAGE_B = 2 * TILE_B + 512;      // Q tile, dO tile, lse, delta
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 stages, V (VL)
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int w = xcd_contiguous(p.tiles * p.splits * p.N * p.Hk);
-  if (w < 0) return;
-  const int split = w % p.splits;
-  w /= p.splits;
-  const int tile = w % p.tiles;
-  w /= p.tiles;
-  const int hk = w % p.Hk, n = w / p.Hk;
-  const int key_wg = tile * 128;
+  const AttnWork w = attn_work(p);
+  if (w.n < 0) return;
+  const int n = w.n, hk = w.hk;
+  const int key_wg = w.tile * 128;
   const int key = key_wg + wave * 32 + l31;
 
-  const int all_steps = p.Rp / QT;
+  const int all_steps = (p.R + QT - 1) / QT;
   int first = 0;
-  if (p.causal) first = min(all_steps, max(0, key_wg - p.off) >= p.Lq ? all_steps : max(0, key_wg - p.off) * p.G / QT);
-  const int per = (all_steps - first + p.splits - 1) / p.splits;
-  const int t0 = min(first + split * per, all_steps), t1 = min(t0 + per, all_steps);
+  if (p.causal) first = max(0, key_wg - p.off) >= p.Lq ? all_steps : max(0, key_wg - p.off) * p.G / QT;
+  const int per = (all_steps - first + w.parts - 1) / w.parts;
+  const int t0 = min(first + w.part * per, all_steps), t1 = min(t0 + per, all_steps);
 
   bool key_ok = key < p.Lk;
   if (MASKED && p.kmask && key_ok) key_ok = p.kmask[n * p.km_n + (long long)key * p.km_k] != 0;
-  AttnFrag<T> kf[KS], vf[KS];
+  AttnFrag<T> kf[KS], vf[VL ? 1 : KS];
   {
     const long long kk = key_ok ? key : 0;
     const char* ks_ = p.k.p + ((long long)n * p.k.n + kk * p.k.l + (long long)hk * p.k.h) * (int)sizeof(T);
@@ -49,23 +56,39 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       kf[ks] = load_frag<T>(ks_, ks, h, p.D, key_ok);
-      vf[ks] = load_frag<T>(vs_, ks, h, p.D, key_ok);
+      if (!VL) vf[ks] = load_frag<T>(vs_, ks, h, p.D, key_ok);
+    }
+    if (VL) {     // this wavefront's 32 rows of V, through registers, in the tiles' permutation
+      char* const vt = smem + 2 * STAGE_B;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) Rd::write_rows(vt, wave * 32, ks, lane, load_frag<T>(vs_, ks, h, p.D, key_ok));
     }
   }
 
-  const int lin = wave * 1024 + lane * 16;
-  const int st_row = lin / Tile::PITCH;
-  const int st_chunk = ((lin % Tile::PITCH) >> 4) ^ Tile::swz(st_row);
-  const bool st_ok = st_chunk * 16 < p.D * (int)sizeof(T);
+  const Piece pc(wave, lane);
+  const int row_b = p.D * (int)sizeof(T);
   const char* const qbase = p.q.p + ((long long)n * p.q.n + (long long)hk * p.G * p.q.h) * (int)sizeof(T);
   const char* const gbase = p.dout.p + ((long long)n * p.dout.n + (long long)hk * p.G * p.dout.h) * (int)sizeof(T);
   const float* const lse2 = p.row_lse2 + ((long long)n * p.Hk + hk) * p.Rp;
-  const float* const delta = p.row_delta + ((long long)n * p.Hk + hk) * p.Rp;
+  const float* const delta = p.minus_delta + ((long long)n * p.Hk + hk) * p.Rp;
   const unsigned char* const mkey =
       MASKED && p.mask ? p.mask + n * p.m_n + (long long)hk * p.G * p.m_h + (long long)(key < p.Lk ? key : 0) * p.m_k : nullptr;
   // Rows without an open key exist under masks and where the diagonal starts above the keys: they are not read, so that
   // whatever their memory holds meets no product.
   const bool empty_rows = MASKED || (p.causal && p.off < 0);
+  // Where the group's heads divide a tile evenly, a lane's place relative to the tile's first token never changes.
+  const bool even = QT % p.G == 0;
+  constexpr int NPC = TILE_B / 4096;
+  unsigned qo[NPC], go[NPC];
+  auto place = [&](int r, int tok0, int c, const AttnView& x) {
+    const int tok = div_g(p, r), hg = r - tok * p.G;
+    return c < row_b ? (unsigned)(((tok - tok0) * x.l + hg * x.h) * (int)sizeof(T)) + c : ATTN_OOB;
+  };
+#pragma unroll
+  for (int i = 0; i < NPC; ++i) {
+    qo[i] = place(pc.row + i * Piece::STEP, 0, pc.chunk(i) * 16, p.q);
+    go[i] = place(pc.row + i * Piece::STEP, 0, pc.chunk(i) * 16, p.dout);
+  }
   const unsigned lds0 = lds_addr(smem);
   auto stage = [&](int t, int buf) {
     const int row0 = t * QT;
@@ -73,19 +96,29 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
     const u32x4 qr = buffer_of(qbase + (long long)tok0 * p.q.l * (int)sizeof(T));
     const u32x4 gr = buffer_of(gbase + (long long)tok0 * p.dout.l * (int)sizeof(T));
     const unsigned at = lds0 + buf * STAGE_B;
+    static_assert(TILE_B % 4096 == 0, "every wavefront stages whole pieces");
+    if (even && !empty_rows && row0 + QT <= p.R) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int r = row0 + st_row + i * (4096 / Tile::PITCH);
-      bool ok = st_ok && r < p.R;
-      if (empty_rows && ok) ok = lse2[r] != INFINITY;
-      const int tok = div_g(p, r), hg = r - tok * p.G;
-      const unsigned qo = (unsigned)(((tok - tok0) * p.q.l + hg * p.q.h) * (int)sizeof(T)) + st_chunk * 16;
-      const unsigned go = (unsigned)(((tok - tok0) * p.dout.l + hg * p.dout.h) * (int)sizeof(T)) + st_chunk * 16;
-      dma_1k(qr, at + wave * 1024 + i * 4096, ok ? qo : ATTN_OOB);
-      dma_1k(gr, at + TILE_B + wave * 1024 + i * 4096, ok ? go : ATTN_OOB);
+      for (int i = 0; i < NPC; ++i) {
+        dma_1k(qr, at + wave * 1024 + i * 4096, qo[i]);
+        dma_1k(gr, at + TILE_B + wave * 1024 + i * 4096, go[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NPC; ++i) {
+        const int r = row0 + pc.row + i * Piece::STEP;
+        bool ok = r < p.R;
+        if (empty_rows && ok) ok = lse2[r] != INFINITY;
+        const unsigned a = even ? qo[i] : place(r, tok0, pc.chunk(i) * 16, p.q);
+        const unsigned b = even ? go[i] : place(r, tok0, pc.chunk(i) * 16, p.dout);
+        dma_1k(qr, at + wave * 1024 + i * 4096, ok ? a : ATTN_OOB);
+        dma_1k(gr, at + TILE_B + wave * 1024 + i * 4096, ok ? b : ATTN_OOB);
+      }
     }
-    if (wave == 0) dma_256(buffer_of((const char*)(lse2 + row0)), at + 2 * TILE_B, lane * 4);
-    if (wave == 1) dma_256(buffer_of((const char*)(delta + row0)), at + 2 * TILE_B + 256, lane * 4);
+    // (the statistics are padded to 64 rows: of a tile of 32 the lanes past it are told to read nothing)
+    const unsigned so = lane < QT ? lane * 4 : ATTN_OOB;
+    if (wave == 0) dma_256(buffer_of((const char*)(lse2 + row0)), at + 2 * TILE_B, so);
+    if (wave == 1) dma_256(buffer_of((const char*)(delta + row0)), at + 2 * TILE_B + 256, so);
   };
 
   f32x16 dk[DB], dv[DB];
@@ -93,17 +126,14 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
 
   if (t0 < t1) stage(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
     tile_barrier();
-    if (t + 1 < t1) stage(t + 1, buf ^ 1);
     const char* qt = smem + buf * STAGE_B;
     const char* gt = qt + TILE_B;
     const float* st = reinterpret_cast<const float*>(qt + 2 * TILE_B);
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
+    for (int rb = 0; rb < QT / 32; ++rb) {
       const int row0 = t * QT + rb * 32;
-      if (row0 >= p.R) break;
       unsigned char open[16];
       if (MASKED && mkey) {
 #pragma unroll
@@ -113,26 +143,29 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
           open[i] = mkey[(long long)(r - tok * p.G) * p.m_h + (long long)tok * p.m_q];
         }
       }
-      f32x16 s = zero16(), dp = zero16();
+      // the score gradients' products start from -delta
+      f32x16 s = zero16(), dp;
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 64 + rb * 32 + 2 * i + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[i + e] = dl[e];
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(qt, rb * 32, ks, lane), kf[ks]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(gt, rb * 32, ks, lane), vf[ks]);
-      float ls[16], dl[16];
+      for (int ks = 0; ks < KS; ++ks)
+        mma32(dp, Rd::rows(gt, rb * 32, ks, lane), VL ? Rd::rows(smem + 2 * STAGE_B, wave * 32, ks, lane) : vf[VL ? 0 : ks]);
+      if (rb == 0 && t + 1 < t1) stage(t + 1, buf ^ 1);     // (behind the first LDS reads, as in the forward kernel)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(st + rb * 32 + 2 * i + 4 * h);
-        const f32x4 b = *reinterpret_cast<const f32x4*>(st + 64 + rb * 32 + 2 * i + 4 * h);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(st + rb * 32 + 2 * i + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ls[i + e] = a[e];
-          dl[i + e] = b[e];
-        }
+        for (int e = 0; e < 4; ++e) s[i + e] = exp2_fast(fmaf(s[i + e], p.scale_log2, -ls[e]));
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = exp2_fast(fmaf(s[i], p.scale_log2, -ls[i]));
       // closed pairs (a closed key's products are those of zeros; the padding rows' lse is +inf)
       if (p.causal && key_wg + 127 > div_g(p, row0) + p.off) {
+        keep_branch();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int r = row0 + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -144,7 +177,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
         for (int i = 0; i < 16; ++i) s[i] = key_ok && (!mkey || open[i] != 0) ? s[i] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - dl[i]);
+      for (int i = 0; i < 16; ++i) dp[i] *= s[i];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const AttnFrag<T> pf = pack_frag<T>(s, j), sf = pack_frag<T>(dp, j);
@@ -155,11 +188,17 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
         }
       }
     }
+  };
+  int t = t0;
+  for (; t + 1 < t1; t += 2) {
+    step(t, 0);
+    step(t + 1, 1);
   }
+  if (t < t1) step(t, 0);
 
   if (key >= p.Lk) return;
   const long long at = (((long long)n * p.Lk + key) * p.Hk + hk) * p.D;
-  if (p.splits == 1) {
+  if (w.parts == 1) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -171,9 +210,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
         }
       }
   } else {
-    const long long all = (long long)p.N * p.Lk * p.Hk * p.D;
-    char* pk = (char*)(p.part + (long long)split * 2 * all + at);
-    char* pv = (char*)(p.part + (long long)split * 2 * all + all + at);
+    float* const at0 = p.part + (((long long)w.slot * p.parts + w.part) * 256 + wave * 32 + l31) * p.D;
+    char *const pk = (char*)at0, *const pv = (char*)(at0 + 128LL * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -187,74 +225,64 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 192 ? 1 : 2))
   }
 }
 
-// out = scale * sum over the parts, in part order; 4 elements a thread (every length is a multiple of 8)
+// Sums the parts of the tiles that were cut, in part order: 4 channels of one key a thread, dk and dv.
 template <typename T>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_sum_kernel(const float* __restrict__ part, long long part_stride, int parts,
-                                                                float scale, char* __restrict__ out, long long count) {
-  const long long i = ((long long)blockIdx.x * ATTN_THREADS + threadIdx.x) * 4;
-  if (i >= count) return;
-  f32x4 v = *reinterpret_cast<const f32x4*>(part + i);
-  for (int s = 1; s < parts; ++s) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * part_stride + i);
+__global__ __launch_bounds__(ATTN_THREADS) void attn_dkv_sum_kernel(const AttnDev p) {
+  const long long x = (long long)blockIdx.x * ATTN_THREADS + threadIdx.x;
+  const int quads = p.D / 4;
+  const long long line = x / quads;           // [rest][dk, dv][128]
+  const int d = (int)(x - line * quads) * 4;
+  if (line >= (long long)p.rest * 256) return;
+  const int slot = (int)(line >> 8), row = (int)(line & 127);
+  const bool is_v = (line & 128) != 0;
+  AttnWork w;
+  attn_decode_tile(p, p.whole + slot, &w);
+  const int key = w.tile * 128 + row;
+  if (key >= p.Lk) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.parts; ++s) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * 256 + (line & 255)) * p.D + d);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += x[e];
+    for (int e = 0; e < 4; ++e) v[e] += y[e];
   }
-  store4<T>(out + i * (int)sizeof(T), 0, v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
-}
-
-int launch_attn_sum(const float* part, long long part_stride, int parts, float scale, char* out, long long count, int dtype,
-                    hipStream_t st) {
-  const long long blocks = (count / 4 + ATTN_THREADS - 1) / ATTN_THREADS;
-  SEGK_UNSUPPORTED(blocks < 0x7fffffffLL, "attention_bwd: too many elements");
-  SEGK_DISPATCH_DTYPE(dtype, T, (attn_sum_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(part, part_stride, parts, scale, out, count)));
-  SEGK_CHECK_LAUNCH("attention_bwd sum");
-  return SEGK_OK;
-}
-
-int attn_dkv_splits(const AttnDev& p, int dtype) {
-  const long long blocks = (long long)ceil_div(p.Lk, 128) * p.N * p.Hk;
-  const int steps = p.Rp / QT;
-  if (blocks >= 256 || steps < 4) return 1;
-  long long s = (512 + blocks - 1) / blocks;
-  if (s > steps / 2) s = steps / 2;
-  return s < 1 ? 1 : (int)s;
+  const float scale = is_v ? 1.f : p.scale;
+  store4<T>((is_v ? p.dv : p.dk) + (((long long)w.n * p.Lk + key) * p.Hk + w.hk) * p.D * (int)sizeof(T), d, v[0] * scale, v[1] * scale,
+            v[2] * scale, v[3] * scale);
 }
 
 template <typename T, int DP>
-static int launch(const AttnDev& p, hipStream_t st) {
-  const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512);
-  const long long blocks = (long long)p.tiles * p.splits * p.N * p.Hk;
-  SEGK_UNSUPPORTED(blocks < 0x7ffffff0LL, "attention_bwd: too many workgroups");
-  auto kern = p.mask || p.kmask ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>;
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) {
-      set_error("attention_bwd: %s", hipGetErrorString(e));
-      return SEGK_HIP_ERROR;
-    }
-  }
-  kern<<<(unsigned)((blocks + 7) / 8 * 8), ATTN_THREADS, lds, st>>>(p);
+static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
+  constexpr int QT = dkv_rows<T, DP>();
+  const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + (dkv_v_in_lds<T, DP>() ? 128 * AttnTile<T, DP>::PITCH : 0);
+  static std::atomic<int> seen[2][ATTN_DEVICES];
+  const bool masked = p->mask || p->kmask;
+  auto kern = masked ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>;
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
+  if (per_cu < 0) return per_cu;
+  p->tiles = ceil_div(p->Lk, 128);
+  SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention_bwd: too many workgroups");
+  const long long grid = attn_deal(p, per_cu, ceil_div(p->R, QT), 2);
+  if (plan_only) return SEGK_OK;
+  kern<<<(unsigned)grid, ATTN_THREADS, lds, st>>>(*p);
   SEGK_CHECK_LAUNCH("attention_bwd keys");
+  if (p->parts > 1) {
+    const long long blocks = ((long long)p->rest * 256 * (p->D / 4) + ATTN_THREADS - 1) / ATTN_THREADS;
+    attn_dkv_sum_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(*p);
+    SEGK_CHECK_LAUNCH("attention_bwd keys' sum");
+  }
   return SEGK_OK;
 }
 
 template <typename T>
-static int dispatch(const AttnDev& p, hipStream_t st) {
-  if (p.D <= 32) return launch<T, 32>(p, st);
-  if (p.D <= 64) return launch<T, 64>(p, st);
-  if (p.D <= 96) return launch<T, 96>(p, st);
-  return launch<T, 128>(p, st);
+static int dispatch(AttnDev* p, bool plan_only, hipStream_t st) {
+  if (p->D <= 32) return launch<T, 32>(p, plan_only, st);
+  if (p->D <= 64) return launch<T, 64>(p, plan_only, st);
+  if (p->D <= 96) return launch<T, 96>(p, plan_only, st);
+  return launch<T, 128>(p, plan_only, st);
 }
 
-int launch_attn_dkv(AttnDev p, int dtype, hipStream_t st) {
-  p.tiles = ceil_div(p.Lk, 128);
-  p.splits = attn_dkv_splits(p, dtype);
-  const int rc = dtype == SEGK_BF16 ? dispatch<bf16_t>(p, st) : dispatch<float>(p, st);
-  if (rc != SEGK_OK || p.splits == 1) return rc;
-  const long long all = (long long)p.N * p.Lk * p.Hk * p.D;
-  const int rk = launch_attn_sum(p.part, 2 * all, p.splits, p.scale, p.dk, all, dtype, st);
-  if (rk != SEGK_OK) return rk;
-  return launch_attn_sum(p.part + all, 2 * all, p.splits, 1.f, p.dv, all, dtype, st);
+int attn_dkv(AttnDev* p, int dtype, bool plan_only, hipStream_t st) {
+  return dtype == SEGK_BF16 ? dispatch<bf16_t>(p, plan_only, st) : dispatch<float>(p, plan_only, st);
 }
 
 }  // namespace segk

@@ -18,13 +18,9 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int w = xcd_contiguous(p.tiles * p.splits * p.N * p.Hk);
-  if (w < 0) return;
-  const int split = w % p.splits;
-  w /= p.splits;
-  const int tile = w % p.tiles;
-  w /= p.tiles;
-  const int hk = w % p.Hk, n = w / p.Hk;
+  const AttnWork w = attn_work(p);
+  if (w.n < 0) return;
+  const int n = w.n, hk = w.hk, tile = w.tile;
   const int row0 = FEW ? 0 : tile * 128 + wave * 32;
   const bool idle = row0 >= p.R;
 
@@ -32,8 +28,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
   const int all_steps = (k_end + KT - 1) / KT;
-  const int per = (all_steps + p.splits - 1) / p.splits;
-  const int t0 = min(split * per, all_steps), t1 = min(t0 + per, all_steps);
+  const int per = (all_steps + w.parts - 1) / w.parts;
+  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
 
   const int r = row0 + l31;
   const bool row_in = r < p.R;
@@ -41,7 +37,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
   const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
   const long long stat = ((long long)n * p.Hk + hk) * p.Rp + rr;
   const float lse2 = row_in ? p.row_lse2[stat] : INFINITY;
-  const float delta = row_in ? p.row_delta[stat] : 0.f;
+  const float minus = row_in ? p.minus_delta[stat] : 0.f;
   const bool row_ok = lse2 != INFINITY;     // (rows without an open key are not read)
   AttnFrag<T> qf[KS], gf[KS];
   {
@@ -73,8 +69,15 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
     }
     st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
   }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  // The score gradients' products start from -delta where 16 registers can be spared for it.
+  constexpr bool START = DP * (int)sizeof(T) <= 128;
+  f32x16 start = zero16();
+  if (START) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) start[i] = minus;
+  }
+
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
     tile_barrier();
     const int key0 = t * KT + (FEW ? wave * 32 : 0);
     unsigned kw[NKB], pw[NKB][4];
@@ -96,29 +99,35 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
         dead = !__any(row_ok && some != 0);
       }
     }
-    if (t + 1 < t1) {
+    auto stage_next = [&]() {       // (behind the first LDS reads, as in the forward kernel)
+      if (t + 1 >= t1) return;
       if (MASKED) {
         km.next();
         km.load((t + 2) * KT);
         pm.load((t + 1) * KT);
       }
       st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    };
+    if (dead) {
+      stage_next();
+      return;
     }
-    if (dead) continue;
     const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
     const char* vt = kt + TILE_B;
     const bool ragged = key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off);
     const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
-      f32x16 s = zero16(), dp = zero16();
+      f32x16 s = zero16(), dp = START ? start : zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(vt, kb * 32, ks, lane), gf[ks]);
+      if (kb == 0) stage_next();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (START ? dp[i] : dp[i] + minus);
       if (ragged) {
+        keep_branch();
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = kb * 32 + 8 * (i >> 2) + (i & 3) <= lim ? dp[i] : 0.f;
       }
@@ -140,7 +149,13 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
         for (int db = 0; db < DB; ++db) mma32(dq[db], Rd::cols(kt, kb * 32 + j * 16, db * 32, lane), sf);
       }
     }
+  };
+  int t = t0;
+  for (; t + 1 < t1; t += 2) {
+    step(t, 0);
+    step(t + 1, 1);
   }
+  if (t < t1) step(t, 0);
 
   if constexpr (FEW) {
     constexpr int LD = DP + 4;
@@ -165,14 +180,14 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       }
       const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
       const long long at = (((long long)n * p.Lq + tk) * p.Hq + hd) * p.D;
-      if (p.splits == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
-      else store4<float>((char*)(p.part + (long long)split * p.N * p.Lq * p.Hq * p.D + at), d, v[0], v[1], v[2], v[3]);
+      if (w.parts == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
+      else store4<float>((char*)(p.part + (((long long)w.slot * p.parts + w.part) * p.R + row) * p.D), d, v[0], v[1], v[2], v[3]);
     }
     return;
   }
   if (!row_in) return;
   const long long at = (((long long)n * p.Lq + tok) * p.Hq + head) * p.D;
-  if (p.splits == 1) {
+  if (w.parts == 1) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -182,7 +197,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
           store4<T>(p.dq + at * (int)sizeof(T), d, dq[db][i] * p.scale, dq[db][i + 1] * p.scale, dq[db][i + 2] * p.scale, dq[db][i + 3] * p.scale);
       }
   } else {
-    char* dst = (char*)(p.part + (long long)split * p.N * p.Lq * p.Hq * p.D + at);
+    char* dst = (char*)(p.part + (((long long)w.slot * p.parts + w.part) * 128 + wave * 32 + l31) * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -193,52 +208,66 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
   }
 }
 
-int attn_dq_splits(const AttnDev& p, int dtype) {
-  const bool few = attn_few(p, dtype);
-  const long long blocks = (long long)(few ? 1 : ceil_div(p.R, 128)) * p.N * p.Hk;
-  const int steps = ceil_div(p.Lk, few ? 128 : 64);
-  if (blocks >= 256 || steps < 2) return 1;
-  long long per = (steps * blocks + 511) / 512;
-  if (!few && per < 2) per = 2;
-  return (int)((steps + per - 1) / per);
+// Sums the parts of the tiles that were cut, in part order: 4 channels of one row a thread.
+template <typename T>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev p, int tile_rows) {
+  const long long x = (long long)blockIdx.x * ATTN_THREADS + threadIdx.x;
+  const int quads = p.D / 4;
+  const long long line = x / quads;
+  const int d = (int)(x - line * quads) * 4;
+  if (line >= (long long)p.rest * tile_rows) return;
+  const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
+  AttnWork w;
+  attn_decode_tile(p, p.whole + slot, &w);
+  const int rr = w.tile * tile_rows + row;
+  if (rr >= p.R) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.parts; ++s) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * tile_rows + row) * p.D + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += y[e];
+  }
+  const int tok = div_g(p, rr), head = w.hk * p.G + rr - tok * p.G;
+  store4<T>(p.dq + (((long long)w.n * p.Lq + tok) * p.Hq + head) * p.D * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale,
+            v[2] * p.scale, v[3] * p.scale);
 }
 
 template <typename T, int DP, bool FEW>
-static int launch(const AttnDev& p, hipStream_t st) {
+static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
-  const long long blocks = (long long)p.tiles * p.splits * p.N * p.Hk;
-  SEGK_UNSUPPORTED(blocks < 0x7ffffff0LL, "attention_bwd: too many workgroups");
-  auto kern = p.mask || p.kmask ? attn_dq_kernel<T, DP, FEW, true> : attn_dq_kernel<T, DP, FEW, false>;
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) {
-      set_error("attention_bwd: %s", hipGetErrorString(e));
-      return SEGK_HIP_ERROR;
-    }
-  }
-  kern<<<(unsigned)((blocks + 7) / 8 * 8), ATTN_THREADS, lds, st>>>(p);
+  static std::atomic<int> seen[2][ATTN_DEVICES];
+  const bool masked = p->mask || p->kmask;
+  auto kern = masked ? attn_dq_kernel<T, DP, FEW, true> : attn_dq_kernel<T, DP, FEW, false>;
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
+  if (per_cu < 0) return per_cu;
+  p->tiles = FEW ? 1 : ceil_div(p->R, 128);
+  SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention_bwd: too many workgroups");
+  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, FEW ? 128 : 64), FEW ? 1 : 2);
+  if (plan_only) return SEGK_OK;
+  kern<<<(unsigned)grid, ATTN_THREADS, lds, st>>>(*p);
   SEGK_CHECK_LAUNCH("attention_bwd queries");
+  if (p->parts > 1) {
+    const int tile_rows = FEW ? p->R : 128;
+    const long long blocks = ((long long)p->rest * tile_rows * (p->D / 4) + ATTN_THREADS - 1) / ATTN_THREADS;
+    attn_dq_sum_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(*p, tile_rows);
+    SEGK_CHECK_LAUNCH("attention_bwd queries' sum");
+  }
   return SEGK_OK;
 }
 
 template <typename T>
-static int dispatch(const AttnDev& p, bool few, hipStream_t st) {
-  if (p.D <= 32) return few ? launch<T, 32, true>(p, st) : launch<T, 32, false>(p, st);
-  if (p.D <= 64) return few ? launch<T, 64, true>(p, st) : launch<T, 64, false>(p, st);
+static int dispatch(AttnDev* p, bool few, bool plan_only, hipStream_t st) {
+  if (p->D <= 32) return few ? launch<T, 32, true>(p, plan_only, st) : launch<T, 32, false>(p, plan_only, st);
+  if (p->D <= 64) return few ? launch<T, 64, true>(p, plan_only, st) : launch<T, 64, false>(p, plan_only, st);
   if constexpr (sizeof(T) == 2) {
-    if (few) return p.D <= 96 ? launch<T, 96, true>(p, st) : launch<T, 128, true>(p, st);
+    if (few) return p->D <= 96 ? launch<T, 96, true>(p, plan_only, st) : launch<T, 128, true>(p, plan_only, st);
   }
-  return p.D <= 96 ? launch<T, 96, false>(p, st) : launch<T, 128, false>(p, st);
+  return p->D <= 96 ? launch<T, 96, false>(p, plan_only, st) : launch<T, 128, false>(p, plan_only, st);
 }
 
-int launch_attn_dq(AttnDev p, int dtype, hipStream_t st) {
-  const bool few = attn_few(p, dtype);
-  p.tiles = few ? 1 : ceil_div(p.R, 128);
-  p.splits = attn_dq_splits(p, dtype);
-  const int rc = dtype == SEGK_BF16 ? dispatch<bf16_t>(p, few, st) : dispatch<float>(p, few, st);
-  if (rc != SEGK_OK || p.splits == 1) return rc;
-  const long long all = (long long)p.N * p.Lq * p.Hq * p.D;
-  return launch_attn_sum(p.part, all, p.splits, p.scale, p.dq, all, dtype, st);
+int attn_dq(AttnDev* p, int dtype, bool plan_only, hipStream_t st) {
+  const bool few = attn_few(*p, dtype);
+  return dtype == SEGK_BF16 ? dispatch<bf16_t>(p, few, plan_only, st) : dispatch<float>(p, few, plan_only, st);
 }
 
 }  // namespace segk

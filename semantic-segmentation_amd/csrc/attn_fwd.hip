@@ -6,6 +6,10 @@
 
 namespace segk {
 
+#ifndef FWD_W
+#define FWD_W 2
+#endif
+
 // One workgroup: 4 wavefronts and a loop over tiles of keys.  Scores are computed transposed (S^T = K Q^T, a lane owns one
 // query), so the row maximum is an in-lane reduction plus one exchange, the running statistics are one register, and S^T is
 // the operand of O^T = V^T P^T as it lies (attn.h).
@@ -14,7 +18,7 @@ namespace segk {
 //                of a tile of 128; their parts are joined in LDS at the end
 // MASKED: a pair mask and / or a key mask is read, one tile ahead of its use.
 template <typename T, int DP, bool FEW, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2)) void attn_fwd_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : FWD_W)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
   constexpr int KT = FEW ? 128 : 64, NKB = FEW ? 1 : 2;
@@ -24,13 +28,9 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int w = xcd_contiguous(p.tiles * p.splits * p.N * p.Hk);
-  if (w < 0) return;
-  const int split = w % p.splits;
-  w /= p.splits;
-  const int tile = w % p.tiles;
-  w /= p.tiles;
-  const int hk = w % p.Hk, n = w / p.Hk;
+  const AttnWork w = attn_work(p);
+  if (w.n < 0) return;
+  const int n = w.n, hk = w.hk, tile = w.tile;
   const int row0 = FEW ? 0 : tile * 128 + wave * 32;      // of this wavefront
   const bool idle = row0 >= p.R;                          // it then only helps to stage the tiles
 
@@ -39,8 +39,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
   const int all_steps = (k_end + KT - 1) / KT;
-  const int per = (all_steps + p.splits - 1) / p.splits;
-  const int t0 = min(split * per, all_steps), t1 = min(t0 + per, all_steps);
+  const int per = (all_steps + w.parts - 1) / w.parts;
+  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
 
   const int r = row0 + l31;
   const bool row_ok = r < p.R;
@@ -73,8 +73,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
     }
     st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
   }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  // (two steps to a turn of the loop: the buffer is a constant of each)
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
     tile_barrier();                       // tile t is here; every wavefront has left tile t - 1
     const int key0 = t * KT + (FEW ? wave * 32 : 0);
     unsigned kw[NKB], pw[NKB][4];
@@ -96,15 +96,20 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
         dead = !__any(row_ok && some != 0);
       }
     }
-    if (t + 1 < t1) {
+    // The next tile is asked for behind this tile's first LDS reads: a wavefront's LDS reads queue behind its own LDS-DMA.
+    auto stage_next = [&]() {
+      if (t + 1 >= t1) return;
       if (MASKED) {
         km.next();
         km.load((t + 2) * KT);
         pm.load((t + 1) * KT);
       }
       st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    };
+    if (dead) {                           // nothing of this tile is open to this wavefront's rows
+      stage_next();
+      return;
     }
-    if (dead) continue;                   // nothing of this tile is open to this wavefront's rows
     const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
     const char* vt = kt + TILE_B;
 
@@ -115,9 +120,11 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) mma32(s[kb], Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
+    stage_next();
 
     // closed pairs: past the last key, above the diagonal, masked
     if (key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off)) {
+      keep_branch();
       const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
@@ -139,42 +146,55 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
       }
     }
 
-    float mx = s[0][0];
+    // p = exp2(s scale log2(e) - m) for a reference m that need not be the maximum: in floating point any m serves that
+    // neither overflows nor loses the largest terms.  m starts as the maximum of the first tile that has an open key and
+    // is raised (accumulators rescaled) only when a tile's sum passes 2^30, so that the common tile needs no maximum.
+    // m = -inf makes the sum infinite or NaN, as do such scores: the raising path sorts those out, too.
+    AttnFrag<T> pf[2 * NKB];
+    float sum = 0.f;
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
+    for (int j = 0; j < 2 * NKB; ++j) {
+      float e[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = pair_max(mx) * p.scale_log2;
-    // The maximum in use may lag the true one by up to 8 (probabilities up to 2^8, harmless in fp32 and in the relative
-    // precision of bf16): the accumulators are then rescaled a few times per row instead of once per tile.
-    if (__any(mx > m + 8.f)) {
-      const float nm = fmaxf(m, mx);
-      const float alpha = exp2_fast(m - (nm == -INFINITY ? 0.f : nm));
+      for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[j >> 1][8 * (j & 1) + i], p.scale_log2, -m));
+      pf[j] = pack_sum<T>(e, sum);
+    }
+    if (__builtin_expect(!__all(sum < 1073741824.f), 0)) {
+      float mx = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+      const float nm = fmaxf(m, pair_max(mx) * p.scale_log2);
+      const float ms = nm == -INFINITY ? 0.f : nm;
+      const float alpha = exp2_fast(m - ms);
       m = nm;
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
+      sum = 0.f;
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
+      for (int j = 0; j < 2 * NKB; ++j) {
+        float e[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = exp2_fast(fmaf(s[kb][i], p.scale_log2, -ms));
-        s[kb][i] = e;
-        sum += e;
+        for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[j >> 1][8 * (j & 1) + i], p.scale_log2, -ms));
+        pf[j] = pack_sum<T>(e, sum);
       }
+    }
     l += sum;
 #pragma unroll
-    for (int j = 0; j < 2 * NKB; ++j) {
-      const AttnFrag<T> pf = pack_frag<T>(s[j >> 1], j & 1);
+    for (int j = 0; j < 2 * NKB; ++j)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) mma32(o[db], Rd::cols(vt, j * 16, db * 32, lane), pf);
-    }
+      for (int db = 0; db < DB; ++db) mma32(o[db], Rd::cols(vt, j * 16, db * 32, lane), pf[j]);
+  };
+  int t = t0;
+  for (; t + 1 < t1; t += 2) {
+    step(t, 0);
+    step(t + 1, 1);
   }
+  if (t < t1) step(t, 0);
 
   float lt = pair_sum(l);
   if constexpr (FEW) {
@@ -210,7 +230,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
         sum += sm[128 + i * 32 + row];
         top = fmaxf(top, sm[i * 32 + row]);
       }
-      if (p.splits == 1) {
+      if (w.parts == 1) {
         const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         store4<T>(p.out + ((long long)n * p.o.n + (long long)tk * p.o.l + (long long)hd * p.o.h) * (int)sizeof(T), d, v[0] * inv, v[1] * inv,
@@ -218,7 +238,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
         if (p.lse && d == 0)
           p.lse[((long long)n * p.Hq + hd) * p.Lq + tk] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
       } else {
-        const long long at = ((long long)split * p.N * p.Hk + (long long)n * p.Hk + hk) * p.R + row;
+        const long long at = ((long long)w.slot * p.parts + w.part) * p.R + row;
         store4<float>((char*)(p.part + at * p.D), d, v[0], v[1], v[2], v[3]);
         if (d == 0) {
           p.part_ml[2 * at] = top;
@@ -229,7 +249,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
     return;
   }
   if (!row_ok) return;
-  if (p.splits == 1) {
+  if (w.parts == 1) {
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     char* dst = p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T);
 #pragma unroll
@@ -242,7 +262,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
     if (p.lse && h == 0)
       p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.6931471805599453f;
   } else {
-    const long long at = ((long long)split * p.N * p.Hk + (long long)n * p.Hk + hk) * p.R + r;
+    const long long at = ((long long)w.slot * p.parts + w.part) * 128 + wave * 32 + l31;
     char* dst = (char*)(p.part + at * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -258,57 +278,60 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   }
 }
 
-// Joins the parts of a split key axis: one workgroup per row; D / 4 (rounded up to a power of two) threads walk the
-// channels of every GROUPS-th part, the groups are joined in LDS in order.
+// Joins the parts of the tiles that were cut.  `lanes` = D / 4 rounded up to a power of two threads walk a row's channels of
+// every `groups`-th part; the groups of a row are joined in LDS in order.  tile_rows: rows of a tile in the partial results.
 template <typename T>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes) {
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes, int groups, int tile_rows) {
   __shared__ f32x4 so[ATTN_THREADS];
-  __shared__ float sl[ATTN_THREADS], sm[4];
-  const long long rows = (long long)p.N * p.Hk * p.R;
-  const long long r = blockIdx.x;
-  const int c = threadIdx.x % lanes, g = threadIdx.x / lanes, groups = ATTN_THREADS / lanes;
-  float m = -INFINITY;
-  for (int s = threadIdx.x; s < p.splits; s += ATTN_THREADS) m = fmaxf(m, p.part_ml[2 * (s * rows + r)]);
-#pragma unroll
-  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __shared__ float sl[ATTN_THREADS], sm[ATTN_THREADS];
+  const int c = threadIdx.x % lanes, g = threadIdx.x / lanes % groups, in = threadIdx.x / (lanes * groups);
+  const long long line = (long long)blockIdx.x * (ATTN_THREADS / (lanes * groups)) + in;
+  const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
+  const bool ok = slot < p.rest;
+  const long long first = ok ? (long long)slot * p.parts * tile_rows + row : 0;
+  // every group looks at its own parts' maxima first, so that the sums are scaled once
+  float m = -INFINITY, l = 0.f;
+  if (ok)
+    for (int s = g; s < p.parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * tile_rows)]);
+  sm[threadIdx.x] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  for (int i = 0; i < groups; ++i) m = fmaxf(m, sm[(in * groups + i) * lanes + c]);
   const float ms = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = g; s < p.splits; s += groups) {
-    const long long at = s * rows + r;
-    const float a = exp2_fast(p.part_ml[2 * at] - ms);
-    l = fmaf(p.part_ml[2 * at + 1], a, l);
-    if (c * 4 < p.D) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * p.D + c * 4);
+  if (ok)
+    for (int s = g; s < p.parts; s += groups) {
+      const long long at = first + (long long)s * tile_rows;
+      const float a = exp2_fast(p.part_ml[2 * at] - ms);
+      l = fmaf(p.part_ml[2 * at + 1], a, l);
+      if (c * 4 < p.D) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * p.D + c * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], a, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], a, o[e]);
+      }
     }
-  }
   so[threadIdx.x] = o;
   sl[threadIdx.x] = l;
   __syncthreads();
-  if (g != 0 || c * 4 >= p.D) return;
+  if (!ok || g != 0 || c * 4 >= p.D) return;
+  AttnWork w;
+  attn_decode_tile(p, p.whole + slot, &w);
+  const int rr = w.tile * tile_rows + row;
+  if (rr >= p.R) return;
   for (int i = 1; i < groups; ++i) {
-    const f32x4 x = so[i * lanes + c];
+    const f32x4 x = so[threadIdx.x + i * lanes];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e];
-    l += sl[i * lanes + c];
+    l += sl[threadIdx.x + i * lanes];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int rr = (int)(r % p.R);
-  const long long nh = r / p.R;
-  const int hk = (int)(nh % p.Hk), n = (int)(nh / p.Hk);
-  const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
+  const int n = w.n, tok = div_g(p, rr), head = w.hk * p.G + rr - tok * p.G;
   store4<T>(p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T), c * 4, o[0] * inv, o[1] * inv,
             o[2] * inv, o[3] * inv);
   if (p.lse && c == 0)
     p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// Row statistics of the backward pass in packed row order: rowsum(dout * out) and the base-2 lse (+inf where a row has no
+// Row statistics of the backward pass in packed row order: -rowsum(dout * out) and the base-2 lse (+inf where a row has no
 // open key and in the padding: its probabilities then come out as zeros).  D / 8 lanes (rounded up to a power of two)
 // share a row.
 template <typename T>
@@ -345,7 +368,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_row_stats_kernel(const Attn
   for (int s = lanes >> 1; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
   if (c == 0) {
     p.row_lse2[r] = lse;
-    p.row_delta[r] = sum;
+    p.minus_delta[r] = -sum;
   }
 }
 
@@ -363,15 +386,51 @@ bool attn_few(const AttnDev& p, int dtype) {
   return p.R <= 32 && attn_pitch(p.D, dtype) <= 256 && far < 0xf0000000LL;
 }
 
-static int fwd_splits(const AttnDev& p, int dtype) {
-  const bool few = attn_few(p, dtype);
-  const long long blocks = (long long)(few ? 1 : ceil_div(p.R, 128)) * p.N * p.Hk;
-  const int steps = ceil_div(p.Lk, few ? 128 : 64);
-  // Too few workgroups for 256 CUs: cut the key axis into parts of `per` steps.
-  if (blocks >= 256 || steps < 2) return 1;
-  long long per = (steps * blocks + 511) / 512;
-  if (!few && per < 2) per = 2;
-  return (int)((steps + per - 1) / per);
+long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps) {
+  const long long all = (long long)p->tiles * p->N * p->Hk;
+  const long long round = 256LL * per_cu;      // workgroups that run at once
+  // Under the diagonal tiles differ in length and even out by themselves once there are enough of them.
+  long long whole = p->causal && all >= round ? all / 8 * 8 : all / round * round;
+  // A last round that is not full is worth cutting up (and joining) only where a round is long: 18 steps of 64 keys gained
+  // nothing, 67 steps 5 %, 261 steps 12 %.
+  if (whole > 0 && steps < 64) whole = (all + 7) / 8 * 8;
+  long long rest = all > whole ? all - whole : 0, parts = 1;
+  if (rest > 0) {
+    parts = round / rest;
+    if (parts > steps / min_steps) parts = steps / min_steps;
+    if (parts < 1) parts = 1;
+    const long long per = (steps + parts - 1) / parts;   // as many as have work
+    parts = per > 0 ? (steps + per - 1) / per : 1;
+    if (parts < 1) parts = 1;
+  }
+  p->whole = (int)whole, p->rest = (int)rest, p->parts = (int)parts;
+  p->rest_x = (int)((rest * parts + 7) / 8);
+  return whole + 8LL * p->rest_x;
+}
+
+int attn_occupancy(const void* kernel, int lds, std::atomic<int>* seen) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= ATTN_DEVICES) {
+    set_error("attention: no current device among the first %d", ATTN_DEVICES);
+    return SEGK_HIP_ERROR;
+  }
+  const int known = seen[dev].load(std::memory_order_relaxed);
+  if (known) return known;
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) {
+      set_error("attention: %s", hipGetErrorString(e));
+      return SEGK_HIP_ERROR;
+    }
+  }
+  int n = 0;
+  const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, ATTN_THREADS, (size_t)lds);
+  if (e != hipSuccess || n < 1) {
+    set_error("attention: no workgroup fits a CU: %s", hipGetErrorString(e));
+    return SEGK_HIP_ERROR;
+  }
+  seen[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 #define CHK_VIEW(v, name, L, H)                                                                                                   \
@@ -418,10 +477,10 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   p->off = a->Lk - a->Lq;
   p->scale = a->scale;
   p->scale_log2 = a->scale * LOG2E;
-  p->tiles = p->splits = 1;
+  p->tiles = p->whole = p->rest = p->parts = p->rest_x = 0;
   p->part = p->part_ml = nullptr;
   p->dq = p->dk = p->dv = nullptr;
-  p->row_lse2 = p->row_delta = nullptr;
+  p->row_lse2 = p->minus_delta = nullptr;
   if (backward) {
     CHK_VIEW(dout, "dout", a->Lq, G);
     p->dout = {(const char*)a->dout.p, a->dout.n, a->dout.l, a->dout.h};
@@ -434,43 +493,62 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
 }
 
 template <typename T, int DP, bool FEW>
-static int launch_fwd(const AttnDev& p, hipStream_t st) {
+static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
   const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
-  const long long blocks = (long long)p.tiles * p.splits * p.N * p.Hk;
-  SEGK_UNSUPPORTED(blocks < 0x7ffffff0LL, "attention: too many workgroups");
-  const unsigned grid = (unsigned)((blocks + 7) / 8 * 8);
-  const bool masked = p.mask || p.kmask;
+  static std::atomic<int> seen[2][ATTN_DEVICES];
+  const bool masked = p->mask || p->kmask;
   auto kern = masked ? attn_fwd_kernel<T, DP, FEW, true> : attn_fwd_kernel<T, DP, FEW, false>;
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) {
-      set_error("attention: %s", hipGetErrorString(e));
-      return SEGK_HIP_ERROR;
-    }
-  }
-  kern<<<grid, ATTN_THREADS, lds, st>>>(p);
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
+  if (per_cu < 0) return per_cu;
+  p->tiles = FEW ? 1 : ceil_div(p->R, 128);
+  SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention: too many workgroups");
+  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, FEW ? 128 : 64), FEW ? 1 : 2);
+  if (plan_only) return SEGK_OK;
+  kern<<<(unsigned)grid, ATTN_THREADS, lds, st>>>(*p);
   SEGK_CHECK_LAUNCH("attention_fwd");
   return SEGK_OK;
 }
 
 template <typename T>
-static int dispatch_fwd(const AttnDev& p, bool few, hipStream_t st) {
-  switch (attn_dp(p.D)) {
-    case 32: return few ? launch_fwd<T, 32, true>(p, st) : launch_fwd<T, 32, false>(p, st);
-    case 64: return few ? launch_fwd<T, 64, true>(p, st) : launch_fwd<T, 64, false>(p, st);
+static int dispatch_fwd(AttnDev* p, bool few, bool plan_only, hipStream_t st) {
+  switch (attn_dp(p->D)) {
+    case 32: return few ? launch_fwd<T, 32, true>(p, plan_only, st) : launch_fwd<T, 32, false>(p, plan_only, st);
+    case 64: return few ? launch_fwd<T, 64, true>(p, plan_only, st) : launch_fwd<T, 64, false>(p, plan_only, st);
     case 96:
       if constexpr (sizeof(T) == 2)
-        if (few) return launch_fwd<T, 96, true>(p, st);
-      return launch_fwd<T, 96, false>(p, st);
+        if (few) return launch_fwd<T, 96, true>(p, plan_only, st);
+      return launch_fwd<T, 96, false>(p, plan_only, st);
     default:
       if constexpr (sizeof(T) == 2)
-        if (few) return launch_fwd<T, 128, true>(p, st);
-      return launch_fwd<T, 128, false>(p, st);
+        if (few) return launch_fwd<T, 128, true>(p, plan_only, st);
+      return launch_fwd<T, 128, false>(p, plan_only, st);
   }
 }
 
-static long long fwd_part_floats(const AttnDev& p, int splits) {
-  return splits > 1 ? (long long)splits * p.N * p.Hk * p.R * (p.D + 2) : 0;
+// The deal of a forward pass, and the floats of its partial results.  Launches unless plan_only.
+static int run_fwd(AttnDev* p, int dtype, bool plan_only, hipStream_t st) {
+  const bool few = attn_few(*p, dtype);
+  return dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, few, plan_only, st) : dispatch_fwd<float>(p, few, plan_only, st);
+}
+static int fwd_tile_rows(const AttnDev& p, int dtype) { return attn_few(p, dtype) ? p.R : 128; }
+
+// Floats of the backward pass's workspace: row statistics, then the partial results of whichever pass is running.
+static int bwd_floats(AttnDev p, int dtype, long long* floats) {
+  const long long stats = 2LL * p.N * p.Hk * p.Rp;
+  long long part = 0;
+  if (p.dk && p.Lk > 0) {
+    const int rc = attn_dkv(&p, dtype, true, nullptr);
+    if (rc != SEGK_OK) return rc;
+    part = attn_part_floats(p, 128, 2 * p.D);
+  }
+  if (p.dq && p.Lk > 0) {
+    const int rc = attn_dq(&p, dtype, true, nullptr);
+    if (rc != SEGK_OK) return rc;
+    const long long x = attn_part_floats(p, fwd_tile_rows(p, dtype), p.D);
+    if (x > part) part = x;
+  }
+  *floats = stats + part;
+  return SEGK_OK;
 }
 
 }  // namespace segk
@@ -479,75 +557,77 @@ using namespace segk;
 
 extern "C" long long segk_attention_workspace(const segk_attention_args* a, int backward) {
   AttnDev p;
-  const int rc = attn_check(a, &p, backward != 0);
+  int rc = attn_check(a, &p, backward != 0);
   if (rc != SEGK_OK) return rc;
-  if (!backward) return fwd_part_floats(p, fwd_splits(p, a->dtype)) * 4;
-  const long long stats = 2LL * p.N * p.Hk * p.Rp;
-  long long part = 0;
-  if (p.dk && p.Lk > 0) {
-    const int s = attn_dkv_splits(p, a->dtype);
-    if (s > 1) part = 2LL * s * p.N * p.Hk * p.Lk * p.D;
+  long long floats = 0;
+  if (backward) {
+    rc = bwd_floats(p, a->dtype, &floats);
+  } else {
+    rc = run_fwd(&p, a->dtype, true, nullptr);
+    floats = attn_part_floats(p, fwd_tile_rows(p, a->dtype), p.D + 2);
   }
-  if (p.dq && p.Lk > 0) {
-    const int s = attn_dq_splits(p, a->dtype);
-    const long long x = s > 1 ? (long long)s * p.N * p.Hk * p.R * p.D : 0;
-    if (x > part) part = x;
+  return rc != SEGK_OK ? rc : floats * 4;
+}
+
+static int take_workspace(const segk_attention_args* a, long long need, const char* name) {
+  SEGK_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0, "%s: workspace missing or not 16-byte aligned", name);
+  if (a->workspace_bytes < need) {
+    set_error("%s: workspace of %lld bytes, needs %lld", name, a->workspace_bytes, need);
+    return SEGK_WORKSPACE_TOO_SMALL;
   }
-  return (stats + part) * 4;
+  return SEGK_OK;
 }
 
 extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t stream) {
   AttnDev p;
-  const int rc = attn_check(a, &p, false);
+  int rc = attn_check(a, &p, false);
   if (rc != SEGK_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const bool few = attn_few(p, a->dtype);
-  p.tiles = few ? 1 : ceil_div(p.R, 128);
-  p.splits = fwd_splits(p, a->dtype);
-  const long long need = fwd_part_floats(p, p.splits) * 4;
-  if (need > 0) {
-    SEGK_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0, "attention_fwd: workspace missing or not 16-byte aligned");
-    if (a->workspace_bytes < need) {
-      set_error("attention_fwd: workspace of %lld bytes, needs %lld", a->workspace_bytes, need);
-      return SEGK_WORKSPACE_TOO_SMALL;
-    }
+  rc = run_fwd(&p, a->dtype, true, st);
+  if (rc != SEGK_OK) return rc;
+  const int tile_rows = fwd_tile_rows(p, a->dtype);
+  const long long floats = attn_part_floats(p, tile_rows, p.D + 2);
+  if (floats > 0) {
+    rc = take_workspace(a, floats * 4, "attention_fwd");
+    if (rc != SEGK_OK) return rc;
     p.part = (float*)a->workspace;
-    p.part_ml = p.part + (long long)p.splits * p.N * p.Hk * p.R * p.D;
+    p.part_ml = p.part + attn_part_floats(p, tile_rows, p.D);
   }
-  const int rc2 = a->dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, few, st) : dispatch_fwd<float>(p, few, st);
-  if (rc2 != SEGK_OK || p.splits == 1) return rc2;
+  rc = run_fwd(&p, a->dtype, false, st);
+  if (rc != SEGK_OK || p.parts == 1) return rc;
   const int lanes = p.D <= 8 ? 2 : p.D <= 16 ? 4 : p.D <= 32 ? 8 : p.D <= 64 ? 16 : 32;
-  const unsigned grid = (unsigned)((long long)p.N * p.Hk * p.R);   // (splits only where workgroups are few: small)
-  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes)));
+  int groups = 1;
+  while (groups < p.parts && groups * lanes < ATTN_THREADS) groups *= 2;
+  const int lines = ATTN_THREADS / (lanes * groups);
+  const unsigned grid = (unsigned)ceil_div((long long)p.rest * tile_rows, lines);   // (rest is less than a round of workgroups)
+  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes, groups, tile_rows)));
   SEGK_CHECK_LAUNCH("attention_fwd join");
   return SEGK_OK;
 }
 
 extern "C" int segk_attention_bwd(const segk_attention_args* a, segk_stream_t stream) {
   AttnDev p;
-  const int rc = attn_check(a, &p, true);
+  int rc = attn_check(a, &p, true);
   if (rc != SEGK_OK) return rc;
   SEGK_REQUIRE(p.Lk > 0, "attention_bwd: no keys");
-  const long long need = segk_attention_workspace(a, 1);
-  SEGK_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0, "attention_bwd: workspace missing or not 16-byte aligned");
-  if (a->workspace_bytes < need) {
-    set_error("attention_bwd: workspace of %lld bytes, needs %lld", a->workspace_bytes, need);
-    return SEGK_WORKSPACE_TOO_SMALL;
-  }
+  long long floats = 0;
+  rc = bwd_floats(p, a->dtype, &floats);
+  if (rc != SEGK_OK) return rc;
+  rc = take_workspace(a, floats * 4, "attention_bwd");
+  if (rc != SEGK_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
   const long long rows = (long long)p.N * p.Hk * p.Rp;
   p.row_lse2 = (float*)a->workspace;
-  p.row_delta = p.row_lse2 + rows;
-  p.part = p.row_delta + rows;
+  p.minus_delta = p.row_lse2 + rows;
+  p.part = p.minus_delta + rows;
   const int lanes = p.D <= 8 ? 1 : p.D <= 16 ? 2 : p.D <= 32 ? 4 : p.D <= 64 ? 8 : 16;
   const long long blocks = (rows * lanes + ATTN_THREADS - 1) / ATTN_THREADS;
   SEGK_UNSUPPORTED(blocks < 0x7fffffffLL, "attention_bwd: too many rows");
   SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_row_stats_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(p, lanes)));
   SEGK_CHECK_LAUNCH("attention_bwd statistics");
   if (p.dk) {
-    const int r = launch_attn_dkv(p, a->dtype, st);
-    if (r != SEGK_OK) return r;
+    rc = attn_dkv(&p, a->dtype, false, st);
+    if (rc != SEGK_OK) return rc;
   }
-  if (p.dq) return launch_attn_dq(p, a->dtype, st);
-  return SEGK_OK;
+  return p.dq ? attn_dq(&p, a->dtype, false, st) : SEGK_OK;
 }
