@@ -265,6 +265,57 @@ struct AttnRead<float, DP> {
   }
 };
 
+// The same reads from LDS byte addresses.  A lane's places differ between k-steps and columns by XORs that are kept in
+// registers; what is added (tile, row block) is a constant of the instruction where the caller's is one.
+template <typename T, int DP>
+struct AttnLane;
+template <int DP>
+struct AttnLane<bf16_t, DP> {
+  typedef AttnTile<bf16_t, DP> Tile;
+  unsigned ra[DP / 16], ca[DP / 32][2];
+  __device__ __forceinline__ AttnLane(const char* smem, int lane) {
+    const unsigned base = (unsigned)(unsigned long long)(attn_lds_ptr)smem;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) ra[ks] = base + Tile::at(lane & 31, 2 * ks + (lane >> 5));
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 8 * j + 4 * (lane >> 5) + ((lane & 15) >> 2);
+        ca[db][j] = base + Tile::at(row, db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) + (lane & 1) * 8;
+      }
+  }
+  // rows / columns of the block of 32 (16) rows that starts at LDS byte `at`
+  __device__ __forceinline__ AttnFrag<bf16_t> rows(int at, int ks) const {
+    AttnFrag<bf16_t> f;
+    f.v = *(const __attribute__((address_space(3))) u32x4*)(size_t)(ra[ks] + at);
+    return f;
+  }
+  __device__ __forceinline__ AttnFrag<bf16_t> cols(int at, int db) const {
+    AttnFrag<bf16_t> f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const attn_s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn_s16x4*)(size_t)(ca[db][j] + at));
+      const u32x2 u = __builtin_bit_cast(u32x2, t);
+      f.v[2 * j] = u[0];
+      f.v[2 * j + 1] = u[1];
+    }
+    return f;
+  }
+};
+template <int DP>
+struct AttnLane<float, DP> {
+  const char* smem;
+  int lane;
+  __device__ __forceinline__ AttnLane(const char* s, int l) : smem(s), lane(l) {}
+  __device__ __forceinline__ AttnFrag<float> rows(int at, int ks) const { return AttnRead<float, DP>::rows(smem + at, 0, ks, lane); }
+  __device__ __forceinline__ AttnFrag<float> cols(int at, int db) const { return AttnRead<float, DP>::cols(smem + at, 0, db * 32, lane); }
+};
+
+// Keeps an operand packed from here on (the compiler would carry the unpacked values to its use).
+__device__ __forceinline__ void pin(AttnFrag<bf16_t>& f) { asm("" : "+v"(f.v)); }
+__device__ __forceinline__ void pin(AttnFrag<float>&) {}
+
 // Operand fragment straight from global memory: 8 elements from channel 16 ks + 8 h of one row (zeros past D and for
 // ok == false).  D is a multiple of 8, so a fragment is whole or absent.
 template <typename T>
@@ -369,6 +420,25 @@ struct AttnStage {
     vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
     lds0 = lds_addr(smem) + wave * 1024;
   }
+  // One operand's tile at byte `at` of LDS.
+  template <int KT, bool MASKED>
+  __device__ __forceinline__ void one(const AttnDev& p, const char* base, unsigned step, int key0, int at, unsigned long long bits) const {
+    static_assert(KT == 64, "one word of key bits");
+    const u32x4 rsrc = buffer_of(base + (long long)key0 * step);
+    const bool inside = !MASKED && key0 + KT <= p.Lk;
+#pragma unroll
+    for (int i = 0; i < KT * Tile::PITCH / 4096; ++i) {
+      const int x = pc.row + i * Piece::STEP, c = pc.chunk(i) * 16;
+      const unsigned off = c < row_b ? x * step + c : ATTN_OOB;
+      if (inside) {
+        dma_1k(rsrc, lds0 + at + i * 4096, off);
+      } else {
+        bool in = key0 + x < p.Lk;
+        if (MASKED) in = in && ((bits >> x) & 1);
+        dma_1k(rsrc, lds0 + at + i * 4096, in ? off : ATTN_OOB);
+      }
+    }
+  }
   // bits: the tile's open keys (MASKED).  A closed key is not read: whatever its memory holds, zeros arrive.
   template <int KT, bool MASKED>
   __device__ __forceinline__ void keys(const AttnDev& p, int key0, int buf, const unsigned long long* bits) const {
@@ -393,6 +463,9 @@ struct AttnStage {
     }
   }
 };
+
+// Keeps a rarely taken uniform branch a branch (the compiler would compute both sides and select).
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 // Key mask of a tile of KT keys as one bit per key, the same in every wavefront: load() asks for a tile's bytes, next()
 // turns the bytes asked for last into bits.  Without a mask all bits are set.
@@ -426,39 +499,64 @@ struct AttnKeyMask {
   __device__ __forceinline__ unsigned word(int key) const { return (unsigned)(bits[KT == 64 ? 0 : key >> 6] >> (key & 63)); }
 };
 
-// Pair mask of one row against 32 * NKB keys: byte e of w[kb][g] belongs to key first + kb * 32 + 8 g + e of the tile, the
-// order of a result tile's registers.
-template <int NKB>
+// The last of the first `keys` keys that the mask leaves open, -1 if none: a wavefront's answer.
+__device__ __forceinline__ int last_open_key(const unsigned char* mask, long long step, int keys, int lane) {
+  for (int j0 = (keys - 1) / 64 * 64; j0 >= 0 && keys > 0; j0 -= 64) {
+    const int j = j0 + lane;
+    const unsigned long long open = __ballot(j < keys && mask[j * step] != 0);
+    if (open) return j0 + 63 - __builtin_clzll(open);
+  }
+  return -1;
+}
+
+// Pair mask of one row against a block of 32 keys: byte e of w[g] belongs to key 8 g + 4 h + e of the block, the order of a
+// result tile's registers.
 struct AttnPairMask {
   const unsigned char* row;
   long long step;
-  int Lk, first;
-  unsigned w[NKB][4];
-  __device__ __forceinline__ AttnPairMask(const unsigned char* m, long long s, int lk, int f) : row(m), step(s), Lk(lk), first(f) {}
+  int Lk, h4;
+  unsigned w[4];
+  __device__ __forceinline__ AttnPairMask(const unsigned char* m, long long s, int lk, int h) : row(m), step(s), Lk(lk), h4(4 * h) {}
   __device__ __forceinline__ void load(int key0) {
     if (!row) return;
-    const int j0 = key0 + first;
-    if (step == 1 && key0 + (NKB == 1 ? 128 : 64) <= Lk) {
+    if (step == 1 && key0 + 32 <= Lk) {
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[kb][g], row + j0 + kb * 32 + 8 * g, 4);
+      for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[g], row + key0 + h4 + 8 * g, 4);
       return;
     }
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
+    for (int g = 0; g < 4; ++g) {
+      unsigned x = 0;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        unsigned x = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + kb * 32 + 8 * g + e;
-          if (j < Lk && row[j * step]) x |= 0xffu << (8 * e);
-        }
-        w[kb][g] = x;
+      for (int e = 0; e < 4; ++e) {
+        const int j = key0 + h4 + 8 * g + e;
+        if (j < Lk && row[j * step]) x |= 0xffu << (8 * e);
       }
+      w[g] = x;
+    }
   }
 };
+
+// Puts `closed` wherever a block's pair is closed: past `lim` (the last open key's place counted from the lane's first),
+// by the key mask's word, by the pair mask.
+template <bool MASKED>
+__device__ __forceinline__ void close_pairs(f32x16& s, float closed, bool ragged, int lim, const unsigned* word, int h,
+                                            const unsigned* pair) {
+  if (ragged) {
+    keep_branch();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) <= lim ? s[i] : closed;
+  }
+  if (MASKED && word) {
+    const unsigned x = *word >> (4 * h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[i] : closed;
+  }
+  if (MASKED && pair) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = pair[i >> 2] & (0xffu << (8 * (i & 3))) ? s[i] : closed;
+  }
+}
 
 // maximum and sum over the two lanes that share a result column (l and l ^ 32)
 __device__ __forceinline__ float pair_max(float v) {
@@ -470,10 +568,21 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
-// Keeps a rarely taken uniform branch a branch (the compiler would compute both sides and select).
-__device__ __forceinline__ void keep_branch() { asm volatile(""); }
-
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Spreads MFMA instructions among the vector instructions and LDS reads of a basic block: `mfma` of them, `reads` LDS reads.
+template <typename T, int MFMA, int READS>
+__device__ __forceinline__ void interleave() {
+  if constexpr (sizeof(T) == 2) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < MFMA; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (READS + MFMA - 1) / MFMA, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, (60 + MFMA - 1) / MFMA, 0);
+    }
+  }
+}
 
 // ---- host side ----------------------------------------------------------------------------------
 int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);                 // attn_fwd.hip

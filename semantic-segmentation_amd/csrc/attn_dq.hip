@@ -27,6 +27,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
   const int last_row = min(FEW ? 32 : tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
+  if (MASKED && !FEW && p.kmask) k_end = min(k_end, last_open_key(p.kmask + n * p.km_n, p.km_k, k_end, lane) + 1);
   const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + w.parts - 1) / w.parts;
   const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
@@ -53,8 +54,16 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
 
   const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
   AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
-  AttnPairMask<NKB> pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k,
-                       p.Lk, (FEW ? wave * 32 : 0) + 4 * h);
+  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
+  unsigned pw_next[NKB][4];
+  auto load_pairs = [&](int t) {
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      pm.load(t * KT + (FEW ? wave * 32 : 0) + kb * 32);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) pw_next[kb][g] = pm.w[g];
+    }
+  };
 
   f32x16 dq[DB];
 #pragma unroll
@@ -65,7 +74,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       km.load(t0 * KT);
       km.next();
       km.load((t0 + 1) * KT);
-      pm.load(t0 * KT);
+      load_pairs(t0);
     }
     st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
   }
@@ -87,7 +96,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       for (int kb = 0; kb < NKB; ++kb) {
         kw[kb] = km.word((FEW ? wave * 32 : 0) + kb * 32);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) pw[kb][g] = pm.w[kb][g];
+        for (int g = 0; g < 4; ++g) pw[kb][g] = pw_next[kb][g];
       }
       dead = dead || !(NKB == 2 ? kw[0] | kw[NKB - 1] : kw[0]);
       if (pm.row && !dead) {
@@ -104,7 +113,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       if (MASKED) {
         km.next();
         km.load((t + 2) * KT);
-        pm.load((t + 1) * KT);
+        load_pairs(t + 1);
       }
       st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
     };
@@ -126,22 +135,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       if (kb == 0) stage_next();
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (START ? dp[i] : dp[i] + minus);
-      if (ragged) {
-        keep_branch();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dp[i] = kb * 32 + 8 * (i >> 2) + (i & 3) <= lim ? dp[i] : 0.f;
-      }
-      if (MASKED) {
-        if (km.mask) {
-          const unsigned x = kw[kb] >> (4 * h);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dp[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? dp[i] : 0.f;
-        }
-        if (pm.row) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dp[i] = pw[kb][i >> 2] & (0xffu << (8 * (i & 3))) ? dp[i] : 0.f;
-        }
-      }
+      close_pairs<MASKED>(dp, 0.f, ragged, lim - kb * 32, km.mask ? &kw[kb] : nullptr, h, pm.row ? pw[kb] : nullptr);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const AttnFrag<T> sf = pack_frag<T>(dp, j);

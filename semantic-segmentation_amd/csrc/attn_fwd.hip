@@ -2,42 +2,81 @@
 // and sum per row (fp32, base-2 exponents), and the host side of the attention entry points.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn.h"
 
 namespace segk {
 
-#ifndef FWD_W
-#define FWD_W 2
-#endif
+// Both kernels: scores are computed transposed (S^T = K Q^T, a lane owns one query), so the running statistics are one
+// register and S^T is the operand of O^T = V^T P^T as it lies (attn.h).  Keys in blocks of 32.
+//   p = exp2(s scale log2(e) - m) for a reference m that need not be the maximum: in floating point any m serves that
+//   neither overflows nor loses the largest terms.  m starts as the maximum of the first block that has an open key and is
+//   raised (accumulators rescaled) only when a block's sum passes 2^30, so that the common block needs no maximum.
+//   m = -inf makes the sum infinite or NaN, as do such scores: the raising path sorts those out, too.
+template <typename T, int DB>
+struct AttnRow {
+  f32x16 o[DB];
+  float m, l;
+  __device__ __forceinline__ AttnRow() : m(-INFINITY), l(0.f) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = zero16();
+  }
+  // probabilities of a block as two operands; their sum
+  __device__ __forceinline__ float weigh(const f32x16& s, float scale_log2, float ref, AttnFrag<T>* pf) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[8 * j + i], scale_log2, -ref));
+      pf[j] = pack_sum<T>(e, sum);
+    }
+    return sum;
+  }
+  __device__ __forceinline__ bool fine(float sum) const { return __builtin_amdgcn_ballot_w64(!(sum < 1073741824.f)) == 0; }
+  // raises m to the block's maximum and weighs it again
+  __device__ __forceinline__ float raise(const f32x16& s, float scale_log2, AttnFrag<T>* pf) {
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    const float nm = fmaxf(m, pair_max(mx) * scale_log2);
+    const float ms = nm == -INFINITY ? 0.f : nm;
+    const float alpha = exp2_fast(m - ms);
+    m = nm;
+    l *= alpha;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+    return weigh(s, scale_log2, ms, pf);
+  }
+};
 
-// One workgroup: 4 wavefronts and a loop over tiles of keys.  Scores are computed transposed (S^T = K Q^T, a lane owns one
-// query), so the row maximum is an in-lane reduction plus one exchange, the running statistics are one register, and S^T is
-// the operand of O^T = V^T P^T as it lies (attn.h).
-//   FEW = false  128 rows, 32 to a wavefront; tiles of 64 keys that every wavefront reads
-//   FEW = true   at most 32 rows (a query token, class queries): all wavefronts take the same rows and each its own 32 keys
-//                of a tile of 128; their parts are joined in LDS at the end
-// MASKED: a pair mask and / or a key mask is read, one tile ahead of its use.
-template <typename T, int DP, bool FEW, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : FWD_W)) void attn_fwd_kernel(const AttnDev p) {
+// Row tiles: 4 wavefronts of 32 rows, tiles of 64 keys shared through LDS.  A wavefront works on three blocks at a time:
+// the scores of block b + 1 and the values of block b - 1 on the matrix cores while the exponentials of block b run on the
+// vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
+// tiles; K runs one tile ahead of V.
+template <typename T, int DP, bool MASKED>
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
-  typedef AttnRead<T, DP> Rd;
-  constexpr int KT = FEW ? 128 : 64, NKB = FEW ? 1 : 2;
-  constexpr int KS = DP / 16, DB = DP / 32;
+  constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // K tiles 0, 1, V tiles 0, 1
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   const AttnWork w = attn_work(p);
   if (w.n < 0) return;
-  const int n = w.n, hk = w.hk, tile = w.tile;
-  const int row0 = FEW ? 0 : tile * 128 + wave * 32;      // of this wavefront
-  const bool idle = row0 >= p.R;                          // it then only helps to stage the tiles
+  const int n = w.n, hk = w.hk;
+  const int row0 = w.tile * 128 + wave * 32;
 
   // keys that some row of the workgroup may use
-  const int last_row = min(FEW ? 32 : tile * 128 + 128, p.R) - 1;
+  const int last_row = min(w.tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
+  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
+  if (MASKED && kmask) k_end = min(k_end, last_open_key(kmask, p.km_k, k_end, lane) + 1);
   const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + w.parts - 1) / w.parts;
   const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
@@ -53,201 +92,109 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
     for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<T>(src, ks, h, p.D, row_ok);
   }
   const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0, p.R - 1)));
+  // last key open to the lane's row, and the first key that is closed to some row of the wavefront
+  const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - 4 * h;
+  const int ragged0 = p.causal ? min(p.Lk, wave_tok0 + p.off + 1) : p.Lk;
 
   const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
-  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
-  AttnPairMask<NKB> pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k,
-                       p.Lk, (FEW ? wave * 32 : 0) + 4 * h);
+  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
+  unsigned long long bits_now = ~0ULL, bits_next = ~0ULL;   // of the V tile and of the K tile last asked for
+  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
+  constexpr int key_b = 32 * Tile::PITCH;
+  constexpr std::integral_constant<int, 0> zero, no;
+  constexpr std::integral_constant<int, 1> one, yes;
 
-  f32x16 o[DB];
-  float m = -INFINITY, l = 0.f;
+  AttnRow<T, DB> row;
+  f32x16 s[2];
+  AttnFrag<T> pf[2][2];
+
+  const AttnLane<T, DP> ln(smem, lane);
+  // scores and values of the block at LDS byte `at`
+  auto scores = [&](f32x16& x, int at) __attribute__((always_inline)) {
+    x = zero16();
 #pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = zero16();
+    for (int ks = 0; ks < KS; ++ks) mma32(x, ln.rows(at, ks), qf[ks]);
+  };
+  auto values = [&](const AttnFrag<T>* f, int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) mma32(row.o[db], ln.cols(at + j * 16 * Tile::PITCH, db), f[j]);
+  };
+  // block b of parity `odd`: its scores are in s[odd]; next_k / last_v: the K block after it, the V block before it
+  auto block = [&](int key0, auto odd_, auto with_k, int next_k, auto with_v, int last_v) __attribute__((always_inline)) {
+    constexpr int odd = odd_.value;
+    unsigned word = 0;
+    if (MASKED && kmask) word = (unsigned)(bits_now >> (odd * 32));
+    close_pairs<MASKED>(s[odd], -INFINITY, key0 + 32 > ragged0, lim - key0, kmask ? &word : nullptr, h, pm.row ? pm.w : nullptr);
+    if (MASKED) pm.load(key0 + 32);
+    if constexpr (with_k.value) scores(s[odd ^ 1], next_k);
+    float sum = row.weigh(s[odd], p.scale_log2, row.m, pf[odd]);
+    if constexpr (with_v.value) values(pf[odd ^ 1], last_v);
+#ifdef IL
+    if constexpr (with_k.value && with_v.value) interleave<T, 4 * DB, 6 * DB>();
+#endif
+    pin(pf[odd][0]);
+    pin(pf[odd][1]);
+    if (__builtin_expect(!row.fine(sum), 0)) sum = row.raise(s[odd], p.scale_log2, pf[odd]);
+    row.l += sum;
+  };
 
   if (t0 < t1) {
+    // tiles are counted from t0 (u = 0, 1, ...)
+    const int last = t1 - t0 - 1;
     if (MASKED) {
       km.load(t0 * KT);
       km.next();
+      bits_now = km.bits[0];
       km.load((t0 + 1) * KT);
       pm.load(t0 * KT);
     }
-    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
-  }
-  // (two steps to a turn of the loop: the buffer is a constant of each)
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
-    tile_barrier();                       // tile t is here; every wavefront has left tile t - 1
-    const int key0 = t * KT + (FEW ? wave * 32 : 0);
-    unsigned kw[NKB], pw[NKB][4];
-    bool dead = idle;
+    st.template one<KT, MASKED>(p, st.kbase, st.k_step, t0 * KT, 0, bits_now);
+    st.template one<KT, MASKED>(p, st.vbase, st.v_step, t0 * KT, 2 * TILE_B, bits_now);
     if (MASKED) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        kw[kb] = km.word((FEW ? wave * 32 : 0) + kb * 32);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) pw[kb][g] = pm.w[kb][g];
-      }
-      dead = dead || !(NKB == 2 ? kw[0] | kw[NKB - 1] : kw[0]);
-      if (pm.row && !dead) {
-        unsigned some = 0;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) some |= pw[kb][g];
-        dead = !__any(row_ok && some != 0);
-      }
+      km.next();
+      bits_next = km.bits[0];
+      km.load((t0 + 2) * KT);
     }
-    // The next tile is asked for behind this tile's first LDS reads: a wavefront's LDS reads queue behind its own LDS-DMA.
-    auto stage_next = [&]() {
-      if (t + 1 >= t1) return;
+    tile_barrier();
+    if (last > 0) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t0 + 1) * KT, TILE_B, bits_next);
+    scores(s[0], 0);
+    block(t0 * KT, zero, yes, key_b, no, 0);
+    // The second block of tile u and the first of tile u + 1; two turns to a round of the loop, so that the buffers are
+    // constants of each.
+    auto turn = [&](int u, auto even_) __attribute__((always_inline)) {
+      constexpr int here = even_.value * TILE_B, there = TILE_B - here;
+      tile_barrier();       // K tile u + 1 and V tile u are here; every wavefront is done with K tile u and V tile u - 1
+      const int t = t0 + u;
+      unsigned long long bits2 = ~0ULL;
       if (MASKED) {
         km.next();
-        km.load((t + 2) * KT);
-        pm.load((t + 1) * KT);
+        bits2 = km.bits[0];
+        km.load((t + 3) * KT);
       }
-      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+      if (u + 2 <= last) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t + 2) * KT, here, bits2);
+      st.template one<KT, MASKED>(p, st.vbase, st.v_step, (t + 1) * KT, 2 * TILE_B + there, bits_next);
+      block(t * KT + 32, one, yes, there, yes, 2 * TILE_B + here);
+      if (MASKED) {
+        bits_now = bits_next;
+        bits_next = bits2;
+      }
+      block((t + 1) * KT, zero, yes, there + key_b, yes, 2 * TILE_B + here + key_b);
     };
-    if (dead) {                           // nothing of this tile is open to this wavefront's rows
-      stage_next();
-      return;
+    int u = 0;
+    for (; u + 1 < last; u += 2) {
+      turn(u, zero);
+      turn(u + 1, one);
     }
-    const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
-    const char* vt = kt + TILE_B;
-
-    f32x16 s[NKB];
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) s[kb] = zero16();
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) mma32(s[kb], Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
-    stage_next();
-
-    // closed pairs: past the last key, above the diagonal, masked
-    if (key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off)) {
-      keep_branch();
-      const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = kb * 32 + 8 * (i >> 2) + (i & 3) <= lim ? s[kb][i] : -INFINITY;
-    }
-    if (MASKED) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        if (km.mask) {
-          const unsigned x = kw[kb] >> (4 * h);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[kb][i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[kb][i] : -INFINITY;
-        }
-        if (pm.row) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[kb][i] = pw[kb][i >> 2] & (0xffu << (8 * (i & 3))) ? s[kb][i] : -INFINITY;
-        }
-      }
-    }
-
-    // p = exp2(s scale log2(e) - m) for a reference m that need not be the maximum: in floating point any m serves that
-    // neither overflows nor loses the largest terms.  m starts as the maximum of the first tile that has an open key and
-    // is raised (accumulators rescaled) only when a tile's sum passes 2^30, so that the common tile needs no maximum.
-    // m = -inf makes the sum infinite or NaN, as do such scores: the raising path sorts those out, too.
-    AttnFrag<T> pf[2 * NKB];
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2 * NKB; ++j) {
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[j >> 1][8 * (j & 1) + i], p.scale_log2, -m));
-      pf[j] = pack_sum<T>(e, sum);
-    }
-    if (__builtin_expect(!__all(sum < 1073741824.f), 0)) {
-      float mx = s[0][0];
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-      const float nm = fmaxf(m, pair_max(mx) * p.scale_log2);
-      const float ms = nm == -INFINITY ? 0.f : nm;
-      const float alpha = exp2_fast(m - ms);
-      m = nm;
-      l *= alpha;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-      sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * NKB; ++j) {
-        float e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[j >> 1][8 * (j & 1) + i], p.scale_log2, -ms));
-        pf[j] = pack_sum<T>(e, sum);
-      }
-    }
-    l += sum;
-#pragma unroll
-    for (int j = 0; j < 2 * NKB; ++j)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) mma32(o[db], Rd::cols(vt, j * 16, db * 32, lane), pf[j]);
-  };
-  int t = t0;
-  for (; t + 1 < t1; t += 2) {
-    step(t, 0);
-    step(t + 1, 1);
+    if (u < last) turn(u, zero);
+    tile_barrier();
+    const int v = (2 + (last & 1)) * TILE_B;
+    block((t0 + last) * KT + 32, one, no, 0, yes, v);
+    values(pf[1], v + key_b);
   }
-  if (t < t1) step(t, 0);
 
-  float lt = pair_sum(l);
-  if constexpr (FEW) {
-    // join the four wavefronts' parts: [wave][row][DP + 4] sums, then 4 x 32 maxima and sums
-    constexpr int LD = DP + 4;
-    float* const so = reinterpret_cast<float*>(smem);
-    float* const sm = so + 4 * 32 * LD;
-    tile_barrier();
-    if (h == 0) sm[wave * 32 + l31] = m;
-    tile_barrier();
-    float all = sm[l31];
-#pragma unroll
-    for (int i = 1; i < 4; ++i) all = fmaxf(all, sm[i * 32 + l31]);
-    const float a = exp2_fast(m - (all == -INFINITY ? 0.f : all));
-    if (h == 0) sm[128 + wave * 32 + l31] = lt * a;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
-            f32x4{o[db][i] * a, o[db][i + 1] * a, o[db][i + 2] * a, o[db][i + 3] * a};
-    tile_barrier();
-    for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
-      const int row = x / (DP / 4), d = x % (DP / 4) * 4;
-      if (row >= p.R || d >= p.D) continue;
-      f32x4 v = *reinterpret_cast<const f32x4*>(so + row * LD + d);
-      float sum = sm[128 + row], top = sm[row];
-#pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + row) * LD + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += y[e];
-        sum += sm[128 + i * 32 + row];
-        top = fmaxf(top, sm[i * 32 + row]);
-      }
-      if (w.parts == 1) {
-        const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store4<T>(p.out + ((long long)n * p.o.n + (long long)tk * p.o.l + (long long)hd * p.o.h) * (int)sizeof(T), d, v[0] * inv, v[1] * inv,
-                  v[2] * inv, v[3] * inv);
-        if (p.lse && d == 0)
-          p.lse[((long long)n * p.Hq + hd) * p.Lq + tk] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-      } else {
-        const long long at = ((long long)w.slot * p.parts + w.part) * p.R + row;
-        store4<float>((char*)(p.part + at * p.D), d, v[0], v[1], v[2], v[3]);
-        if (d == 0) {
-          p.part_ml[2 * at] = top;
-          p.part_ml[2 * at + 1] = sum;
-        }
-      }
-    }
-    return;
-  }
+  const float lt = pair_sum(row.l);
   if (!row_ok) return;
   if (w.parts == 1) {
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
@@ -257,10 +204,10 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int d = db * 32 + 2 * i + 4 * h;
-        if (d < p.D) store4<T>(dst, d, o[db][i] * inv, o[db][i + 1] * inv, o[db][i + 2] * inv, o[db][i + 3] * inv);
+        if (d < p.D) store4<T>(dst, d, row.o[db][i] * inv, row.o[db][i + 1] * inv, row.o[db][i + 2] * inv, row.o[db][i + 3] * inv);
       }
     if (p.lse && h == 0)
-      p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.6931471805599453f;
+      p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (row.m + log2f(lt)) * 0.6931471805599453f;
   } else {
     const long long at = ((long long)w.slot * p.parts + w.part) * 128 + wave * 32 + l31;
     char* dst = (char*)(p.part + at * p.D);
@@ -269,11 +216,148 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int d = db * 32 + 2 * i + 4 * h;
-        if (d < p.D) store4<float>(dst, d, o[db][i], o[db][i + 1], o[db][i + 2], o[db][i + 3]);
+        if (d < p.D) store4<float>(dst, d, row.o[db][i], row.o[db][i + 1], row.o[db][i + 2], row.o[db][i + 3]);
       }
     if (h == 0) {
-      p.part_ml[2 * at] = m;
+      p.part_ml[2 * at] = row.m;
       p.part_ml[2 * at + 1] = lt;
+    }
+  }
+}
+
+// At most 32 rows (a query token, class queries): the wavefronts take the same rows and each its own 32 keys of a tile of
+// 128; their parts are joined in LDS at the end.  Memory-bound: nothing is pipelined but the tiles.  Blocks that the masks
+// close for every row are skipped.
+template <typename T, int DP, bool MASKED>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_fwd_few_kernel(const AttnDev p) {
+  typedef AttnTile<T, DP> Tile;
+  typedef AttnRead<T, DP> Rd;
+  constexpr int KT = 128, KS = DP / 16, DB = DP / 32;
+  constexpr int TILE_B = KT * Tile::PITCH;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
+  const AttnWork w = attn_work(p);
+  if (w.n < 0) return;
+  const int n = w.n, hk = w.hk;
+
+  int k_end = p.Lk;
+  if (p.causal) k_end = max(0, min(k_end, div_g(p, p.R - 1) + p.off + 1));
+  const int all_steps = (k_end + KT - 1) / KT;
+  const int per = (all_steps + w.parts - 1) / w.parts;
+  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
+
+  const bool row_ok = l31 < p.R;
+  const int rr = row_ok ? l31 : 0;
+  const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
+  AttnFrag<T> qf[KS];
+  {
+    const char* src = p.q.p + ((long long)n * p.q.n + (long long)tok * p.q.l + (long long)head * p.q.h) * (int)sizeof(T);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<T>(src, ks, h, p.D, row_ok);
+  }
+  const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - 4 * h;
+  const int ragged0 = p.causal ? min(p.Lk, p.off + 1) : p.Lk;      // (row 0 is token 0)
+
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
+  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
+
+  AttnRow<T, DB> row;
+  if (t0 < t1) {
+    if (MASKED) {
+      km.load(t0 * KT);
+      km.next();
+      km.load((t0 + 1) * KT);
+      pm.load(t0 * KT + wave * 32);
+    }
+    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    tile_barrier();                       // tile t is here; every wavefront has left tile t - 1
+    const int key0 = t * KT + wave * 32;
+    unsigned word = 0, pair[4];
+    bool dead = false;
+    if (MASKED) {
+      word = km.word(wave * 32);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) pair[g] = pm.w[g];
+      dead = word == 0;
+      if (pm.row && !dead) dead = !__any(row_ok && (pair[0] | pair[1] | pair[2] | pair[3]) != 0);
+    }
+    if (t + 1 < t1) {
+      if (MASKED) {
+        km.next();
+        km.load((t + 2) * KT);
+        pm.load((t + 1) * KT + wave * 32);
+      }
+      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    }
+    if (dead) continue;
+    const char* kt = smem + buf * (2 * TILE_B) + wave * 32 * Tile::PITCH;
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, 0, ks, lane), qf[ks]);
+    close_pairs<MASKED>(s, -INFINITY, key0 + 32 > ragged0, lim - key0, km.mask ? &word : nullptr, h, pm.row ? pair : nullptr);
+    AttnFrag<T> pf[2];
+    float sum = row.weigh(s, p.scale_log2, row.m, pf);
+    if (!row.fine(sum)) sum = row.raise(s, p.scale_log2, pf);
+    row.l += sum;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) mma32(row.o[db], Rd::cols(kt + TILE_B, j * 16, db * 32, lane), pf[j]);
+  }
+
+  // join the four wavefronts' parts: [wave][row][DP + 4] sums, then 4 x 32 maxima and sums
+  const float lt = pair_sum(row.l);
+  constexpr int LD = DP + 4;
+  float* const so = reinterpret_cast<float*>(smem);
+  float* const sm = so + 4 * 32 * LD;
+  tile_barrier();
+  if (h == 0) sm[wave * 32 + l31] = row.m;
+  tile_barrier();
+  float all = sm[l31];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) all = fmaxf(all, sm[i * 32 + l31]);
+  const float a = exp2_fast(row.m - (all == -INFINITY ? 0.f : all));
+  if (h == 0) sm[128 + wave * 32 + l31] = lt * a;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
+          f32x4{row.o[db][i] * a, row.o[db][i + 1] * a, row.o[db][i + 2] * a, row.o[db][i + 3] * a};
+  tile_barrier();
+  for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
+    const int rw = x / (DP / 4), d = x % (DP / 4) * 4;
+    if (rw >= p.R || d >= p.D) continue;
+    f32x4 v = *reinterpret_cast<const f32x4*>(so + rw * LD + d);
+    float sum = sm[128 + rw], top = sm[rw];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + rw) * LD + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += y[e];
+      sum += sm[128 + i * 32 + rw];
+      top = fmaxf(top, sm[i * 32 + rw]);
+    }
+    if (w.parts == 1) {
+      const int tk = div_g(p, rw), hd = hk * p.G + rw - tk * p.G;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store4<T>(p.out + ((long long)n * p.o.n + (long long)tk * p.o.l + (long long)hd * p.o.h) * (int)sizeof(T), d, v[0] * inv, v[1] * inv,
+                v[2] * inv, v[3] * inv);
+      if (p.lse && d == 0)
+        p.lse[((long long)n * p.Hq + hd) * p.Lq + tk] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    } else {
+      const long long at = ((long long)w.slot * p.parts + w.part) * p.R + rw;
+      store4<float>((char*)(p.part + at * p.D), d, v[0], v[1], v[2], v[3]);
+      if (d == 0) {
+        p.part_ml[2 * at] = top;
+        p.part_ml[2 * at + 1] = sum;
+      }
     }
   }
 }
@@ -497,7 +581,9 @@ static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
   const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
   static std::atomic<int> seen[2][ATTN_DEVICES];
   const bool masked = p->mask || p->kmask;
-  auto kern = masked ? attn_fwd_kernel<T, DP, FEW, true> : attn_fwd_kernel<T, DP, FEW, false>;
+  void (*kern)(const AttnDev);
+  if constexpr (FEW) kern = masked ? attn_fwd_few_kernel<T, DP, true> : attn_fwd_few_kernel<T, DP, false>;
+  else kern = masked ? attn_fwd_kernel<T, DP, true> : attn_fwd_kernel<T, DP, false>;
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
   p->tiles = FEW ? 1 : ceil_div(p->R, 128);
