@@ -468,7 +468,7 @@ struct AttnStage {
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 // Key mask of a tile of KT keys as one bit per key, the same in every wavefront: load() asks for a tile's bytes, next()
-// turns the bytes asked for last into bits.  Without a mask all bits are set.
+// turns the bytes asked for last into bits.  Without a mask a key's bit says whether the key exists.
 template <int KT>
 struct AttnKeyMask {
   const unsigned char* mask;
@@ -476,37 +476,58 @@ struct AttnKeyMask {
   int Lk, lane;
   unsigned char raw[KT / 64];
   unsigned long long bits[KT / 64];
-  __device__ __forceinline__ AttnKeyMask(const unsigned char* m, long long s, int lk, int ln) : mask(m), step(s), Lk(lk), lane(ln) {
-#pragma unroll
-    for (int i = 0; i < KT / 64; ++i) {
-      raw[i] = 1;
-      bits[i] = ~0ULL;
-    }
-  }
+  __device__ __forceinline__ AttnKeyMask(const unsigned char* m, long long s, int lk, int ln) : mask(m), step(s), Lk(lk), lane(ln) {}
   __device__ __forceinline__ void load(int key0) {
-    if (!mask) return;
 #pragma unroll
     for (int i = 0; i < KT / 64; ++i) {
       const int j = key0 + i * 64 + lane;
-      raw[i] = j < Lk ? mask[j * step] : 0;
+      raw[i] = j < Lk ? (mask ? mask[j * step] : 1) : 0;
     }
   }
   __device__ __forceinline__ void next() {
-    if (!mask) return;
 #pragma unroll
     for (int i = 0; i < KT / 64; ++i) bits[i] = __ballot(raw[i] != 0);
   }
   __device__ __forceinline__ unsigned word(int key) const { return (unsigned)(bits[KT == 64 ? 0 : key >> 6] >> (key & 63)); }
 };
 
-// The last of the first `keys` keys that the mask leaves open, -1 if none: a wavefront's answer.
+// The closed keys of a tile of 64 as what the products of its scores start from: 0 or -inf for every key, in LDS.
+__device__ __forceinline__ void write_start(char* at, unsigned long long bits, int lane) {
+  reinterpret_cast<float*>(at)[lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
+}
+__device__ __forceinline__ f32x16 read_start(const char* at, int h) {
+  f32x16 x;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const f32x4 y = reinterpret_cast<const f32x4*>(at)[i / 2 + h];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i + e] = y[e];
+  }
+  return x;
+}
+
+// The last of the first `keys` keys that the mask leaves open, -1 if none: a wavefront's answer, 256 keys at a time.
 __device__ __forceinline__ int last_open_key(const unsigned char* mask, long long step, int keys, int lane) {
-  for (int j0 = (keys - 1) / 64 * 64; j0 >= 0 && keys > 0; j0 -= 64) {
-    const int j = j0 + lane;
-    const unsigned long long open = __ballot(j < keys && mask[j * step] != 0);
-    if (open) return j0 + 63 - __builtin_clzll(open);
+  for (int j0 = (keys - 1) / 256 * 256; j0 >= 0 && keys > 0; j0 -= 256) {
+    unsigned char x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * 64 + lane;
+      x[i] = j < keys ? mask[j * step] : 0;
+    }
+    for (int i = 3; i >= 0; --i) {
+      const unsigned long long open = __ballot(x[i] != 0);
+      if (open) return j0 + i * 64 + 63 - __builtin_clzll(open);
+    }
   }
   return -1;
+}
+
+// Whether any of the 128 keys from key0 is open: the same answer in every wavefront.
+__device__ __forceinline__ bool any_open_key(const unsigned char* mask, long long step, int key0, int Lk, int lane) {
+  const int a = key0 + lane, b = a + 64;
+  const unsigned char x = a < Lk ? mask[a * step] : 0, y = b < Lk ? mask[b * step] : 0;
+  return __ballot((x | y) != 0) != 0;
 }
 
 // Pair mask of one row against a block of 32 keys: byte e of w[g] belongs to key 8 g + 4 h + e of the block, the order of a
@@ -537,25 +558,21 @@ struct AttnPairMask {
   }
 };
 
-// Puts `closed` wherever a block's pair is closed: past `lim` (the last open key's place counted from the lane's first),
-// by the key mask's word, by the pair mask.
-template <bool MASKED>
-__device__ __forceinline__ void close_pairs(f32x16& s, float closed, bool ragged, int lim, const unsigned* word, int h,
-                                            const unsigned* pair) {
-  if (ragged) {
-    keep_branch();
+// Puts `closed` wherever a block's pair is closed: past `lim` (the last open key's place counted from the lane's first) ...
+__device__ __forceinline__ void close_past(f32x16& s, float closed, int lim) {
+  keep_branch();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) <= lim ? s[i] : closed;
-  }
-  if (MASKED && word) {
-    const unsigned x = *word >> (4 * h);
+  for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) <= lim ? s[i] : closed;
+}
+// ... by the key mask's word, by the pair mask.
+__device__ __forceinline__ void close_word(f32x16& s, float closed, unsigned word, int h) {
+  const unsigned x = word >> (4 * h);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[i] : closed;
-  }
-  if (MASKED && pair) {
+  for (int i = 0; i < 16; ++i) s[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[i] : closed;
+}
+__device__ __forceinline__ void close_pairs(f32x16& s, float closed, const unsigned* pair) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = pair[i >> 2] & (0xffu << (8 * (i & 3))) ? s[i] : closed;
-  }
+  for (int i = 0; i < 16; ++i) s[i] = pair[i >> 2] & (0xffu << (8 * (i & 3))) ? s[i] : closed;
 }
 
 // maximum and sum over the two lanes that share a result column (l and l ^ 32)

@@ -44,10 +44,13 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   int first = 0;
   if (p.causal) first = max(0, key_wg - p.off) >= p.Lq ? all_steps : max(0, key_wg - p.off) * p.G / QT;
   const int per = (all_steps - first + w.parts - 1) / w.parts;
-  const int t0 = min(first + w.part * per, all_steps), t1 = min(t0 + per, all_steps);
+  const int t0 = min(first + w.part * per, all_steps);
+  int t1 = min(t0 + per, all_steps);
 
   bool key_ok = key < p.Lk;
   if (MASKED && p.kmask && key_ok) key_ok = p.kmask[n * p.km_n + (long long)key * p.km_k] != 0;
+  // (a tile without an open key has nothing to walk over: its gradients are zeros)
+  if (MASKED && p.kmask && !any_open_key(p.kmask + n * p.km_n, p.km_k, key_wg, p.Lk, lane)) t1 = t0;
   AttnFrag<T> kf[KS], vf[VL ? 1 : KS];
   {
     const long long kk = key_ok ? key : 0;
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i + e] = exp2_fast(fmaf(s[i + e], p.scale_log2, -ls[e]));
       }
-      // closed pairs (a closed key's products are those of zeros; the padding rows' lse is +inf)
+      // closed pairs (what a closed key's column holds is not stored; the padding rows' lse is +inf)
       if (p.causal && key_wg + 127 > div_g(p, row0) + p.off) {
         keep_branch();
 #pragma unroll
@@ -172,9 +175,9 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
           s[i] = key <= div_g(p, r) + p.off ? s[i] : 0.f;
         }
       }
-      if (MASKED) {
+      if (MASKED && mkey) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = key_ok && (!mkey || open[i] != 0) ? s[i] : 0.f;
+        for (int i = 0; i < 16; ++i) s[i] = open[i] != 0 ? s[i] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= s[i];
@@ -197,6 +200,10 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   if (t < t1) step(t, 0);
 
   if (key >= p.Lk) return;
+  if (MASKED && !key_ok) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
+  }
   const long long at = (((long long)n * p.Lk + key) * p.Hk + hk) * p.D;
   if (w.parts == 1) {
 #pragma unroll

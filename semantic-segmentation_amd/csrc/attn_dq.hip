@@ -135,7 +135,11 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
       if (kb == 0) stage_next();
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (START ? dp[i] : dp[i] + minus);
-      close_pairs<MASKED>(dp, 0.f, ragged, lim - kb * 32, km.mask ? &kw[kb] : nullptr, h, pm.row ? pw[kb] : nullptr);
+      if (ragged) close_past(dp, 0.f, lim - kb * 32);
+      if (MASKED) {
+        close_word(dp, 0.f, kw[kb], h);
+        if (pm.row) close_pairs(dp, 0.f, pw[kb]);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const AttnFrag<T> sf = pack_frag<T>(dp, j);

@@ -62,7 +62,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   typedef AttnTile<T, DP> Tile;
   constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];   // K tiles 0, 1, V tiles 0, 1
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // K tiles 0, 1, V tiles 0, 1; MASKED: 2 x 64 starts
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
@@ -71,15 +71,33 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   const int n = w.n, hk = w.hk;
   const int row0 = w.tile * 128 + wave * 32;
 
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
+  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
+  unsigned long long bits_next = ~0ULL;      // open keys of the K tile last asked for: V follows
+
   // keys that some row of the workgroup may use
   const int last_row = min(w.tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
-  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
   if (MASKED && kmask) k_end = min(k_end, last_open_key(kmask, p.km_k, k_end, lane) + 1);
   const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + w.parts - 1) / w.parts;
   const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
+  const int last = t1 - t0 - 1;              // tiles are counted from t0: u = 0 .. last
+
+  char* const start0 = smem + 4 * TILE_B;    // MASKED: what the scores of K tiles 0, 1 start from
+  if (t0 < t1) {                             // the first tile is asked for before anything else
+    if (MASKED) {
+      km.load(t0 * KT);
+      km.next();
+      bits_next = km.bits[0];
+      km.load((t0 + 1) * KT);
+      if (wave == 0) write_start(start0, bits_next, lane);
+    }
+    st.template one<KT, MASKED>(p, st.kbase, st.k_step, t0 * KT, 0, bits_next);
+    st.template one<KT, MASKED>(p, st.vbase, st.v_step, t0 * KT, 2 * TILE_B, bits_next);
+  }
 
   const int r = row0 + l31;
   const bool row_ok = r < p.R;
@@ -96,9 +114,6 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - 4 * h;
   const int ragged0 = p.causal ? min(p.Lk, wave_tok0 + p.off + 1) : p.Lk;
 
-  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
-  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
-  unsigned long long bits_now = ~0ULL, bits_next = ~0ULL;   // of the V tile and of the K tile last asked for
   AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
   constexpr int key_b = 32 * Tile::PITCH;
   constexpr std::integral_constant<int, 0> zero, no;
@@ -109,9 +124,10 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
   AttnFrag<T> pf[2][2];
 
   const AttnLane<T, DP> ln(smem, lane);
-  // scores and values of the block at LDS byte `at`
-  auto scores = [&](f32x16& x, int at) __attribute__((always_inline)) {
-    x = zero16();
+  // scores and values of the block at LDS byte `at`; `half` of K tile `buf`
+  auto scores = [&](f32x16& x, int at, int buf, int half) __attribute__((always_inline)) {
+    if (MASKED) x = read_start(start0 + buf * 256 + half * 128, h);
+    else x = zero16();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) mma32(x, ln.rows(at, ks), qf[ks]);
   };
@@ -121,66 +137,69 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
 #pragma unroll
       for (int db = 0; db < DB; ++db) mma32(row.o[db], ln.cols(at + j * 16 * Tile::PITCH, db), f[j]);
   };
-  // block b of parity `odd`: its scores are in s[odd]; next_k / last_v: the K block after it, the V block before it
-  auto block = [&](int key0, auto odd_, auto with_k, int next_k, auto with_v, int last_v) __attribute__((always_inline)) {
+  // block b of parity `odd`: its scores are in s[odd]; next_k: the K block after it (of tile buffer next_buf), last_v: the V
+  // block before it
+  auto block = [&](int key0, auto odd_, auto with_k, int next_k, int next_buf, auto with_v, int last_v) __attribute__((always_inline)) {
     constexpr int odd = odd_.value;
-    unsigned word = 0;
-    if (MASKED && kmask) word = (unsigned)(bits_now >> (odd * 32));
-    close_pairs<MASKED>(s[odd], -INFINITY, key0 + 32 > ragged0, lim - key0, kmask ? &word : nullptr, h, pm.row ? pm.w : nullptr);
-    if (MASKED) pm.load(key0 + 32);
-    if constexpr (with_k.value) scores(s[odd ^ 1], next_k);
+    if (key0 + 32 > ragged0) close_past(s[odd], -INFINITY, lim - key0);
+    if (MASKED && pm.row) {
+      close_pairs(s[odd], -INFINITY, pm.w);
+      pm.load(key0 + 32);
+    }
+    if constexpr (with_k.value) scores(s[odd ^ 1], next_k, next_buf, odd ^ 1);
     float sum = row.weigh(s[odd], p.scale_log2, row.m, pf[odd]);
     if constexpr (with_v.value) values(pf[odd ^ 1], last_v);
-#ifdef IL
-    if constexpr (with_k.value && with_v.value) interleave<T, 4 * DB, 6 * DB>();
-#endif
     pin(pf[odd][0]);
     pin(pf[odd][1]);
     if (__builtin_expect(!row.fine(sum), 0)) sum = row.raise(s[odd], p.scale_log2, pf[odd]);
     row.l += sum;
   };
+  // at the barrier of turn u: K tile u + 1 and V tile u are here; every wavefront is done with K tile u and V tile u - 1
+  auto stage = [&](int u, int here) __attribute__((always_inline)) {
+    const int t = t0 + u, there = TILE_B - here;
+    unsigned long long bits2 = ~0ULL;
+    if (MASKED) {
+      km.next();
+      bits2 = km.bits[0];
+      km.load((t + 3) * KT);
+      if (wave == 0) write_start(start0 + (here ? 256 : 0), bits2, lane);
+    }
+    if (u + 2 <= last) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t + 2) * KT, here, bits2);
+    st.template one<KT, MASKED>(p, st.vbase, st.v_step, (t + 1) * KT, 2 * TILE_B + there, bits_next);
+    if (MASKED) bits_next = bits2;
+  };
 
   if (t0 < t1) {
-    // tiles are counted from t0 (u = 0, 1, ...)
-    const int last = t1 - t0 - 1;
     if (MASKED) {
-      km.load(t0 * KT);
-      km.next();
-      bits_now = km.bits[0];
-      km.load((t0 + 1) * KT);
-      pm.load(t0 * KT);
-    }
-    st.template one<KT, MASKED>(p, st.kbase, st.k_step, t0 * KT, 0, bits_now);
-    st.template one<KT, MASKED>(p, st.vbase, st.v_step, t0 * KT, 2 * TILE_B, bits_now);
-    if (MASKED) {
+      if (pm.row) pm.load(t0 * KT);
       km.next();
       bits_next = km.bits[0];
       km.load((t0 + 2) * KT);
     }
     tile_barrier();
-    if (last > 0) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t0 + 1) * KT, TILE_B, bits_next);
-    scores(s[0], 0);
-    block(t0 * KT, zero, yes, key_b, no, 0);
+    if (last > 0) {
+      st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t0 + 1) * KT, TILE_B, bits_next);
+      if (MASKED && wave == 0) write_start(start0 + 256, bits_next, lane);
+    }
+    if (row0 >= p.R) {          // no rows: this wavefront only helps to stage the tiles
+      for (int u = 0; u < last; ++u) {
+        tile_barrier();
+        stage(u, (u & 1) * TILE_B);
+      }
+      tile_barrier();
+      return;
+    }
+    scores(s[0], 0, 0, 0);
+    block(t0 * KT, zero, yes, key_b, 0, no, 0);
     // The second block of tile u and the first of tile u + 1; two turns to a round of the loop, so that the buffers are
     // constants of each.
     auto turn = [&](int u, auto even_) __attribute__((always_inline)) {
       constexpr int here = even_.value * TILE_B, there = TILE_B - here;
-      tile_barrier();       // K tile u + 1 and V tile u are here; every wavefront is done with K tile u and V tile u - 1
-      const int t = t0 + u;
-      unsigned long long bits2 = ~0ULL;
-      if (MASKED) {
-        km.next();
-        bits2 = km.bits[0];
-        km.load((t + 3) * KT);
-      }
-      if (u + 2 <= last) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t + 2) * KT, here, bits2);
-      st.template one<KT, MASKED>(p, st.vbase, st.v_step, (t + 1) * KT, 2 * TILE_B + there, bits_next);
-      block(t * KT + 32, one, yes, there, yes, 2 * TILE_B + here);
-      if (MASKED) {
-        bits_now = bits_next;
-        bits_next = bits2;
-      }
-      block((t + 1) * KT, zero, yes, there + key_b, yes, 2 * TILE_B + here + key_b);
+      tile_barrier();
+      stage(u, here);
+      const int key0 = (t0 + u) * KT + 32;
+      block(key0, one, yes, there, even_.value ^ 1, yes, 2 * TILE_B + here);
+      block(key0 + 32, zero, yes, there + key_b, even_.value ^ 1, yes, 2 * TILE_B + here + key_b);
     };
     int u = 0;
     for (; u + 1 < last; u += 2) {
@@ -189,9 +208,13 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2))
     }
     if (u < last) turn(u, zero);
     tile_barrier();
-    const int v = (2 + (last & 1)) * TILE_B;
-    block((t0 + last) * KT + 32, one, no, 0, yes, v);
-    values(pf[1], v + key_b);
+    const int v = (2 + (last & 1)) * TILE_B, key0 = (t0 + last) * KT + 32;
+    if (key0 < k_end) {
+      block(key0, one, no, 0, 0, yes, v);
+      values(pf[1], v + key_b);
+    } else {
+      values(pf[0], v);
+    }
   }
 
   const float lt = pair_sum(row.l);
@@ -300,7 +323,11 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_fwd_few_kernel(const Att
     f32x16 s = zero16();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, 0, ks, lane), qf[ks]);
-    close_pairs<MASKED>(s, -INFINITY, key0 + 32 > ragged0, lim - key0, km.mask ? &word : nullptr, h, pm.row ? pair : nullptr);
+    if (key0 + 32 > ragged0) close_past(s, -INFINITY, lim - key0);
+    if (MASKED) {
+      close_word(s, -INFINITY, word, h);
+      if (pm.row) close_pairs(s, -INFINITY, pair);
+    }
     AttnFrag<T> pf[2];
     float sum = row.weigh(s, p.scale_log2, row.m, pf);
     if (!row.fine(sum)) sum = row.raise(s, p.scale_log2, pf);
@@ -578,9 +605,9 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
 
 template <typename T, int DP, bool FEW>
 static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
-  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
   static std::atomic<int> seen[2][ATTN_DEVICES];
   const bool masked = p->mask || p->kmask;
+  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH + (masked && !FEW ? 512 : 0);
   void (*kern)(const AttnDev);
   if constexpr (FEW) kern = masked ? attn_fwd_few_kernel<T, DP, true> : attn_fwd_few_kernel<T, DP, false>;
   else kern = masked ? attn_fwd_kernel<T, DP, true> : attn_fwd_kernel<T, DP, false>;
