@@ -2,13 +2,11 @@
 //   dv_j = sum_i p_ij dout_i,   ds_ij = p_ij (dout_i . v_j - delta_i),   dk_j = scale sum_i ds_ij q_i.
 // A workgroup owns 128 keys and walks over the packed rows (tokens x heads of the group): shared heads add up in its
 // registers, nothing is added atomically, every sum has a fixed order.
+#include <type_traits>
+
 #include "attn.h"
 
 namespace segk {
-
-#ifndef DKV_W
-#define DKV_W 2
-#endif
 
 template <typename T, int DP>
 constexpr bool dkv_v_in_lds() { return DP * (int)sizeof(T) >= 192; }
@@ -21,7 +19,7 @@ constexpr int dkv_rows() { return dkv_v_in_lds<T, DP>() ? 32 : 64; }
 // V stays in registers too where the heads are small; where they are not (VL) it lies in LDS: 32 registers less bring two
 // wavefronts to a SIMD, which cover each other's exponentials, for a quarter more LDS reads.
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : DKV_W)) void attn_dkv_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
   typedef AttnPiece<T, DP> Piece;
@@ -68,6 +66,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
     }
   }
 
+  const AttnLane<T, DP> ln(smem, lane);
+  const AttnLane<T, DP> lv(smem + wave * 32 * Tile::PITCH, lane);     // (VL: this wavefront's rows of V)
   const Piece pc(wave, lane);
   const int row_b = p.D * (int)sizeof(T);
   const char* const qbase = p.q.p + ((long long)n * p.q.n + (long long)hk * p.G * p.q.h) * (int)sizeof(T);
@@ -92,6 +92,15 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
     qo[i] = place(pc.row + i * Piece::STEP, 0, pc.chunk(i) * 16, p.q);
     go[i] = place(pc.row + i * Piece::STEP, 0, pc.chunk(i) * 16, p.dout);
   }
+  // (their lse is asked for one tile ahead)
+  float live[NPC];
+  auto ask_live = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < NPC; ++i) {
+      const int r = t * QT + pc.row + i * Piece::STEP;
+      live[i] = r < p.R ? lse2[r] : INFINITY;
+    }
+  };
   const unsigned lds0 = lds_addr(smem);
   auto stage = [&](int t, int buf) {
     const int row0 = t * QT;
@@ -111,13 +120,14 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
       for (int i = 0; i < NPC; ++i) {
         const int r = row0 + pc.row + i * Piece::STEP;
         bool ok = r < p.R;
-        if (empty_rows && ok) ok = lse2[r] != INFINITY;
+        if (empty_rows) ok = live[i] != INFINITY;
         const unsigned a = even ? qo[i] : place(r, tok0, pc.chunk(i) * 16, p.q);
         const unsigned b = even ? go[i] : place(r, tok0, pc.chunk(i) * 16, p.dout);
         dma_1k(qr, at + wave * 1024 + i * 4096, ok ? a : ATTN_OOB);
         dma_1k(gr, at + TILE_B + wave * 1024 + i * 4096, ok ? b : ATTN_OOB);
       }
     }
+    if (empty_rows) ask_live(t + 1);
     // (the statistics are padded to 64 rows: of a tile of 32 the lanes past it are told to read nothing)
     const unsigned so = lane < QT ? lane * 4 : ATTN_OOB;
     if (wave == 0) dma_256(buffer_of((const char*)(lse2 + row0)), at + 2 * TILE_B, so);
@@ -128,12 +138,15 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
 
-  if (t0 < t1) stage(t0, 0);
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+  if (t0 < t1) {
+    if (empty_rows) ask_live(t0);
+    stage(t0, 0);
+  }
+  auto step = [&](int t, auto buf_) __attribute__((always_inline)) {
+    constexpr int buf = buf_.value;
     tile_barrier();
-    const char* qt = smem + buf * STAGE_B;
-    const char* gt = qt + TILE_B;
-    const float* st = reinterpret_cast<const float*>(qt + 2 * TILE_B);
+    const int qt = buf * STAGE_B, gt = qt + TILE_B;
+    const float* st = reinterpret_cast<const float*>(smem + qt + 2 * TILE_B);
 #pragma unroll
     for (int rb = 0; rb < QT / 32; ++rb) {
       const int row0 = t * QT + rb * 32;
@@ -155,10 +168,10 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
         for (int e = 0; e < 4; ++e) dp[i + e] = dl[e];
       }
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(qt, rb * 32, ks, lane), kf[ks]);
+      for (int ks = 0; ks < KS; ++ks) mma32(s, ln.rows(qt + rb * 32 * Tile::PITCH, ks), kf[ks]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        mma32(dp, Rd::rows(gt, rb * 32, ks, lane), VL ? Rd::rows(smem + 2 * STAGE_B, wave * 32, ks, lane) : vf[VL ? 0 : ks]);
+        mma32(dp, ln.rows(gt + rb * 32 * Tile::PITCH, ks), VL ? lv.rows(2 * STAGE_B, ks) : vf[VL ? 0 : ks]);
       if (rb == 0 && t + 1 < t1) stage(t + 1, buf ^ 1);     // (behind the first LDS reads, as in the forward kernel)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
@@ -186,18 +199,20 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
         const AttnFrag<T> pf = pack_frag<T>(s, j), sf = pack_frag<T>(dp, j);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          mma32(dv[db], Rd::cols(gt, rb * 32 + j * 16, db * 32, lane), pf);
-          mma32(dk[db], Rd::cols(qt, rb * 32 + j * 16, db * 32, lane), sf);
+          mma32(dv[db], ln.cols(gt + (rb * 32 + j * 16) * Tile::PITCH, db), pf);
+          mma32(dk[db], ln.cols(qt + (rb * 32 + j * 16) * Tile::PITCH, db), sf);
         }
       }
     }
   };
+  constexpr std::integral_constant<int, 0> zero;
+  constexpr std::integral_constant<int, 1> one;
   int t = t0;
   for (; t + 1 < t1; t += 2) {
-    step(t, 0);
-    step(t + 1, 1);
+    step(t, zero);
+    step(t + 1, one);
   }
-  if (t < t1) step(t, 0);
+  if (t < t1) step(t, zero);
 
   if (key >= p.Lk) return;
   if (MASKED && !key_ok) {

@@ -1,191 +1,151 @@
 // Multi-head attention, backward: gradient of the queries, dq_i = scale sum_j ds_ij k_j with ds as in attn_dkv.hip.  The
 // scores are computed a third time instead of adding dq up with atomics from the key-owning workgroups: two more products
 // of seven in all, for sums whose order is fixed.
+#include <type_traits>
+
 #include "attn.h"
 
 namespace segk {
 
-// As the forward kernel (attn_fwd.hip), FEW and MASKED included: a lane owns one query,
+// Both kernels as their forward counterparts (attn_fwd.hip): a lane owns one query,
 //   S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
-template <typename T, int DP, bool FEW, bool MASKED>
+// What a row needs: its statistics and its query and output gradient in registers (zeros for a row that has no open key,
+// whatever its memory holds).
+template <typename T, int DP>
+struct AttnGradRow {
+  static constexpr int KS = DP / 16;
+  int tok, head;
+  float lse2, minus;     // base-2 lse, -delta
+  AttnFrag<T> qf[KS], gf[KS];
+  __device__ __forceinline__ AttnGradRow(const AttnDev& p, int n, int hk, int r, int h) {
+    const bool in = r < p.R;
+    const int rr = in ? r : 0;
+    tok = div_g(p, rr);
+    head = hk * p.G + rr - tok * p.G;
+    const long long stat = ((long long)n * p.Hk + hk) * p.Rp + rr;
+    lse2 = in ? p.row_lse2[stat] : INFINITY;
+    minus = in ? p.minus_delta[stat] : 0.f;
+    const char* qs = p.q.p + ((long long)n * p.q.n + (long long)tok * p.q.l + (long long)head * p.q.h) * (int)sizeof(T);
+    const char* gs = p.dout.p + ((long long)n * p.dout.n + (long long)tok * p.dout.l + (long long)head * p.dout.h) * (int)sizeof(T);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = load_frag<T>(qs, ks, h, p.D, in);
+      gf[ks] = load_frag<T>(gs, ks, h, p.D, in);
+    }
+    const bool live = lse2 != INFINITY;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (unsigned e = 0; e < sizeof(qf[0].v) / sizeof(qf[0].v[0]); ++e) {
+        qf[ks].v[e] = live ? qf[ks].v[e] : 0;
+        gf[ks].v[e] = live ? gf[ks].v[e] : 0;
+      }
+  }
+};
+
+template <typename T, int DP, bool MASKED>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2)) void attn_dq_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
-  typedef AttnRead<T, DP> Rd;
-  constexpr int KT = FEW ? 128 : 64, NKB = FEW ? 1 : 2;
-  constexpr int KS = DP / 16, DB = DP / 32;
+  constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile); MASKED: 2 x 64 starts
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   const AttnWork w = attn_work(p);
   if (w.n < 0) return;
-  const int n = w.n, hk = w.hk, tile = w.tile;
-  const int row0 = FEW ? 0 : tile * 128 + wave * 32;
-  const bool idle = row0 >= p.R;
+  const int n = w.n, hk = w.hk;
+  const int row0 = w.tile * 128 + wave * 32;
 
-  const int last_row = min(FEW ? 32 : tile * 128 + 128, p.R) - 1;
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
+  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
+  char* const start0 = smem + 4 * TILE_B;
+
+  const int last_row = min(w.tile * 128 + 128, p.R) - 1;
   int k_end = p.Lk;
   if (p.causal) k_end = max(0, min(k_end, div_g(p, last_row) + p.off + 1));
-  if (MASKED && !FEW && p.kmask) k_end = min(k_end, last_open_key(p.kmask + n * p.km_n, p.km_k, k_end, lane) + 1);
+  if (MASKED && kmask) k_end = min(k_end, last_open_key(kmask, p.km_k, k_end, lane) + 1);
   const int all_steps = (k_end + KT - 1) / KT;
   const int per = (all_steps + w.parts - 1) / w.parts;
   const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
+  auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+    if (MASKED) {
+      km.next();
+      km.load((t + 1) * KT);
+      if (wave == 0) write_start(start0 + buf * 256, km.bits[0], lane);
+    }
+    st.template keys<KT, MASKED>(p, t * KT, buf, km.bits);
+  };
+  if (t0 < t1) {               // the first tile is asked for before anything else
+    if (MASKED) km.load(t0 * KT);
+    stage(t0, 0);
+  }
 
   const int r = row0 + l31;
-  const bool row_in = r < p.R;
-  const int rr = row_in ? r : 0;
-  const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
-  const long long stat = ((long long)n * p.Hk + hk) * p.Rp + rr;
-  const float lse2 = row_in ? p.row_lse2[stat] : INFINITY;
-  const float minus = row_in ? p.minus_delta[stat] : 0.f;
-  const bool row_ok = lse2 != INFINITY;     // (rows without an open key are not read)
-  AttnFrag<T> qf[KS], gf[KS];
-  {
-    const char* qs = p.q.p + ((long long)n * p.q.n + (long long)tok * p.q.l + (long long)head * p.q.h) * (int)sizeof(T);
-    const char* gs = p.dout.p + ((long long)n * p.dout.n + (long long)tok * p.dout.l + (long long)head * p.dout.h) * (int)sizeof(T);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[ks] = load_frag<T>(qs, ks, h, p.D, row_ok);
-      gf[ks] = load_frag<T>(gs, ks, h, p.D, row_ok);
-    }
-  }
+  const AttnGradRow<T, DP> row(p, n, hk, r, h);
   const int wave_tok0 = __builtin_amdgcn_readfirstlane(div_g(p, min(row0, p.R - 1)));
-
-  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
-  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
-  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
-  unsigned pw_next[NKB][4];
-  auto load_pairs = [&](int t) {
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      pm.load(t * KT + (FEW ? wave * 32 : 0) + kb * 32);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pw_next[kb][g] = pm.w[g];
-    }
-  };
+  const int lim = (p.causal ? min(p.Lk - 1, row.tok + p.off) : p.Lk - 1) - 4 * h;
+  const int ragged0 = p.causal ? min(p.Lk, wave_tok0 + p.off + 1) : p.Lk;
+  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)row.head * p.m_h + (long long)row.tok * p.m_q : nullptr, p.m_k, p.Lk, h);
+  if (MASKED && pm.row && t0 < t1) pm.load(t0 * KT);
 
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = zero16();
-
-  if (t0 < t1) {
-    if (MASKED) {
-      km.load(t0 * KT);
-      km.next();
-      km.load((t0 + 1) * KT);
-      load_pairs(t0);
-    }
-    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
-  }
   // The score gradients' products start from -delta where 16 registers can be spared for it.
   constexpr bool START = DP * (int)sizeof(T) <= 128;
   f32x16 start = zero16();
   if (START) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) start[i] = minus;
+    for (int i = 0; i < 16; ++i) start[i] = row.minus;
   }
 
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+  const AttnLane<T, DP> ln(smem, lane);
+  const bool idle = row0 >= p.R;
+  auto step = [&](int t, auto buf_) __attribute__((always_inline)) {
+    constexpr int buf = buf_.value, kt = buf * 2 * TILE_B, vt = kt + TILE_B;
     tile_barrier();
-    const int key0 = t * KT + (FEW ? wave * 32 : 0);
-    unsigned kw[NKB], pw[NKB][4];
-    bool dead = idle;
-    if (MASKED) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        kw[kb] = km.word((FEW ? wave * 32 : 0) + kb * 32);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) pw[kb][g] = pw_next[kb][g];
-      }
-      dead = dead || !(NKB == 2 ? kw[0] | kw[NKB - 1] : kw[0]);
-      if (pm.row && !dead) {
-        unsigned some = 0;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) some |= pw[kb][g];
-        dead = !__any(row_ok && some != 0);
-      }
-    }
-    auto stage_next = [&]() {       // (behind the first LDS reads, as in the forward kernel)
-      if (t + 1 >= t1) return;
-      if (MASKED) {
-        km.next();
-        km.load((t + 2) * KT);
-        load_pairs(t + 1);
-      }
-      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
-    };
-    if (dead) {
-      stage_next();
+    if (idle) {
+      if (t + 1 < t1) stage(t + 1, buf ^ 1);
       return;
     }
-    const char* kt = smem + buf * (2 * TILE_B) + (FEW ? wave * 32 * Tile::PITCH : 0);
-    const char* vt = kt + TILE_B;
-    const bool ragged = key0 + NKB * 32 > p.Lk || (p.causal && key0 + NKB * 32 - 1 > wave_tok0 + p.off);
-    const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - key0 - 4 * h;
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      f32x16 s = zero16(), dp = START ? start : zero16();
+    for (int kb = 0; kb < 2; ++kb) {
+      const int key0 = t * KT + kb * 32, at = kb * 32 * Tile::PITCH;
+      f32x16 s = MASKED ? read_start(start0 + buf * 256 + kb * 128, h) : zero16(), dp = START ? start : zero16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, kb * 32, ks, lane), qf[ks]);
+      for (int ks = 0; ks < KS; ++ks) mma32(s, ln.rows(kt + at, ks), row.qf[ks]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(vt, kb * 32, ks, lane), gf[ks]);
-      if (kb == 0) stage_next();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -lse2)) * (START ? dp[i] : dp[i] + minus);
-      if (ragged) close_past(dp, 0.f, lim - kb * 32);
-      if (MASKED) {
-        close_word(dp, 0.f, kw[kb], h);
-        if (pm.row) close_pairs(dp, 0.f, pw[kb]);
+      for (int ks = 0; ks < KS; ++ks) mma32(dp, ln.rows(vt + at, ks), row.gf[ks]);
+      if (kb == 0 && t + 1 < t1) stage(t + 1, buf ^ 1);       // (behind the first LDS reads: see the forward kernel)
+      if (key0 + 32 > ragged0) close_past(s, -INFINITY, lim - key0);
+      if (MASKED && pm.row) {
+        close_pairs(s, -INFINITY, pm.w);
+        pm.load(key0 + 32);
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -row.lse2)) * (START ? dp[i] : dp[i] + row.minus);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const AttnFrag<T> sf = pack_frag<T>(dp, j);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) mma32(dq[db], Rd::cols(kt, kb * 32 + j * 16, db * 32, lane), sf);
+        for (int db = 0; db < DB; ++db) mma32(dq[db], ln.cols(kt + at + j * 16 * Tile::PITCH, db), sf);
       }
     }
   };
+  constexpr std::integral_constant<int, 0> zero;
+  constexpr std::integral_constant<int, 1> one;
   int t = t0;
   for (; t + 1 < t1; t += 2) {
-    step(t, 0);
-    step(t + 1, 1);
+    step(t, zero);
+    step(t + 1, one);
   }
-  if (t < t1) step(t, 0);
+  if (t < t1) step(t, zero);
 
-  if constexpr (FEW) {
-    constexpr int LD = DP + 4;
-    float* const so = reinterpret_cast<float*>(smem);
-    tile_barrier();
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
-            f32x4{dq[db][i], dq[db][i + 1], dq[db][i + 2], dq[db][i + 3]};
-    tile_barrier();
-    for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
-      const int row = x / (DP / 4), d = x % (DP / 4) * 4;
-      if (row >= p.R || d >= p.D) continue;
-      f32x4 v = *reinterpret_cast<const f32x4*>(so + row * LD + d);
-#pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + row) * LD + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += y[e];
-      }
-      const int tk = div_g(p, row), hd = hk * p.G + row - tk * p.G;
-      const long long at = (((long long)n * p.Lq + tk) * p.Hq + hd) * p.D;
-      if (w.parts == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
-      else store4<float>((char*)(p.part + (((long long)w.slot * p.parts + w.part) * p.R + row) * p.D), d, v[0], v[1], v[2], v[3]);
-    }
-    return;
-  }
-  if (!row_in) return;
-  const long long at = (((long long)n * p.Lq + tok) * p.Hq + head) * p.D;
+  if (r >= p.R) return;
   if (w.parts == 1) {
+    const long long at = (((long long)n * p.Lq + row.tok) * p.Hq + row.head) * p.D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -203,6 +163,115 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2))
         const int d = db * 32 + 2 * i + 4 * h;
         if (d < p.D) store4<float>(dst, d, dq[db][i], dq[db][i + 1], dq[db][i + 2], dq[db][i + 3]);
       }
+  }
+}
+
+template <typename T, int DP, bool MASKED>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_dq_few_kernel(const AttnDev p) {
+  typedef AttnTile<T, DP> Tile;
+  typedef AttnRead<T, DP> Rd;
+  constexpr int KT = 128, KS = DP / 16, DB = DP / 32;
+  constexpr int TILE_B = KT * Tile::PITCH;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
+  const AttnWork w = attn_work(p);
+  if (w.n < 0) return;
+  const int n = w.n, hk = w.hk;
+
+  int k_end = p.Lk;
+  if (p.causal) k_end = max(0, min(k_end, div_g(p, p.R - 1) + p.off + 1));
+  const int all_steps = (k_end + KT - 1) / KT;
+  const int per = (all_steps + w.parts - 1) / w.parts;
+  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
+
+  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
+  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
+  if (t0 < t1) {
+    if (MASKED) {
+      km.load(t0 * KT);
+      km.next();
+      km.load((t0 + 1) * KT);
+    }
+    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
+  }
+  const AttnGradRow<T, DP> row(p, n, hk, l31, h);
+  const int lim = (p.causal ? min(p.Lk - 1, row.tok + p.off) : p.Lk - 1) - 4 * h;
+  const int ragged0 = p.causal ? min(p.Lk, p.off + 1) : p.Lk;
+  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)row.head * p.m_h + (long long)row.tok * p.m_q : nullptr, p.m_k, p.Lk, h);
+  if (MASKED && t0 < t1) pm.load(t0 * KT + wave * 32);
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dq[db] = zero16();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    tile_barrier();
+    const int key0 = t * KT + wave * 32;
+    unsigned word = 0, pair[4];
+    bool dead = false;
+    if (MASKED) {
+      word = km.word(wave * 32);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) pair[g] = pm.w[g];
+      dead = word == 0;
+      if (pm.row && !dead) dead = !__any(row.lse2 != INFINITY && (pair[0] | pair[1] | pair[2] | pair[3]) != 0);
+    }
+    if (t + 1 < t1) {
+      if (MASKED) {
+        km.next();
+        km.load((t + 2) * KT);
+        pm.load((t + 1) * KT + wave * 32);
+      }
+      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
+    }
+    if (dead) continue;
+    const char* kt = smem + buf * (2 * TILE_B) + wave * 32 * Tile::PITCH;
+    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, 0, ks, lane), row.qf[ks]);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(kt + TILE_B, 0, ks, lane), row.gf[ks]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -row.lse2)) * (dp[i] + row.minus);
+    if (key0 + 32 > ragged0) close_past(dp, 0.f, lim - key0);
+    if (MASKED) {
+      close_word(dp, 0.f, word, h);
+      if (pm.row) close_pairs(dp, 0.f, pair);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const AttnFrag<T> sf = pack_frag<T>(dp, j);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) mma32(dq[db], Rd::cols(kt, j * 16, db * 32, lane), sf);
+    }
+  }
+
+  constexpr int LD = DP + 4;
+  float* const so = reinterpret_cast<float*>(smem);
+  tile_barrier();
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
+          f32x4{dq[db][i], dq[db][i + 1], dq[db][i + 2], dq[db][i + 3]};
+  tile_barrier();
+  for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
+    const int rw = x / (DP / 4), d = x % (DP / 4) * 4;
+    if (rw >= p.R || d >= p.D) continue;
+    f32x4 v = *reinterpret_cast<const f32x4*>(so + rw * LD + d);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + rw) * LD + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += y[e];
+    }
+    const int tk = div_g(p, rw), hd = hk * p.G + rw - tk * p.G;
+    const long long at = (((long long)n * p.Lq + tk) * p.Hq + hd) * p.D;
+    if (w.parts == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
+    else store4<float>((char*)(p.part + (((long long)w.slot * p.parts + w.part) * p.R + rw) * p.D), d, v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -232,10 +301,12 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev
 
 template <typename T, int DP, bool FEW>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
-  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH;
   static std::atomic<int> seen[2][ATTN_DEVICES];
   const bool masked = p->mask || p->kmask;
-  auto kern = masked ? attn_dq_kernel<T, DP, FEW, true> : attn_dq_kernel<T, DP, FEW, false>;
+  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH + (masked && !FEW ? 512 : 0);
+  void (*kern)(const AttnDev);
+  if constexpr (FEW) kern = masked ? attn_dq_few_kernel<T, DP, true> : attn_dq_few_kernel<T, DP, false>;
+  else kern = masked ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>;
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
   p->tiles = FEW ? 1 : ceil_div(p->R, 128);

@@ -58,7 +58,7 @@ struct AttnRow {
 // vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
 // tiles; K runs one tile ahead of V.
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : 2)) void attn_fwd_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : 3)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
