@@ -49,7 +49,7 @@ struct AttnDev {
   int causal, off;                // key j is open to token i when j <= i + off, off = Lk - Lq
   float scale, scale_log2;
   int tiles;                      // workgroup tiles of one problem
-  int whole, rest, parts, rest_x; // how the tiles are dealt out, see attn_deal
+  int whole, rest, parts, rest_x; // how the tiles are dealt out, see attn_work
   float* part;                    // partial results: [rest][parts][rows of a tile][D] (dk and dv: one after the other)
   float* part_ml;                 // [rest][parts][rows of a tile][2]: maxima and sums of the forward pass
   float *row_lse2, *minus_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and -rowsum(dout * out)

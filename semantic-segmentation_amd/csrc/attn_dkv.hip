@@ -150,6 +150,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 #pragma unroll
     for (int rb = 0; rb < QT / 32; ++rb) {
       const int row0 = t * QT + rb * 32;
+      if (rb > 0 && row0 >= p.R) return;
       unsigned char open[16];
       if (MASKED && mkey) {
 #pragma unroll

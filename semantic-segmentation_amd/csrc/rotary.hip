@@ -8,7 +8,7 @@
 namespace segk {
 
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_UNROLL = 4;        // heads in flight per group of lanes
+constexpr int ROT_UNROLL = 4;        // heads in flight per group of lanes (and as many asked for)
 constexpr int ROT_MAX_BLOCKS = 2048; // of the backward pass: rows of weight-gradient partials
 
 struct RotSide {   // queries or keys
@@ -38,23 +38,29 @@ struct RotDev {
   int blocks;
 };
 
+// 4 channels as they lie in memory
 template <typename T>
-__device__ __forceinline__ void rot_load4(const char* p, float* v);
+struct RotRaw;
 template <>
-__device__ __forceinline__ void rot_load4<bf16_t>(const char* p, float* v) {
-  const u32x2 a = *reinterpret_cast<const u32x2*>(p);
+struct RotRaw<bf16_t> {
+  u32x2 v;
+  __device__ __forceinline__ void to(float* x) const {
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    v[2 * e] = __uint_as_float(a[e] << 16);
-    v[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u);
+    for (int e = 0; e < 2; ++e) {
+      x[2 * e] = __uint_as_float(v[e] << 16);
+      x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+    }
   }
-}
+};
 template <>
-__device__ __forceinline__ void rot_load4<float>(const char* p, float* v) {
-  const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+struct RotRaw<float> {
+  f32x4 v;
+  __device__ __forceinline__ void to(float* x) const {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = a[e];
-}
+    for (int e = 0; e < 4; ++e) x[e] = v[e];
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void rot_store4(char* p, const float* v);
 template <>
@@ -79,6 +85,7 @@ struct RotLane {
     const bool turned = 4 * j < p.pairs;
     lo = INTER ? 8 * j : turned ? 4 * j : p.pairs + 4 * j;
     hi = INTER ? 8 * j + 4 : turned ? p.pairs + 4 * j : p.D / 2 + 4 * j;
+    if (!live) lo = hi = 0;      // (never stored)
 #pragma unroll
     for (int e = 0; e < 4; ++e) c[e] = 1.f, s[e] = 0.f;
   }
@@ -115,9 +122,9 @@ struct RotLane {
     }
   }
   template <typename T>
-  __device__ __forceinline__ void load(const char* row, float* v) const {
-    rot_load4<T>(row + lo * (int)sizeof(T), v);
-    rot_load4<T>(row + hi * (int)sizeof(T), v + 4);
+  __device__ __forceinline__ void load_raw(const char* row, RotRaw<T>* x) const {
+    x[0].v = *reinterpret_cast<const decltype(x[0].v)*>(row + lo * (int)sizeof(T));
+    x[1].v = *reinterpret_cast<const decltype(x[0].v)*>(row + hi * (int)sizeof(T));
   }
   template <typename T>
   __device__ __forceinline__ void store(char* row, const float* v) const {
@@ -177,17 +184,30 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_kernel(const RotDe
     for (int e = 0; e < 8; ++e) w[e] = t.live && sd.w ? sd.w[t.channel(e)] : 1.f;
     const char* src = sd.x + n * sd.xn + l * sd.xl;
     char* dst = sd.y + (long long)nl * sd.heads * p.D * (int)sizeof(T);
+    // the next heads are asked for before these are worked on (lanes past D re-read channel 0 and count for nothing)
+    RotRaw<T> raw[ROT_UNROLL][2];
+    auto ask = [&](int hb) {
+#pragma unroll
+      for (int u = 0; u < ROT_UNROLL; ++u) t.template load_raw<T>(src + min(hb + u, b - 1) * sd.xh, raw[u]);
+    };
+    ask(a);
     for (int hb = a; hb < b; hb += ROT_UNROLL) {
-      float v[ROT_UNROLL][8];
+      RotRaw<T> now[ROT_UNROLL][2];
 #pragma unroll
-      for (int u = 0; u < ROT_UNROLL; ++u) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-        if (hb + u < b && t.live) t.template load<T>(src + (hb + u) * sd.xh, v[u]);
-      }
+      for (int u = 0; u < ROT_UNROLL; ++u) now[u][0] = raw[u][0], now[u][1] = raw[u][1];
+      if (hb + ROT_UNROLL < b) ask(hb + ROT_UNROLL);
 #pragma unroll
       for (int u = 0; u < ROT_UNROLL; ++u)
-        if (hb + u < b) rot_head<T, LPH, INTER>(p, t, w, v[u], dst + (long long)(hb + u) * p.D * (int)sizeof(T));
+        if (hb + u < b) {
+          float v[8];
+          now[u][0].to(v);
+          now[u][1].to(v + 4);
+          if (!t.live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          }
+          rot_head<T, LPH, INTER>(p, t, w, v, dst + (long long)(hb + u) * p.D * (int)sizeof(T));
+        }
     }
   }
 }
@@ -223,17 +243,33 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
       const char* src = sd.x + n * sd.xn + l * sd.xl;
       const char* dys = sd.dy + n * sd.dn + l * sd.dl;
       char* dst = sd.y + (long long)nl * sd.heads * p.D * (int)sizeof(T);
+      // (two heads in flight, two asked for, as in the forward kernel)
+      RotRaw<T> raw[2][4];
+      auto ask = [&](int hb) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int hh = min(hb + u, b - 1);
+          t.template load_raw<T>(dys + hh * sd.dh, raw[u]);
+          if (p.norm) t.template load_raw<T>(src + hh * sd.xh, raw[u] + 2);
+        }
+      };
+      ask(a);
       for (int hb = a; hb < b; hb += 2) {
         float v[2][8], g[2][8];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          raw[u][0].to(g[u]);
+          raw[u][1].to(g[u] + 4);
+          if (p.norm) {
+            raw[u][2].to(v[u]);
+            raw[u][3].to(v[u] + 4);
+          }
+          if (!t.live) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] = 0.f;
-          if (hb + u < b && t.live) {
-            t.template load<T>(dys + (hb + u) * sd.dh, g[u]);
-            if (p.norm) t.template load<T>(src + (hb + u) * sd.xh, v[u]);
+            for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] = 0.f;
           }
         }
+        if (hb + 2 < b) ask(hb + 2);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           if (hb + u >= b) break;
