@@ -1317,18 +1317,13 @@ class CAMFunction(torch.autograd.Function):
 
 
 # ------------------------------------------------------ multi-head attention ----
-def _attention_operand(t):
-    """The tensor itself where the kernels can read it, else a contiguous copy."""
-    return t if ops.attention_operand_ok(t) else t.clone(memory_format=torch.contiguous_format)
-
-
 class AttentionFunction(torch.autograd.Function):
     """Multi-head attention with fused softmax; the backward pass computes the probabilities again from lse."""
 
     @staticmethod
     def forward(ctx, q, k, v, mask, key_mask, causal, scale):
-        q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q, k, v = ops.attention_operand(q), ops.attention_operand(k), ops.attention_operand(v)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=True)
         ctx.save_for_backward(q, k, v, out, lse, mask, key_mask)
         ctx.how = (causal, scale)
@@ -1340,7 +1335,7 @@ class AttentionFunction(torch.autograd.Function):
         q, k, v, out, lse, mask, key_mask = ctx.saved_tensors
         causal, scale = ctx.how
         need = ctx.needs_input_grad
-        dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, _attention_operand(g), scale, causal, mask, key_mask,
+        dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, ops.attention_operand(g), scale, causal, mask, key_mask,
                                        need_dq=need[0], need_dkv=need[1] or need[2])
         return dq, (dk if need[1] else None), (dv if need[2] else None), None, None, None, None
 
@@ -1364,8 +1359,8 @@ def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
     scale = float(q.shape[3]) ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return AttentionFunction.apply(q, k, v, mask, key_mask, bool(causal), scale)
-    q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q, k, v = ops.attention_operand(q), ops.attention_operand(k), ops.attention_operand(v)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask)
     return out
 
@@ -1373,7 +1368,7 @@ def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
 class QkNormRotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved):
-        q, k = _attention_operand(q), (None if k is None else _attention_operand(k))
+        q, k = ops.attention_operand(q), (None if k is None else ops.attention_operand(k))
         wq, wk = _fp32_weight(q_weight), _fp32_weight(k_weight)
         res = ops.qk_norm_rotary_fwd(q, k, wq, wk, positions, inv_freq, sections, eps, interleaved)
         ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
@@ -1386,16 +1381,18 @@ class QkNormRotaryFunction(torch.autograd.Function):
     def backward(ctx, gq, gk=None):
         q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
         need = ctx.needs_input_grad
-        gq = _attention_operand(gq)
-        gk = None if k is None else _attention_operand(gk)
+        gq = ops.attention_operand(gq)
+        gk = None if k is None else ops.attention_operand(gk)
         dq, dk, dwq, dwk = ops.qk_norm_rotary_bwd(gq, gk, q, k, wq, wk, positions, inv_freq, *ctx.how,
                                                   need_weights=need[2:4])
-        dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.weight_dtypes))
+        dwq, dwk = (g if g is None or g.dtype is dt else g.to(dt) for g, dt in zip((dwq, dwk), ctx.weight_dtypes))
         return (dq if need[0] else None), (dk if need[1] else None), dwq, dwk, None, None, None, None, None
 
 
 def _fp32_weight(w):
-    return None if w is None else w.detach().float().contiguous()
+    if w is None or (w.dtype is torch.float32 and w.is_contiguous()):
+        return w
+    return w.detach().float().contiguous()
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, interleaved=False):
@@ -1412,8 +1409,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None,
       sections     how many of the pairs, in order, turn by each axis; default: equal shares
       interleaved  pairs are channels (2c, 2c + 1) instead of (c, c + pairs); channels past the pairs stay as normalised
     Angles are formed in 64 bits.  Differentiable once with respect to q, k and the weights."""
-    args = (positions, inv_freq, None if sections is None else tuple(int(z) for z in sections),
-            None if eps is None else float(eps), bool(interleaved))
+    args = (positions, inv_freq, None if sections is None else tuple(map(int, sections)), eps, interleaved)
     tensors = (q, k, q_weight, k_weight)
     if positions.requires_grad or inv_freq.requires_grad:
         raise ValueError("positions and inv_freq get no gradient here")
@@ -1422,6 +1418,6 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None,
             raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return QkNormRotaryFunction.apply(*tensors, *args)
-    res = ops.qk_norm_rotary_fwd(_attention_operand(q), None if k is None else _attention_operand(k),
+    res = ops.qk_norm_rotary_fwd(ops.attention_operand(q), None if k is None else ops.attention_operand(k),
                                  _fp32_weight(q_weight), _fp32_weight(k_weight), *args)
     return res if k is not None else res[0]

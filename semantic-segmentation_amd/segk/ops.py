@@ -876,70 +876,92 @@ def _launch_packed(name, args, t):
             call(name, args, _stream())
 
 
+def _like(t):
+    """A contiguous tensor of t's shape, type and device, unset."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _with_workspace(args, need, t):
     """(packed arguments with `need` bytes of workspace, the tensor that owns them)."""
     ws = torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
     return args + WORKSPACE_ARGS.pack(ws.data_ptr() if need else 0, need), ws
 
 
-def attention_operand_ok(t):
-    """Whether a [N, L, heads, D] tensor can be read where it lies: unit stride over D, 16-byte aligned rows."""
+def _attention_view(t, z=None):
+    """(pointer, strides over images, tokens, heads) of a [N, L, heads, D] tensor (of shape z) that can be read where it lies
+    - unit stride over D, 16-byte aligned rows - or None.  Strides of dimensions of one element are 0."""
     n, l, h, d = t.stride()
-    per = 4 if t.dtype == torch.float32 else 8
-    if d != 1 or t.data_ptr() % 16 != 0:
-        return False
-    if n % per == 0 and l % per == 0 and h % per == 0:
-        return True
-    z = t.shape
-    return (n % per == 0 or z[0] == 1) and (l % per == 0 or z[1] == 1) and (h % per == 0 or z[2] == 1)
+    p = t.data_ptr()
+    zn, zl, zh, _ = t.shape if z is None else z
+    if zn == 1:
+        n = 0
+    if zl == 1:
+        l = 0
+    if zh == 1:
+        h = 0
+    if d != 1 or p & 15 or (n | l | h) & (3 if t.dtype is torch.float32 else 7):
+        return None
+    return p, n, l, h
 
 
-def _attention_view(t, name):
-    if not attention_operand_ok(t):
+def attention_operand(t):
+    """The tensor itself where the attention kernels can read it, else a contiguous copy."""
+    return t if _attention_view(t) is not None else t.clone(memory_format=torch.contiguous_format)
+
+
+def _need_view(t, name, z=None):
+    view = _attention_view(t, z)
+    if view is None:
         raise ValueError("%s needs unit stride over its channels and 16-byte aligned rows, got strides %s" % (name, t.stride()))
-    (n, l, h, _), z = t.stride(), t.shape
-    return t.data_ptr(), (n if z[0] > 1 else 0), (l if z[1] > 1 else 0), (h if z[2] > 1 else 0)
+    return view
 
 
 _NO_VIEW = (0, 0, 0, 0)
 
 
+def _same_kind(index, dtype, t, name):
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError("operands share one dtype and device (%s on cuda:%d, %s: %s on %s)" % (dtype, index, name, t.dtype, t.device))
+
+
+def _bool_mask(index, t, name):
+    if t.dtype is not torch.bool or t.get_device() != index:
+        raise ValueError("%s must be a bool tensor on cuda:%d, got %s on %s" % (name, index, t.dtype, t.device))
+
+
 def _attention_args(q, k, v, out, scale, causal, mask, key_mask):
-    """Checked arguments as far as key_mask_k: (tuple of fields, shape, lse and gradients to follow)."""
-    _dev(q, k, v, out, mask, key_mask)
-    dtype, device = q.dtype, q.device
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        if t.dim() != 4:
-            raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
-        if t.dtype != dtype or t.device != device:
-            raise ValueError("attention operands share one dtype and device (q: %s on %s, %s: %s on %s)"
-                             % (dtype, device, name, t.dtype, t.device))
-    N, Lq, Hq, D = q.shape
-    kn, Lk, Hk, kd = k.shape
-    if k.shape != v.shape or kn != N or kd != D or out.shape != q.shape:
+    """Checked arguments: the fields up to the view of out, and those of the masks (lse comes between them)."""
+    index, dtype = q.get_device(), q.dtype
+    if index < 0:
+        _dev(q)
+    _same_kind(index, dtype, k, "k")
+    _same_kind(index, dtype, v, "v")
+    _same_kind(index, dtype, out, "out")
+    zq, zk = q.shape, k.shape
+    if len(zq) != 4 or len(zk) != 4:
+        raise ValueError("attention operands must be [N, L, heads, D], got q %s k %s" % (tuple(zq), tuple(zk)))
+    N, Lq, Hq, D = zq
+    kn, Lk, Hk, kd = zk
+    if zk != v.shape or kn != N or kd != D or out.shape != zq:
         raise ValueError("attention shapes disagree: q %s k %s v %s out %s"
-                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape), tuple(out.shape)))
+                         % (tuple(zq), tuple(zk), tuple(v.shape), tuple(out.shape)))
     if Hk == 0 or Hq % Hk != 0:
         raise ValueError("%d query heads cannot share %d key / value heads evenly" % (Hq, Hk))
-    dt = _dt(q)
     m, km = (0, 0, 0, 0, 0), (0, 0, 0)
     if mask is not None:
-        if mask.dtype != torch.bool or mask.device != device:
-            raise ValueError("mask must be a bool tensor on %s, got %s on %s" % (device, mask.dtype, mask.device))
-        if mask.dim() != 4 or any(z != f and z != 1 for z, f in zip(mask.shape, (N, Hq, Lq, Lk))):
-            raise ValueError("mask of shape %s does not broadcast to [N, heads, Lq, Lk] = %s"
-                             % (tuple(mask.shape), (N, Hq, Lq, Lk)))
-        m = (mask.data_ptr(),) + tuple(0 if z == 1 else s for s, z in zip(mask.stride(), mask.shape))
+        _bool_mask(index, mask, "mask")
+        z = mask.shape
+        if len(z) != 4 or any(a != f and a != 1 for a, f in zip(z, (N, Hq, Lq, Lk))):
+            raise ValueError("mask of shape %s does not broadcast to [N, heads, Lq, Lk] = %s" % (tuple(z), (N, Hq, Lq, Lk)))
+        m = (mask.data_ptr(),) + tuple(0 if a == 1 else s for s, a in zip(mask.stride(), z))
     if key_mask is not None:
-        if key_mask.dtype != torch.bool or key_mask.device != device:
-            raise ValueError("key_mask must be a bool tensor on %s, got %s on %s" % (device, key_mask.dtype, key_mask.device))
+        _bool_mask(index, key_mask, "key_mask")
         if tuple(key_mask.shape) != (N, Lk):
             raise ValueError("key_mask of shape %s, expected [N, Lk] = %s" % (tuple(key_mask.shape), (N, Lk)))
         km = (key_mask.data_ptr(),) + key_mask.stride()
-    views = _attention_view(q, "q")
-    views += _attention_view(k, "k") + _attention_view(v, "v") if Lk > 0 else _NO_VIEW + _NO_VIEW
-    views += _attention_view(out, "out")
-    return (N, Lq, Lk, Hq, Hk, D, dt, 1 if causal else 0, ctypes.c_float(scale).value) + views, m + km
+    head = (N, Lq, Lk, Hq, Hk, D, _dt(q), 1 if causal else 0, ctypes.c_float(scale).value) + _need_view(q, "q", zq)
+    head += _need_view(k, "k", zk) + _need_view(v, "v", zk) if Lk > 0 else _NO_VIEW + _NO_VIEW
+    return head + _need_view(out, "out", zq), m + km
 
 
 def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, want_lse=False):
@@ -962,18 +984,20 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_m
     """Gradients (dq, dk, dv) of attention_fwd, contiguous, of the operands' dtype; None where not wanted."""
     head, masks = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
     N, Lq, Lk, Hq = head[:4]
-    if dout.shape != out.shape or dout.dtype != out.dtype or dout.device != out.device:
-        raise ValueError("dout %s %s does not match out %s %s" % (tuple(dout.shape), dout.dtype, tuple(out.shape), out.dtype))
-    if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (N, Hq, Lq) or lse.device != q.device:
+    index = q.get_device()
+    _same_kind(index, q.dtype, dout, "dout")
+    if dout.shape != out.shape:
+        raise ValueError("dout %s does not match out %s" % (tuple(dout.shape), tuple(out.shape)))
+    if lse.dtype is not torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (N, Hq, Lq) or lse.get_device() != index:
         raise ValueError("lse must be contiguous float32 [N, Hq, Lq]")
     some = N > 0 and Lq > 0 and Lk > 0
-    new = torch.empty if some else torch.zeros
-    dq = new(q.shape, dtype=q.dtype, device=q.device) if need_dq else None
-    dk = new(k.shape, dtype=q.dtype, device=q.device) if need_dkv else None
-    dv = new(k.shape, dtype=q.dtype, device=q.device) if need_dkv else None
+    new = _like if some else torch.zeros_like
+    dq = new(q) if need_dq else None
+    dk = new(k) if need_dkv else None
+    dv = new(k) if need_dkv else None
     if not some or not (need_dq or need_dkv):
         return dq, dk, dv
-    args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), *masks, *_attention_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
+    args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), *masks, *_need_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
                                dk.data_ptr() if need_dkv else 0, dv.data_ptr() if need_dkv else 0)
     args, ws = _with_workspace(args, call("segk_attention_workspace", args + bytes(16), 1), q)
     _launch_packed("segk_attention_bwd", args, q)
@@ -985,30 +1009,37 @@ _POS_DTYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 def _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved):
     """Checked arguments: (N .. dtype and the views of q and k, the weights, positions .. eps)."""
-    _dev(q, k, q_weight, k_weight, positions, inv_freq)
-    device = q.device
-    if q.dim() != 4:
-        raise ValueError("q must be [N, L, heads, D], got shape %s" % (tuple(q.shape),))
-    N, L, Hq, D = q.shape
-    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.device != device or k.shape[:2] != q.shape[:2]
-                          or k.shape[3] != D):
-        raise ValueError("queries %s %s and keys %s %s share images, tokens, head size, dtype and device"
-                         % (tuple(q.shape), q.dtype, tuple(k.shape), k.dtype))
+    index, dtype, zq = q.get_device(), q.dtype, q.shape
+    if index < 0:
+        _dev(q)
+    if len(zq) != 4:
+        raise ValueError("q must be [N, L, heads, D], got shape %s" % (tuple(zq),))
+    N, L, Hq, D = zq
+    Hk, view_k = 0, _NO_VIEW
+    if k is not None:
+        _same_kind(index, dtype, k, "k")
+        zk = k.shape
+        if len(zk) != 4 or zk[0] != N or zk[1] != L or zk[3] != D:
+            raise ValueError("queries %s and keys %s share images, tokens and head size" % (tuple(zq), tuple(zk)))
+        Hk, view_k = zk[2], _need_view(k, "k", zk)
     for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != D or not t.is_contiguous()
-                              or t.device != device):
-            raise ValueError("%s must be contiguous float32 [%d] on %s, got %s %s" % (name, D, device, tuple(t.shape), t.dtype))
-    if eps is None and (q_weight is not None or k_weight is not None):
-        raise ValueError("weights belong to the norm: none without eps")
-    axes = positions.shape[-1] if positions.dim() in (2, 3) else 0
-    if not 1 <= axes <= 4 or tuple(positions.shape[:-1]) not in ((L,), (N, L)):
-        raise ValueError("positions must be [L, axes] or [N, L, axes] with 1 to 4 axes, got %s for N=%d L=%d"
-                         % (tuple(positions.shape), N, L))
-    if positions.dtype not in _POS_DTYPES or positions.device != device:
-        raise ValueError("positions must be int32, int64 or float32 on %s, got %s on %s"
-                         % (device, positions.dtype, positions.device))
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != device:
-        raise ValueError("inv_freq must be contiguous float32 of one dimension on %s" % (device,))
+        if t is not None:
+            _same_kind(index, torch.float32, t, name)
+            if t.dim() != 1 or t.shape[0] != D or not t.is_contiguous():
+                raise ValueError("%s must be contiguous [%d], got %s" % (name, D, tuple(t.shape)))
+            if eps is None:
+                raise ValueError("weights belong to the norm: none without eps")
+    zp = positions.shape
+    axes = zp[-1] if len(zp) in (2, 3) else 0
+    if not 1 <= axes <= 4 or zp[-2] != L or (len(zp) == 3 and zp[0] != N):
+        raise ValueError("positions must be [L, axes] or [N, L, axes] with 1 to 4 axes, got %s for N=%d L=%d" % (tuple(zp), N, L))
+    pos_dtype = _POS_DTYPES.get(positions.dtype)
+    if pos_dtype is None or positions.get_device() != index:
+        raise ValueError("positions must be int32, int64 or float32 on cuda:%d, got %s on %s"
+                         % (index, positions.dtype, positions.device))
+    _same_kind(index, torch.float32, inv_freq, "inv_freq")
+    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be contiguous and of one dimension")
     pairs = inv_freq.shape[0]
     if sections is None:
         if pairs % axes != 0:
@@ -1017,11 +1048,9 @@ def _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, i
     if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
         raise ValueError("sections %s: %d axes share %d pairs" % (tuple(sections), axes, pairs))
     s = positions.stride()
-    head = (N, L, Hq, 0 if k is None else k.shape[2], D, _dt(q)) + _attention_view(q, "q") \
-        + (_NO_VIEW if k is None else _attention_view(k, "k"))
-    weights = (q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0)
-    rest = (positions.data_ptr(), _POS_DTYPES[positions.dtype], s[0] if len(s) == 3 else 0, s[-2], s[-1], axes) \
-        + tuple(sections) + (0,) * (4 - axes) \
+    head = (N, L, Hq, Hk, D, _dt(q)) + _need_view(q, "q", zq) + view_k
+    weights = (0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr())
+    rest = (positions.data_ptr(), pos_dtype, s[0] if len(s) == 3 else 0, s[-2], s[-1], axes, *sections) + (0,) * (4 - axes) \
         + (inv_freq.data_ptr(), 0 if eps is None else 1, 1 if interleaved else 0, 0.0 if eps is None else ctypes.c_float(eps).value)
     return head, weights, rest
 
@@ -1031,8 +1060,8 @@ def qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, sections=N
     (q', k').  Operands as attention_fwd, D up to 256; eps None: rotation only.  segk.functional.qk_norm_rotary has the
     formula."""
     head, weights, rest = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k is not None else None
+    q_out = _like(q)
+    k_out = None if k is None else _like(k)
     if q.shape[0] > 0 and q.shape[1] > 0:
         args = QK_NORM_ROTARY_ARGS.pack(*head, q_out.data_ptr(), 0 if k is None else k_out.data_ptr(), *weights, *rest,
                                         *_NO_VIEW, *_NO_VIEW, 0, 0)
@@ -1045,10 +1074,12 @@ def qk_norm_rotary_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_
     """Gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rotary_fwd; weight gradients (float32) where wanted."""
     head, weights, rest = _rotary_args(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, interleaved)
     for g, t in ((dq_out, q), (dk_out, k)):
-        if t is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
-            raise ValueError("gradient %s %s does not match %s %s" % (tuple(g.shape), g.dtype, tuple(t.shape), t.dtype))
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k is not None else None
+        if t is not None:
+            _same_kind(q.get_device(), q.dtype, g, "a gradient")
+            if g.shape != t.shape:
+                raise ValueError("gradient %s does not match %s" % (tuple(g.shape), tuple(t.shape)))
+    dq = _like(q)
+    dk = None if k is None else _like(k)
     some = q.shape[0] > 0 and q.shape[1] > 0
     new = torch.empty if some else torch.zeros
     dqw = new(q.shape[3], dtype=torch.float32, device=q.device) if need_weights[0] and q_weight is not None else None
@@ -1056,7 +1087,7 @@ def qk_norm_rotary_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_
     if not some:
         return dq, dk, dqw, dkw
     args = QK_NORM_ROTARY_ARGS.pack(*head, dq.data_ptr(), 0 if k is None else dk.data_ptr(), *weights, *rest,
-                                    *_attention_view(dq_out, "dq"), *(_NO_VIEW if k is None else _attention_view(dk_out, "dk")),
+                                    *_need_view(dq_out, "dq"), *(_NO_VIEW if k is None else _need_view(dk_out, "dk")),
                                     0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr())
     need = call("segk_qk_norm_rotary_bwd_workspace", args + bytes(16))
     args, ws = _with_workspace(args, need, q)
