@@ -50,6 +50,8 @@ struct AttnDev {
   float scale, scale_log2;
   int tiles;                      // workgroup tiles of one problem
   int whole, rest, parts, rest_x; // how the tiles are dealt out, see attn_work
+  int even_steps, even_units;     // tiles of different lengths: steps of a part, parts of one problem (0: equal lengths)
+  int loop_rows;                  // what a tile's loop runs over: 0 keys by 64, else packed rows by this many
   float* part;                    // partial results: [rest][parts][rows of a tile][D] (dk and dv: one after the other)
   float* part_ml;                 // [rest][parts][rows of a tile][2]: maxima and sums of the forward pass
   float *row_lse2, *minus_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and -rowsum(dout * out)
@@ -75,6 +77,21 @@ __device__ __forceinline__ void attn_decode_tile(const AttnDev& p, int g, AttnWo
   w->hk = g % p.Hk;
   w->n = g / p.Hk;
 }
+// Steps of a tile's loop under the diagonal.
+__host__ __device__ inline int attn_causal_steps(const AttnDev& p, int tile) {
+  if (p.loop_rows) {           // keys tile * 128 .. : rows from the first token that may use one of them
+    const int all = (p.R + p.loop_rows - 1) / p.loop_rows, tok = tile * 128 - p.off;
+    return tok >= p.Lq ? 0 : all - (tok > 0 ? tok : 0) * p.G / p.loop_rows;
+  }
+  const int last = (tile * 128 + 128 < p.R ? tile * 128 + 128 : p.R) - 1;
+  const int end = last / p.G + p.off + 1;
+  return ((end < p.Lk ? (end > 0 ? end : 0) : p.Lk) + 63) / 64;
+}
+__host__ __device__ inline int attn_tile_parts(const AttnDev& p, int tile) {
+  if (!p.even_steps) return p.parts;
+  const int s = attn_causal_steps(p, tile);
+  return s > p.even_steps ? (s + p.even_steps - 1) / p.even_steps : 1;
+}
 __device__ __forceinline__ AttnWork attn_work(const AttnDev& p) {
   AttnWork w = {-1, 0, 0, 0, 1, 0};
   const int x = (int)blockIdx.x & 7, i = (int)blockIdx.x >> 3, whole_x = p.whole >> 3;
@@ -82,7 +99,22 @@ __device__ __forceinline__ AttnWork attn_work(const AttnDev& p) {
     if (x * whole_x + i < p.tiles * p.N * p.Hk) attn_decode_tile(p, x * whole_x + i, &w);
     return w;
   }
-  const int u = x * p.rest_x + i - whole_x;
+  int u = x * p.rest_x + i - whole_x;
+  if (p.even_steps) {          // few tiles of different lengths: every part has about as many steps
+    const int head = u / p.even_units;
+    if (head >= p.N * p.Hk) return w;
+    u -= head * p.even_units;
+    for (int t = 0; t < p.tiles; ++t) {
+      attn_decode_tile(p, head * p.tiles + t, &w);
+      w.parts = attn_tile_parts(p, w.tile);
+      w.slot = head * p.tiles + t;
+      w.part = u;
+      if (u < w.parts) return w;
+      u -= w.parts;
+    }
+    w.n = -1;
+    return w;
+  }
   if (u >= p.rest * p.parts) return w;
   w.part = u / p.rest;
   w.parts = p.parts;

@@ -260,10 +260,10 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dkv_sum_kernel(const AttnDe
   const bool is_v = (line & 128) != 0;
   AttnWork w;
   attn_decode_tile(p, p.whole + slot, &w);
-  const int key = w.tile * 128 + row;
-  if (key >= p.Lk) return;
+  const int key = w.tile * 128 + row, parts = attn_tile_parts(p, w.tile);
+  if (key >= p.Lk || parts == 1) return;     // (a tile in one part is finished)
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.parts; ++s) {
+  for (int s = 0; s < parts; ++s) {
     const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * 256 + (line & 255)) * p.D + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += y[e];
@@ -283,6 +283,7 @@ static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
   p->tiles = ceil_div(p->Lk, 128);
+  p->loop_rows = QT;
   SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention_bwd: too many workgroups");
   const long long grid = attn_deal(p, per_cu, ceil_div(p->R, QT), 2);
   if (plan_only) return SEGK_OK;

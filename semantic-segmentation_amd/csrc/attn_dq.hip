@@ -286,10 +286,10 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev
   const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
   AttnWork w;
   attn_decode_tile(p, p.whole + slot, &w);
-  const int rr = w.tile * tile_rows + row;
-  if (rr >= p.R) return;
+  const int rr = w.tile * tile_rows + row, parts = attn_tile_parts(p, w.tile);
+  if (rr >= p.R || parts == 1) return;       // (a tile in one part is finished)
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.parts; ++s) {
+  for (int s = 0; s < parts; ++s) {
     const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * tile_rows + row) * p.D + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += y[e];
@@ -310,6 +310,7 @@ static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
   p->tiles = FEW ? 1 : ceil_div(p->R, 128);
+  p->loop_rows = 0;
   SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention_bwd: too many workgroups");
   const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, FEW ? 128 : 64), FEW ? 1 : 2);
   if (plan_only) return SEGK_OK;

@@ -398,19 +398,25 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   const int c = threadIdx.x % lanes, g = threadIdx.x / lanes % groups, in = threadIdx.x / (lanes * groups);
   const long long line = (long long)blockIdx.x * (ATTN_THREADS / (lanes * groups)) + in;
   const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
-  const bool ok = slot < p.rest;
+  AttnWork w = {0, 0, 0, 0, 1, 0};
+  int parts = 0;
+  if (slot < p.rest) {
+    attn_decode_tile(p, p.whole + slot, &w);
+    parts = attn_tile_parts(p, w.tile);
+  }
+  const bool ok = parts > 1;       // (a tile in one part is finished)
   const long long first = ok ? (long long)slot * p.parts * tile_rows + row : 0;
   // every group looks at its own parts' maxima first, so that the sums are scaled once
   float m = -INFINITY, l = 0.f;
   if (ok)
-    for (int s = g; s < p.parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * tile_rows)]);
+    for (int s = g; s < parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * tile_rows)]);
   sm[threadIdx.x] = m;
   __syncthreads();
   for (int i = 0; i < groups; ++i) m = fmaxf(m, sm[(in * groups + i) * lanes + c]);
   const float ms = m == -INFINITY ? 0.f : m;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (ok)
-    for (int s = g; s < p.parts; s += groups) {
+    for (int s = g; s < parts; s += groups) {
       const long long at = first + (long long)s * tile_rows;
       const float a = exp2_fast(p.part_ml[2 * at] - ms);
       l = fmaf(p.part_ml[2 * at + 1], a, l);
@@ -424,8 +430,6 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   sl[threadIdx.x] = l;
   __syncthreads();
   if (!ok || g != 0 || c * 4 >= p.D) return;
-  AttnWork w;
-  attn_decode_tile(p, p.whole + slot, &w);
   const int rr = w.tile * tile_rows + row;
   if (rr >= p.R) return;
   for (int i = 1; i < groups; ++i) {
@@ -500,6 +504,24 @@ bool attn_few(const AttnDev& p, int dtype) {
 long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps) {
   const long long all = (long long)p->tiles * p->N * p->Hk;
   const long long round = 256LL * per_cu;      // workgroups that run at once
+  p->even_steps = p->even_units = 0;
+  if (p->causal && p->tiles > 1 && all < round && p->tiles <= 64) {
+    // Few tiles of different lengths: parts of equal length, a round of them.
+    long long sum = 0;
+    for (int t = 0; t < p->tiles; ++t) sum += attn_causal_steps(*p, t);
+    long long per = (sum * p->N * p->Hk + round - 1) / round;
+    p->even_steps = (int)(per < min_steps ? min_steps : per);
+    int most = 1, units = 0;
+    for (int t = 0; t < p->tiles; ++t) {
+      const int n = attn_tile_parts(*p, t);
+      units += n;
+      if (n > most) most = n;
+    }
+    p->even_units = units;
+    p->whole = 0, p->rest = (int)all, p->parts = most;
+    p->rest_x = (int)(((long long)units * p->N * p->Hk + 7) / 8);
+    return 8LL * p->rest_x;
+  }
   // Under the diagonal tiles differ in length and even out by themselves once there are enough of them.
   long long whole = p->causal && all >= round ? all / 8 * 8 : all / round * round;
   // A last round that is not full is worth cutting up (and joining) only where a round is long: 18 steps of 64 keys gained
@@ -589,6 +611,7 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   p->scale = a->scale;
   p->scale_log2 = a->scale * LOG2E;
   p->tiles = p->whole = p->rest = p->parts = p->rest_x = 0;
+  p->even_steps = p->even_units = p->loop_rows = 0;
   p->part = p->part_ml = nullptr;
   p->dq = p->dk = p->dv = nullptr;
   p->row_lse2 = p->minus_delta = nullptr;
@@ -710,7 +733,7 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
   if (rc != SEGK_OK || p.parts == 1) return rc;
   const int lanes = p.D <= 8 ? 2 : p.D <= 16 ? 4 : p.D <= 32 ? 8 : p.D <= 64 ? 16 : 32;
   int groups = 1;
-  while (groups < p.parts && groups * lanes < ATTN_THREADS) groups *= 2;
+  while (groups * 4 < p.parts && groups * lanes < ATTN_THREADS) groups *= 2;     // about four parts a thread
   const int lines = ATTN_THREADS / (lanes * groups);
   const unsigned grid = (unsigned)ceil_div((long long)p.rest * tile_rows, lines);   // (rest is less than a round of workgroups)
   SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes, groups, tile_rows)));
