@@ -18,13 +18,15 @@ constexpr int dkv_rows() { return dkv_v_in_lds<T, DP>() ? 32 : 64; }
 // are staged through LDS and read both along rows and along columns.
 // V stays in registers too where the heads are small; where they are not (VL) it lies in LDS: 32 registers less bring two
 // wavefronts to a SIMD, which cover each other's exponentials, for a quarter more LDS reads.
-template <typename T, int DP, bool MASKED>
+// MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
+template <typename T, int DP, int MASKS>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnRead<T, DP> Rd;
   typedef AttnPiece<T, DP> Piece;
   constexpr bool VL = dkv_v_in_lds<T, DP>();
   constexpr int QT = dkv_rows<T, DP>();
+  constexpr bool MASKED = MASKS != 0, PAIRS = MASKS == 2;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = QT * Tile::PITCH;
   constexpr int STAGE_B = 2 * TILE_B + 512;      // Q tile, dO tile, lse, delta
@@ -49,22 +51,6 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   if (MASKED && p.kmask && key_ok) key_ok = p.kmask[n * p.km_n + (long long)key * p.km_k] != 0;
   // (a tile without an open key has nothing to walk over: its gradients are zeros)
   if (MASKED && p.kmask && !any_open_key(p.kmask + n * p.km_n, p.km_k, key_wg, p.Lk, lane)) t1 = t0;
-  AttnFrag<T> kf[KS], vf[VL ? 1 : KS];
-  {
-    const long long kk = key_ok ? key : 0;
-    const char* ks_ = p.k.p + ((long long)n * p.k.n + kk * p.k.l + (long long)hk * p.k.h) * (int)sizeof(T);
-    const char* vs_ = p.v.p + ((long long)n * p.v.n + kk * p.v.l + (long long)hk * p.v.h) * (int)sizeof(T);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kf[ks] = load_frag<T>(ks_, ks, h, p.D, key_ok);
-      if (!VL) vf[ks] = load_frag<T>(vs_, ks, h, p.D, key_ok);
-    }
-    if (VL) {     // this wavefront's 32 rows of V, through registers, in the tiles' permutation
-      char* const vt = smem + 2 * STAGE_B;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) Rd::write_rows(vt, wave * 32, ks, lane, load_frag<T>(vs_, ks, h, p.D, key_ok));
-    }
-  }
 
   const AttnLane<T, DP> ln(smem, lane);
   const AttnLane<T, DP> lv(smem + wave * 32 * Tile::PITCH, lane);     // (VL: this wavefront's rows of V)
@@ -75,7 +61,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   const float* const lse2 = p.row_lse2 + ((long long)n * p.Hk + hk) * p.Rp;
   const float* const delta = p.minus_delta + ((long long)n * p.Hk + hk) * p.Rp;
   const unsigned char* const mkey =
-      MASKED && p.mask ? p.mask + n * p.m_n + (long long)hk * p.G * p.m_h + (long long)(key < p.Lk ? key : 0) * p.m_k : nullptr;
+      PAIRS ? p.mask + n * p.m_n + (long long)hk * p.G * p.m_h + (long long)(key < p.Lk ? key : 0) * p.m_k : nullptr;
   // Rows without an open key exist under masks and where the diagonal starts above the keys: they are not read, so that
   // whatever their memory holds meets no product.
   const bool empty_rows = MASKED || (p.causal && p.off < 0);
@@ -138,9 +124,27 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
 
+  // The first tile of rows is asked for before the wavefront's own keys and values (of a closed key: zeros, whatever its
+  // memory holds).
   if (t0 < t1) {
     if (empty_rows) ask_live(t0);
     stage(t0, 0);
+  }
+  AttnFrag<T> kf[KS], vf[VL ? 1 : KS];
+  {
+    const long long kk = key_ok ? key : 0;
+    const char* ks_ = p.k.p + ((long long)n * p.k.n + kk * p.k.l + (long long)hk * p.k.h) * (int)sizeof(T);
+    const char* vs_ = p.v.p + ((long long)n * p.v.n + kk * p.v.l + (long long)hk * p.v.h) * (int)sizeof(T);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = load_frag<T>(ks_, ks, h, p.D, key_ok);
+      if (!VL) vf[ks] = load_frag<T>(vs_, ks, h, p.D, key_ok);
+    }
+    if (VL) {     // this wavefront's 32 rows of V, through registers, in the tiles' permutation
+      char* const vt = smem + 2 * STAGE_B;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) Rd::write_rows(vt, wave * 32, ks, lane, load_frag<T>(vs_, ks, h, p.D, key_ok));
+    }
   }
   auto step = [&](int t, auto buf_) __attribute__((always_inline)) {
     constexpr int buf = buf_.value;
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
       const int row0 = t * QT + rb * 32;
       if (rb > 0 && row0 >= p.R) return;
       unsigned char open[16];
-      if (MASKED && mkey) {
+      if (PAIRS) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int r = min(row0 + 8 * (i >> 2) + 4 * h + (i & 3), p.R - 1);
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
           s[i] = key <= div_g(p, r) + p.off ? s[i] : 0.f;
         }
       }
-      if (MASKED && mkey) {
+      if (PAIRS) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = open[i] != 0 ? s[i] : 0.f;
       }
@@ -277,10 +281,10 @@ template <typename T, int DP>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   constexpr int QT = dkv_rows<T, DP>();
   const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + (dkv_v_in_lds<T, DP>() ? 128 * AttnTile<T, DP>::PITCH : 0);
-  static std::atomic<int> seen[2][ATTN_DEVICES];
-  const bool masked = p->mask || p->kmask;
-  auto kern = masked ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>;
-  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
+  static std::atomic<int> seen[3][ATTN_DEVICES];
+  const int masks = p->mask ? 2 : p->kmask ? 1 : 0;
+  auto kern = p->mask ? attn_dkv_kernel<T, DP, 2> : p->kmask ? attn_dkv_kernel<T, DP, 1> : attn_dkv_kernel<T, DP, 0>;
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masks]);
   if (per_cu < 0) return per_cu;
   p->tiles = ceil_div(p->Lk, 128);
   p->loop_rows = QT;

@@ -44,7 +44,7 @@ struct AttnGradRow {
 };
 
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : 2)) void attn_dq_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : 3)) void attn_dq_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
