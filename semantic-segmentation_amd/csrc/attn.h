@@ -59,24 +59,35 @@ struct AttnDev {
 
 __device__ __forceinline__ int div_g(const AttnDev& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.g_magic); }
 
-// What a workgroup does.  The tiles of all problems are numbered; the first `whole` of them (full rounds of the chip) go to
-// one workgroup each, the `rest` that would leave most of the chip idle for a round are cut along their loop into `parts`
-// parts, whose results another kernel joins in part order.  A problem with few tiles is all rest.  Workgroups of one XCD
-// (blockIdx % 8 in launch order) take neighbouring tiles, or the same part of neighbouring tiles: they share keys and
-// values (rows, in the backward pass over keys) in that XCD's L2.
+// What a workgroup does.  The tiles of all problems (a problem: one image's key / value head) are numbered; the first
+// `whole` of them (full rounds of the chip) go to one workgroup each, the `rest` that would leave most of the chip idle for
+// a round are cut along their loop into `parts` parts, whose results another kernel joins in part order.  A problem with few
+// tiles is all rest.  The tiles of one problem stay on one XCD (blockIdx % 8 in launch order): they share keys and values
+// (rows, in the backward pass over keys) in its L2.  Problems are dealt to the XCDs in turns where their number allows, so
+// that images of different lengths even out; else XCDs take runs of tiles.
 struct AttnWork {
   int n, hk, tile;   // n < 0: nothing
   int part, parts;
   int slot;          // number among the tiles that are cut
 };
-__device__ __forceinline__ void attn_decode_tile(const AttnDev& p, int g, AttnWork* w) {
-  w->tile = g % p.tiles;
-  g /= p.tiles;
+__device__ __forceinline__ void attn_decode(const AttnDev& p, int problem, int tile, AttnWork* w) {
   // (under the diagonal the last tiles are the longest: they start first)
-  if (p.causal) w->tile = p.tiles - 1 - w->tile;
-  w->hk = g % p.Hk;
-  w->n = g / p.Hk;
+  w->tile = p.causal ? p.tiles - 1 - tile : tile;
+  w->hk = problem % p.Hk;
+  w->n = problem / p.Hk;
 }
+// tile number g of all
+__device__ __forceinline__ void attn_decode_tile(const AttnDev& p, int g, AttnWork* w) {
+  if (((p.N * p.Hk) & 7) == 0 && !p.even_steps) {
+    const int whole_x = p.whole >> 3, rest_x = p.rest >> 3, s = g - p.whole;
+    const int x = s < 0 ? g / whole_x : s / rest_x;
+    const int i = s < 0 ? g - x * whole_x : whole_x + s - x * rest_x;
+    attn_decode(p, x + 8 * (i / p.tiles), i % p.tiles, w);
+  } else {
+    attn_decode(p, g / p.tiles, g % p.tiles, w);
+  }
+}
+
 // Steps of a tile's loop under the diagonal.
 __host__ __device__ inline int attn_causal_steps(const AttnDev& p, int tile) {
   if (p.loop_rows) {           // keys tile * 128 .. : rows from the first token that may use one of them
