@@ -6,7 +6,7 @@
 // The contracted elements may be dealt to the (h, e) slots in any order as long as both operands use the same one.  A
 // result tile therefore IS the operand of the next product without any exchange between lanes: registers 8 s .. 8 s + 7
 // of a tile of scores hold rows 16 s + 8 (e / 4) + 4 h + e % 4, and the other operand is read from LDS in that order
-// (AttnRead::cols below).  So the probabilities never leave the registers of the lane that computed them.
+// (AttnLane::cols below).  So the probabilities never leave the registers of the lane that computed them.
 //   bf16: v_mfma_f32_32x32x16_bf16; fp32: eight v_mfma_f32_32x32x2_f32 on the same fragments.
 //
 // Shared heads: the G = Hq / Hk query heads that read one key / value head are packed into the rows of one problem,
@@ -52,8 +52,9 @@ struct AttnDev {
   int whole, rest, parts, rest_x; // how the tiles are dealt out, see attn_work
   int even_steps, even_units;     // tiles of different lengths: steps of a part, parts of one problem (0: equal lengths)
   int loop_rows;                  // what a tile's loop runs over: 0 keys by 64, else packed rows by this many
-  float* part;                    // partial results: [rest][parts][rows of a tile][D] (dk and dv: one after the other)
-  float* part_ml;                 // [rest][parts][rows of a tile][2]: maxima and sums of the forward pass
+  int tile_rows;                  // rows of a tile that exist: 128, of a shorter problem all of it
+  float* part;                    // partial results: [rest][parts][tile_rows][D] (keys: [rest][parts][dk, dv][128][D])
+  float* part_ml;                 // [rest][parts][tile_rows][2]: maxima and sums of the forward pass
   float *row_lse2, *minus_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and -rowsum(dout * out)
 };
 
@@ -63,8 +64,9 @@ __device__ __forceinline__ int div_g(const AttnDev& p, int r) { return p.G == 1 
 // `whole` of them (full rounds of the chip) go to one workgroup each, the `rest` that would leave most of the chip idle for
 // a round are cut along their loop into `parts` parts, whose results another kernel joins in part order.  A problem with few
 // tiles is all rest.  The tiles of one problem stay on one XCD (blockIdx % 8 in launch order): they share keys and values
-// (rows, in the backward pass over keys) in its L2.  Problems are dealt to the XCDs in turns where their number allows, so
-// that images of different lengths even out; else XCDs take runs of tiles.
+// (rows, in the backward pass over keys) in its L2.  XCDs take runs of problems; under a key mask, whose images differ in
+// length, problems are dealt to them in turns where their number allows.  16 images of 961 keys, a third of them padding:
+// forward 90.5 -> 87, dq 108 -> 103 us; of equal images it costs 1.5 % (1089 tokens, 64 heads: 104.8 -> 106.2 us).
 struct AttnWork {
   int n, hk, tile;   // n < 0: nothing
   int part, parts;
@@ -78,7 +80,7 @@ __device__ __forceinline__ void attn_decode(const AttnDev& p, int problem, int t
 }
 // tile number g of all
 __device__ __forceinline__ void attn_decode_tile(const AttnDev& p, int g, AttnWork* w) {
-  if (((p.N * p.Hk) & 7) == 0 && !p.even_steps) {
+  if (p.kmask && ((p.N * p.Hk) & 7) == 0 && !p.even_steps) {
     const int whole_x = p.whole >> 3, rest_x = p.rest >> 3, s = g - p.whole;
     const int x = s < 0 ? g / whole_x : s / rest_x;
     const int i = s < 0 ? g - x * whole_x : whole_x + s - x * rest_x;
@@ -209,7 +211,7 @@ __device__ __forceinline__ AttnFrag<float> pack_sum<float>(const float* x, float
 
 // ---- tiles in LDS -------------------------------------------------------------------------------
 // Rows of DP elements at a pitch of a power of two; the 16-byte chunks of a row are permuted by XOR with a function of
-// the row.  LDS serves 256 bytes a clock: 16 lanes of a 16-byte read (AttnRead::rows: the same chunk of 16 neighbouring
+// the row.  LDS serves 256 bytes a clock: 16 lanes of a 16-byte read (AttnLane::rows: the same chunk of 16 neighbouring
 // rows), 32 lanes of an 8-byte transposing read (cols in bf16: 64 bytes of four neighbouring rows) or 64 lanes of a 4-byte
 // read (cols in fp32: 128 bytes of two rows, four apart).  swz() gives each of these groups distinct banks (fp32 columns of
 // 128-byte rows excepted: both rows lie in the same half).
@@ -243,73 +245,14 @@ struct AttnPiece {
   __device__ __forceinline__ int chunk(int i) const { return Tile::PITCH == 512 ? chunk0 ^ (i & 1) : chunk0; }
 };
 
-// rows(): operand fragment contracted along the tile's rows in memory: lane (l & 31, h) reads elements 16 ks + 8 h .. + 7
-// of row row0 + (l & 31).
-// cols(): operand fragment contracted over the tile's rows: lane (l & 31, h) gets column d0 + (l & 31) of rows
-// row0 + 8 (e / 4) + 4 h + e % 4, the order in which a result tile holds them.
-template <typename T, int DP>
-struct AttnRead;
-template <int DP>
-struct AttnRead<bf16_t, DP> {
-  typedef AttnTile<bf16_t, DP> Tile;
-  static __device__ __forceinline__ AttnFrag<bf16_t> rows(const char* tile, int row0, int ks, int lane) {
-    AttnFrag<bf16_t> f;
-    f.v = *reinterpret_cast<const u32x4*>(tile + Tile::at(row0 + (lane & 31), 2 * ks + (lane >> 5)));
-    return f;
-  }
-  static __device__ __forceinline__ void write_rows(char* tile, int row0, int ks, int lane, const AttnFrag<bf16_t>& f) {
-    *reinterpret_cast<u32x4*>(tile + Tile::at(row0 + (lane & 31), 2 * ks + (lane >> 5))) = f.v;
-  }
-  static __device__ __forceinline__ AttnFrag<bf16_t> cols(const char* tile, int row0, int d0, int lane) {
-    // a group of 16 lanes reads a block of 4 rows x 16 columns, 8 bytes a lane, and receives it transposed
-    const int c0 = (d0 >> 3) + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-    AttnFrag<bf16_t> f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = row0 + 8 * j + 4 * (lane >> 5) + ((lane & 15) >> 2);
-      const attn_s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) attn_s16x4*)(__attribute__((address_space(3))) char*)(tile + Tile::at(row, c0) +
-                                                                                                (lane & 1) * 8));
-      const u32x2 u = __builtin_bit_cast(u32x2, t);
-      f.v[2 * j] = u[0];
-      f.v[2 * j + 1] = u[1];
-    }
-    return f;
-  }
-};
-template <int DP>
-struct AttnRead<float, DP> {
-  typedef AttnTile<float, DP> Tile;
-  static __device__ __forceinline__ AttnFrag<float> rows(const char* tile, int row0, int ks, int lane) {
-    AttnFrag<float> f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(tile + Tile::at(row0 + (lane & 31), 4 * ks + 2 * (lane >> 5) + j));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[4 * j + e] = t[e];
-    }
-    return f;
-  }
-  static __device__ __forceinline__ void write_rows(char* tile, int row0, int ks, int lane, const AttnFrag<float>& f) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<f32x4*>(tile + Tile::at(row0 + (lane & 31), 4 * ks + 2 * (lane >> 5) + j)) =
-          f32x4{f.v[4 * j], f.v[4 * j + 1], f.v[4 * j + 2], f.v[4 * j + 3]};
-  }
-  static __device__ __forceinline__ AttnFrag<float> cols(const char* tile, int row0, int d0, int lane) {
-    const int d = d0 + (lane & 31);
-    AttnFrag<float> f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int row = row0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-      f.v[e] = *reinterpret_cast<const float*>(tile + Tile::at(row, d >> 2) + (d & 3) * 4);
-    }
-    return f;
-  }
-};
-
-// The same reads from LDS byte addresses.  A lane's places differ between k-steps and columns by XORs that are kept in
-// registers; what is added (tile, row block) is a constant of the instruction where the caller's is one.
+// One lane's reads of a tile in LDS, from byte addresses; `at`: LDS byte of the block of rows.
+//   rows(): operand fragment contracted along the tile's rows in memory: lane (l & 31, h) reads elements 16 ks + 8 h .. + 7
+//           of row l & 31.
+//   cols(): operand fragment contracted over the tile's rows: lane (l & 31, h) gets column 32 db + (l & 31) of rows
+//           8 (e / 4) + 4 h + e % 4, the order in which a result tile holds them.
+//   write_rows(): stores what rows() reads.
+// bf16: a lane's places differ between k-steps and columns by XORs that are kept in registers; what is added (tile, row
+// block) is a constant of the instruction where the caller's is one.
 template <typename T, int DP>
 struct AttnLane;
 template <int DP>
@@ -324,15 +267,18 @@ struct AttnLane<bf16_t, DP> {
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        // (a group of 16 lanes reads a block of 4 rows x 16 columns, 8 bytes a lane, and receives it transposed)
         const int row = 8 * j + 4 * (lane >> 5) + ((lane & 15) >> 2);
         ca[db][j] = base + Tile::at(row, db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) + (lane & 1) * 8;
       }
   }
-  // rows / columns of the block of 32 (16) rows that starts at LDS byte `at`
   __device__ __forceinline__ AttnFrag<bf16_t> rows(int at, int ks) const {
     AttnFrag<bf16_t> f;
     f.v = *(const __attribute__((address_space(3))) u32x4*)(size_t)(ra[ks] + at);
     return f;
+  }
+  __device__ __forceinline__ void write_rows(int at, int ks, const AttnFrag<bf16_t>& f) const {
+    *(__attribute__((address_space(3))) u32x4*)(size_t)(ra[ks] + at) = f.v;
   }
   __device__ __forceinline__ AttnFrag<bf16_t> cols(int at, int db) const {
     AttnFrag<bf16_t> f;
@@ -348,11 +294,36 @@ struct AttnLane<bf16_t, DP> {
 };
 template <int DP>
 struct AttnLane<float, DP> {
-  const char* smem;
+  typedef AttnTile<float, DP> Tile;
+  char* smem;
   int lane;
-  __device__ __forceinline__ AttnLane(const char* s, int l) : smem(s), lane(l) {}
-  __device__ __forceinline__ AttnFrag<float> rows(int at, int ks) const { return AttnRead<float, DP>::rows(smem + at, 0, ks, lane); }
-  __device__ __forceinline__ AttnFrag<float> cols(int at, int db) const { return AttnRead<float, DP>::cols(smem + at, 0, db * 32, lane); }
+  __device__ __forceinline__ AttnLane(char* s, int l) : smem(s), lane(l) {}
+  __device__ __forceinline__ AttnFrag<float> rows(int at, int ks) const {
+    AttnFrag<float> f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(smem + at + Tile::at(lane & 31, 4 * ks + 2 * (lane >> 5) + j));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[4 * j + e] = t[e];
+    }
+    return f;
+  }
+  __device__ __forceinline__ void write_rows(int at, int ks, const AttnFrag<float>& f) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<f32x4*>(smem + at + Tile::at(lane & 31, 4 * ks + 2 * (lane >> 5) + j)) =
+          f32x4{f.v[4 * j], f.v[4 * j + 1], f.v[4 * j + 2], f.v[4 * j + 3]};
+  }
+  __device__ __forceinline__ AttnFrag<float> cols(int at, int db) const {
+    const int d = db * 32 + (lane & 31);
+    AttnFrag<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+      f.v[e] = *reinterpret_cast<const float*>(smem + at + Tile::at(row, d >> 2) + (d & 3) * 4);
+    }
+    return f;
+  }
 };
 
 // Keeps an operand packed from here on (the compiler would carry the unpacked values to its use).
@@ -447,11 +418,12 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Stages tiles of KT keys and their values.
+// Stages tiles of 64 keys and their values.
 template <typename T, int DP>
 struct AttnStage {
   typedef AttnTile<T, DP> Tile;
   typedef AttnPiece<T, DP> Piece;
+  static constexpr int KT = 64, TILE_B = KT * Tile::PITCH;
   Piece pc;
   int row_b;               // bytes of a row that exist
   unsigned k_step, v_step, lds0;
@@ -463,14 +435,14 @@ struct AttnStage {
     vbase = p.v.p + ((long long)n * p.v.n + (long long)hk * p.v.h) * (int)sizeof(T);
     lds0 = lds_addr(smem) + wave * 1024;
   }
-  // One operand's tile at byte `at` of LDS.
-  template <int KT, bool MASKED>
+  // One operand's tile at byte `at` of LDS.  bits: the tile's open keys (MASKED).  A closed key is not read: whatever its
+  // memory holds, zeros arrive.
+  template <bool MASKED>
   __device__ __forceinline__ void one(const AttnDev& p, const char* base, unsigned step, int key0, int at, unsigned long long bits) const {
-    static_assert(KT == 64, "one word of key bits");
     const u32x4 rsrc = buffer_of(base + (long long)key0 * step);
     const bool inside = !MASKED && key0 + KT <= p.Lk;
 #pragma unroll
-    for (int i = 0; i < KT * Tile::PITCH / 4096; ++i) {
+    for (int i = 0; i < TILE_B / 4096; ++i) {
       const int x = pc.row + i * Piece::STEP, c = pc.chunk(i) * 16;
       const unsigned off = c < row_b ? x * step + c : ATTN_OOB;
       if (inside) {
@@ -482,56 +454,30 @@ struct AttnStage {
       }
     }
   }
-  // bits: the tile's open keys (MASKED).  A closed key is not read: whatever its memory holds, zeros arrive.
-  template <int KT, bool MASKED>
-  __device__ __forceinline__ void keys(const AttnDev& p, int key0, int buf, const unsigned long long* bits) const {
-    constexpr int TILE_B = KT * Tile::PITCH;
-    const u32x4 kr = buffer_of(kbase + (long long)key0 * k_step), vr = buffer_of(vbase + (long long)key0 * v_step);
-    const bool inside = !MASKED && key0 + KT <= p.Lk;
-#pragma unroll
-    for (int i = 0; i < TILE_B / 4096; ++i) {
-      const int x = pc.row + i * Piece::STEP, c = pc.chunk(i) * 16;
-      const unsigned lds = lds0 + buf * (2 * TILE_B) + i * 4096;
-      // (a row's missing chunks are the same in every tile)
-      const unsigned ko = c < row_b ? x * k_step + c : ATTN_OOB, vo = c < row_b ? x * v_step + c : ATTN_OOB;
-      if (inside) {
-        dma_1k(kr, lds, ko);
-        dma_1k(vr, lds + TILE_B, vo);
-      } else {
-        bool in = key0 + x < p.Lk;
-        if (MASKED) in = in && ((bits[i * Piece::STEP >> 6] >> (x & 63)) & 1);
-        dma_1k(kr, lds, in ? ko : ATTN_OOB);
-        dma_1k(vr, lds + TILE_B, in ? vo : ATTN_OOB);
-      }
-    }
+  // both operands' tiles of buffer `buf`: K and V one after the other
+  template <bool MASKED>
+  __device__ __forceinline__ void both(const AttnDev& p, int key0, int buf, unsigned long long bits) const {
+    one<MASKED>(p, kbase, k_step, key0, buf * 2 * TILE_B, bits);
+    one<MASKED>(p, vbase, v_step, key0, buf * 2 * TILE_B + TILE_B, bits);
   }
 };
 
 // Keeps a rarely taken uniform branch a branch (the compiler would compute both sides and select).
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
-// Key mask of a tile of KT keys as one bit per key, the same in every wavefront: load() asks for a tile's bytes, next()
-// turns the bytes asked for last into bits.  Without a mask a key's bit says whether the key exists.
-template <int KT>
+// Key mask of a tile of 64 keys as one bit per key, the same in every wavefront: load() asks for a tile's bytes, next()
+// turns the bytes asked for last into bits.  Without a key mask (under a pair mask) a key's bit says whether the key exists.
 struct AttnKeyMask {
   const unsigned char* mask;
   long long step;
   int Lk, lane;
-  unsigned char raw[KT / 64];
-  unsigned long long bits[KT / 64];
+  unsigned char raw;
   __device__ __forceinline__ AttnKeyMask(const unsigned char* m, long long s, int lk, int ln) : mask(m), step(s), Lk(lk), lane(ln) {}
   __device__ __forceinline__ void load(int key0) {
-#pragma unroll
-    for (int i = 0; i < KT / 64; ++i) {
-      const int j = key0 + i * 64 + lane;
-      raw[i] = j < Lk ? (mask ? mask[j * step] : 1) : 0;
-    }
+    const int j = key0 + lane;
+    raw = j < Lk ? (mask ? mask[j * step] : 1) : 0;
   }
-  __device__ __forceinline__ void next() {
-#pragma unroll
-    for (int i = 0; i < KT / 64; ++i) bits[i] = __ballot(raw[i] != 0);
-  }
-  __device__ __forceinline__ unsigned word(int key) const { return (unsigned)(bits[KT == 64 ? 0 : key >> 6] >> (key & 63)); }
+  __device__ __forceinline__ unsigned long long next() const { return __ballot(raw != 0); }
 };
 
 // The closed keys of a tile of 64 as what the products of its scores start from: 0 or -inf for every key, in LDS.
@@ -607,12 +553,7 @@ __device__ __forceinline__ void close_past(f32x16& s, float closed, int lim) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) <= lim ? s[i] : closed;
 }
-// ... by the key mask's word, by the pair mask.
-__device__ __forceinline__ void close_word(f32x16& s, float closed, unsigned word, int h) {
-  const unsigned x = word >> (4 * h);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = x & (1u << (8 * (i >> 2) + (i & 3))) ? s[i] : closed;
-}
+// ... by the pair mask.
 __device__ __forceinline__ void close_pairs(f32x16& s, float closed, const unsigned* pair) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = pair[i >> 2] & (0xffu << (8 * (i & 3))) ? s[i] : closed;
@@ -630,23 +571,8 @@ __device__ __forceinline__ float pair_sum(float v) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Spreads MFMA instructions among the vector instructions and LDS reads of a basic block: `mfma` of them, `reads` LDS reads.
-template <typename T, int MFMA, int READS>
-__device__ __forceinline__ void interleave() {
-  if constexpr (sizeof(T) == 2) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-    for (int i = 0; i < MFMA; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, (READS + MFMA - 1) / MFMA, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, (60 + MFMA - 1) / MFMA, 0);
-    }
-  }
-}
-
 // ---- host side ----------------------------------------------------------------------------------
 int attn_check(const segk_attention_args* a, AttnDev* p, bool backward);                 // attn_fwd.hip
-bool attn_few(const AttnDev& p, int dtype);
 // Deals p->tiles of every problem out to workgroups of which `per_cu` share a CU; `steps`: length of a tile's loop, of
 // which a part takes at least min_steps.  Returns the grid.
 long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps);

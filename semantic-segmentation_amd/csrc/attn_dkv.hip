@@ -8,29 +8,28 @@
 
 namespace segk {
 
+// Rows of a tile: 32, or 64 where 32 are less than a KiB for every wavefront to stage (64 channels, bf16, 16 images of 961
+// tokens, 16 heads: 159 us with 32, 170 us with 64).
 template <typename T, int DP>
-constexpr bool dkv_v_in_lds() { return DP * (int)sizeof(T) >= 192; }
-template <typename T, int DP>
-constexpr int dkv_rows() { return dkv_v_in_lds<T, DP>() ? 32 : 64; }
+constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 
 // 4 wavefronts of 32 keys.  Scores are computed with queries as rows (a lane owns one key), so P and dS are the operands
 // of dV^T = dO^T P and dK^T = Q^T dS as they lie.  K of the wavefront's keys stays in registers; Q and dO tiles of QT rows
 // are staged through LDS and read both along rows and along columns.
-// V stays in registers too where the heads are small; where they are not (VL) it lies in LDS: 32 registers less bring two
-// wavefronts to a SIMD, which cover each other's exponentials, for a quarter more LDS reads.
+// V lies in LDS, too: at 128 channels the registers it would take leave one wavefront to a SIMD instead of two, which cover
+// each other's exponentials (2.49 -> 1.13 ms at 4225 tokens, 32 heads over 8, bf16); at 64 channels 165 -> 159 us; at
+// 32 it costs 1.5 % (class queries, 47.7 -> 48.5 us), which is not worth a second form.
 // MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
 template <typename T, int DP, int MASKS>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
-  typedef AttnRead<T, DP> Rd;
   typedef AttnPiece<T, DP> Piece;
-  constexpr bool VL = dkv_v_in_lds<T, DP>();
   constexpr int QT = dkv_rows<T, DP>();
   constexpr bool MASKED = MASKS != 0, PAIRS = MASKS == 2;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = QT * Tile::PITCH;
   constexpr int STAGE_B = 2 * TILE_B + 512;      // Q tile, dO tile, lse, delta
-  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 stages, V (VL)
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 stages, V
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
@@ -53,7 +52,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   if (MASKED && p.kmask && !any_open_key(p.kmask + n * p.km_n, p.km_k, key_wg, p.Lk, lane)) t1 = t0;
 
   const AttnLane<T, DP> ln(smem, lane);
-  const AttnLane<T, DP> lv(smem + wave * 32 * Tile::PITCH, lane);     // (VL: this wavefront's rows of V)
+  const AttnLane<T, DP> lv(smem + wave * 32 * Tile::PITCH, lane);     // this wavefront's rows of V
   const Piece pc(wave, lane);
   const int row_b = p.D * (int)sizeof(T);
   const char* const qbase = p.q.p + ((long long)n * p.q.n + (long long)hk * p.G * p.q.h) * (int)sizeof(T);
@@ -130,21 +129,15 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
     if (empty_rows) ask_live(t0);
     stage(t0, 0);
   }
-  AttnFrag<T> kf[KS], vf[VL ? 1 : KS];
+  AttnFrag<T> kf[KS];
   {
     const long long kk = key_ok ? key : 0;
     const char* ks_ = p.k.p + ((long long)n * p.k.n + kk * p.k.l + (long long)hk * p.k.h) * (int)sizeof(T);
     const char* vs_ = p.v.p + ((long long)n * p.v.n + kk * p.v.l + (long long)hk * p.v.h) * (int)sizeof(T);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kf[ks] = load_frag<T>(ks_, ks, h, p.D, key_ok);
-      if (!VL) vf[ks] = load_frag<T>(vs_, ks, h, p.D, key_ok);
-    }
-    if (VL) {     // this wavefront's 32 rows of V, through registers, in the tiles' permutation
-      char* const vt = smem + 2 * STAGE_B;
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = load_frag<T>(ks_, ks, h, p.D, key_ok);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) Rd::write_rows(vt, wave * 32, ks, lane, load_frag<T>(vs_, ks, h, p.D, key_ok));
-    }
+    for (int ks = 0; ks < KS; ++ks) lv.write_rows(2 * STAGE_B, ks, load_frag<T>(vs_, ks, h, p.D, key_ok));
   }
   auto step = [&](int t, auto buf_) __attribute__((always_inline)) {
     constexpr int buf = buf_.value;
@@ -175,8 +168,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) mma32(s, ln.rows(qt + rb * 32 * Tile::PITCH, ks), kf[ks]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        mma32(dp, ln.rows(gt + rb * 32 * Tile::PITCH, ks), VL ? lv.rows(2 * STAGE_B, ks) : vf[VL ? 0 : ks]);
+      for (int ks = 0; ks < KS; ++ks) mma32(dp, ln.rows(gt + rb * 32 * Tile::PITCH, ks), lv.rows(2 * STAGE_B, ks));
       if (rb == 0 && t + 1 < t1) stage(t + 1, buf ^ 1);     // (behind the first LDS reads, as in the forward kernel)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
@@ -280,7 +272,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dkv_sum_kernel(const AttnDe
 template <typename T, int DP>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   constexpr int QT = dkv_rows<T, DP>();
-  const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + (dkv_v_in_lds<T, DP>() ? 128 * AttnTile<T, DP>::PITCH : 0);
+  const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + 128 * AttnTile<T, DP>::PITCH;
   static std::atomic<int> seen[3][ATTN_DEVICES];
   const int masks = p->mask ? 2 : p->kmask ? 1 : 0;
   auto kern = p->mask ? attn_dkv_kernel<T, DP, 2> : p->kmask ? attn_dkv_kernel<T, DP, 1> : attn_dkv_kernel<T, DP, 0>;

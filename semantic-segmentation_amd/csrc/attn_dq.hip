@@ -7,7 +7,7 @@
 
 namespace segk {
 
-// Both kernels as their forward counterparts (attn_fwd.hip): a lane owns one query,
+// As the forward kernel (attn_fwd.hip): a lane owns one query,
 //   S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
 // What a row needs: its statistics and its query and output gradient in registers (zeros for a row that has no open key,
 // whatever its memory holds).
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
 
   const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
   const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
-  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
+  AttnKeyMask km(kmask, p.km_k, p.Lk, lane);
   char* const start0 = smem + 4 * TILE_B;
 
   const int last_row = min(w.tile * 128 + 128, p.R) - 1;
@@ -70,12 +70,13 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   const int per = (all_steps + w.parts - 1) / w.parts;
   const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
   auto stage = [&](int t, int buf) __attribute__((always_inline)) {
+    unsigned long long bits = 0;
     if (MASKED) {
-      km.next();
+      bits = km.next();
       km.load((t + 1) * KT);
-      if (wave == 0) write_start(start0 + buf * 256, km.bits[0], lane);
+      if (wave == 0) write_start(start0 + buf * 256, bits, lane);
     }
-    st.template keys<KT, MASKED>(p, t * KT, buf, km.bits);
+    st.template both<MASKED>(p, t * KT, buf, bits);
   };
   if (t0 < t1) {               // the first tile is asked for before anything else
     if (MASKED) km.load(t0 * KT);
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
           store4<T>(p.dq + at * (int)sizeof(T), d, dq[db][i] * p.scale, dq[db][i + 1] * p.scale, dq[db][i + 2] * p.scale, dq[db][i + 3] * p.scale);
       }
   } else {
-    char* dst = (char*)(p.part + (((long long)w.slot * p.parts + w.part) * 128 + wave * 32 + l31) * p.D);
+    char* dst = (char*)(p.part + (((long long)w.slot * p.parts + w.part) * p.tile_rows + wave * 32 + l31) * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -166,131 +167,22 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
   }
 }
 
-template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_dq_few_kernel(const AttnDev p) {
-  typedef AttnTile<T, DP> Tile;
-  typedef AttnRead<T, DP> Rd;
-  constexpr int KT = 128, KS = DP / 16, DB = DP / 32;
-  constexpr int TILE_B = KT * Tile::PITCH;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
-
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  const AttnWork w = attn_work(p);
-  if (w.n < 0) return;
-  const int n = w.n, hk = w.hk;
-
-  int k_end = p.Lk;
-  if (p.causal) k_end = max(0, min(k_end, div_g(p, p.R - 1) + p.off + 1));
-  const int all_steps = (k_end + KT - 1) / KT;
-  const int per = (all_steps + w.parts - 1) / w.parts;
-  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
-
-  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
-  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
-  if (t0 < t1) {
-    if (MASKED) {
-      km.load(t0 * KT);
-      km.next();
-      km.load((t0 + 1) * KT);
-    }
-    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
-  }
-  const AttnGradRow<T, DP> row(p, n, hk, l31, h);
-  const int lim = (p.causal ? min(p.Lk - 1, row.tok + p.off) : p.Lk - 1) - 4 * h;
-  const int ragged0 = p.causal ? min(p.Lk, p.off + 1) : p.Lk;
-  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)row.head * p.m_h + (long long)row.tok * p.m_q : nullptr, p.m_k, p.Lk, h);
-  if (MASKED && t0 < t1) pm.load(t0 * KT + wave * 32);
-
-  f32x16 dq[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) dq[db] = zero16();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    tile_barrier();
-    const int key0 = t * KT + wave * 32;
-    unsigned word = 0, pair[4];
-    bool dead = false;
-    if (MASKED) {
-      word = km.word(wave * 32);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pair[g] = pm.w[g];
-      dead = word == 0;
-      if (pm.row && !dead) dead = !__any(row.lse2 != INFINITY && (pair[0] | pair[1] | pair[2] | pair[3]) != 0);
-    }
-    if (t + 1 < t1) {
-      if (MASKED) {
-        km.next();
-        km.load((t + 2) * KT);
-        pm.load((t + 1) * KT + wave * 32);
-      }
-      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
-    }
-    if (dead) continue;
-    const char* kt = smem + buf * (2 * TILE_B) + wave * 32 * Tile::PITCH;
-    f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, 0, ks, lane), row.qf[ks]);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) mma32(dp, Rd::rows(kt + TILE_B, 0, ks, lane), row.gf[ks]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dp[i] = exp2_fast(fmaf(s[i], p.scale_log2, -row.lse2)) * (dp[i] + row.minus);
-    if (key0 + 32 > ragged0) close_past(dp, 0.f, lim - key0);
-    if (MASKED) {
-      close_word(dp, 0.f, word, h);
-      if (pm.row) close_pairs(dp, 0.f, pair);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const AttnFrag<T> sf = pack_frag<T>(dp, j);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) mma32(dq[db], Rd::cols(kt, j * 16, db * 32, lane), sf);
-    }
-  }
-
-  constexpr int LD = DP + 4;
-  float* const so = reinterpret_cast<float*>(smem);
-  tile_barrier();
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
-          f32x4{dq[db][i], dq[db][i + 1], dq[db][i + 2], dq[db][i + 3]};
-  tile_barrier();
-  for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
-    const int rw = x / (DP / 4), d = x % (DP / 4) * 4;
-    if (rw >= p.R || d >= p.D) continue;
-    f32x4 v = *reinterpret_cast<const f32x4*>(so + rw * LD + d);
-#pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + rw) * LD + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += y[e];
-    }
-    const int tk = div_g(p, rw), hd = hk * p.G + rw - tk * p.G;
-    const long long at = (((long long)n * p.Lq + tk) * p.Hq + hd) * p.D;
-    if (w.parts == 1) store4<T>(p.dq + at * (int)sizeof(T), d, v[0] * p.scale, v[1] * p.scale, v[2] * p.scale, v[3] * p.scale);
-    else store4<float>((char*)(p.part + (((long long)w.slot * p.parts + w.part) * p.R + rw) * p.D), d, v[0], v[1], v[2], v[3]);
-  }
-}
-
 // Sums the parts of the tiles that were cut, in part order: 4 channels of one row a thread.
 template <typename T>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev p, int tile_rows) {
+__global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev p) {
   const long long x = (long long)blockIdx.x * ATTN_THREADS + threadIdx.x;
   const int quads = p.D / 4;
   const long long line = x / quads;
   const int d = (int)(x - line * quads) * 4;
-  if (line >= (long long)p.rest * tile_rows) return;
-  const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
+  if (line >= (long long)p.rest * p.tile_rows) return;
+  const int slot = (int)(line / p.tile_rows), row = (int)(line - (long long)slot * p.tile_rows);
   AttnWork w;
   attn_decode_tile(p, p.whole + slot, &w);
-  const int rr = w.tile * tile_rows + row, parts = attn_tile_parts(p, w.tile);
+  const int rr = w.tile * 128 + row, parts = attn_tile_parts(p, w.tile);
   if (rr >= p.R || parts == 1) return;       // (a tile in one part is finished)
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < parts; ++s) {
-    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * tile_rows + row) * p.D + d);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * p.tile_rows + row) * p.D + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += y[e];
   }
@@ -299,45 +191,39 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dq_sum_kernel(const AttnDev
             v[2] * p.scale, v[3] * p.scale);
 }
 
-template <typename T, int DP, bool FEW>
+template <typename T, int DP>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   static std::atomic<int> seen[2][ATTN_DEVICES];
   const bool masked = p->mask || p->kmask;
-  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH + (masked && !FEW ? 512 : 0);
-  void (*kern)(const AttnDev);
-  if constexpr (FEW) kern = masked ? attn_dq_few_kernel<T, DP, true> : attn_dq_few_kernel<T, DP, false>;
-  else kern = masked ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>;
+  const int lds = 4 * 64 * AttnTile<T, DP>::PITCH + (masked ? 512 : 0);
+  void (*const kern)(const AttnDev) = masked ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>;
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
-  p->tiles = FEW ? 1 : ceil_div(p->R, 128);
+  p->tiles = ceil_div(p->R, 128);
   p->loop_rows = 0;
   SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention_bwd: too many workgroups");
-  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, FEW ? 128 : 64), FEW ? 1 : 2);
+  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, 64), 2);
   if (plan_only) return SEGK_OK;
   kern<<<(unsigned)grid, ATTN_THREADS, lds, st>>>(*p);
   SEGK_CHECK_LAUNCH("attention_bwd queries");
   if (p->parts > 1) {
-    const int tile_rows = FEW ? p->R : 128;
-    const long long blocks = ((long long)p->rest * tile_rows * (p->D / 4) + ATTN_THREADS - 1) / ATTN_THREADS;
-    attn_dq_sum_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(*p, tile_rows);
+    const long long blocks = ((long long)p->rest * p->tile_rows * (p->D / 4) + ATTN_THREADS - 1) / ATTN_THREADS;
+    attn_dq_sum_kernel<T><<<(unsigned)blocks, ATTN_THREADS, 0, st>>>(*p);
     SEGK_CHECK_LAUNCH("attention_bwd queries' sum");
   }
   return SEGK_OK;
 }
 
 template <typename T>
-static int dispatch(AttnDev* p, bool few, bool plan_only, hipStream_t st) {
-  if (p->D <= 32) return few ? launch<T, 32, true>(p, plan_only, st) : launch<T, 32, false>(p, plan_only, st);
-  if (p->D <= 64) return few ? launch<T, 64, true>(p, plan_only, st) : launch<T, 64, false>(p, plan_only, st);
-  if constexpr (sizeof(T) == 2) {
-    if (few) return p->D <= 96 ? launch<T, 96, true>(p, plan_only, st) : launch<T, 128, true>(p, plan_only, st);
-  }
-  return p->D <= 96 ? launch<T, 96, false>(p, plan_only, st) : launch<T, 128, false>(p, plan_only, st);
+static int dispatch(AttnDev* p, bool plan_only, hipStream_t st) {
+  if (p->D <= 32) return launch<T, 32>(p, plan_only, st);
+  if (p->D <= 64) return launch<T, 64>(p, plan_only, st);
+  if (p->D <= 96) return launch<T, 96>(p, plan_only, st);
+  return launch<T, 128>(p, plan_only, st);
 }
 
 int attn_dq(AttnDev* p, int dtype, bool plan_only, hipStream_t st) {
-  const bool few = attn_few(*p, dtype);
-  return dtype == SEGK_BF16 ? dispatch<bf16_t>(p, few, plan_only, st) : dispatch<float>(p, few, plan_only, st);
+  return dtype == SEGK_BF16 ? dispatch<bf16_t>(p, plan_only, st) : dispatch<float>(p, plan_only, st);
 }
 
 }  // namespace segk

@@ -8,7 +8,7 @@
 
 namespace segk {
 
-// Both kernels: scores are computed transposed (S^T = K Q^T, a lane owns one query), so the running statistics are one
+// Scores are computed transposed (S^T = K Q^T, a lane owns one query), so the running statistics are one
 // register and S^T is the operand of O^T = V^T P^T as it lies (attn.h).  Keys in blocks of 32.
 //   p = exp2(s scale log2(e) - m) for a reference m that need not be the maximum: in floating point any m serves that
 //   neither overflows nor loses the largest terms.  m starts as the maximum of the first block that has an open key and is
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
 
   const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
   const unsigned char* const kmask = MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr;
-  AttnKeyMask<KT> km(kmask, p.km_k, p.Lk, lane);
+  AttnKeyMask km(kmask, p.km_k, p.Lk, lane);
   unsigned long long bits_next = ~0ULL;      // open keys of the K tile last asked for: V follows
 
   // keys that some row of the workgroup may use
@@ -90,13 +90,12 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
   if (t0 < t1) {                             // the first tile is asked for before anything else
     if (MASKED) {
       km.load(t0 * KT);
-      km.next();
-      bits_next = km.bits[0];
+      bits_next = km.next();
       km.load((t0 + 1) * KT);
       if (wave == 0) write_start(start0, bits_next, lane);
     }
-    st.template one<KT, MASKED>(p, st.kbase, st.k_step, t0 * KT, 0, bits_next);
-    st.template one<KT, MASKED>(p, st.vbase, st.v_step, t0 * KT, 2 * TILE_B, bits_next);
+    st.template one<MASKED>(p, st.kbase, st.k_step, t0 * KT, 0, bits_next);
+    st.template one<MASKED>(p, st.vbase, st.v_step, t0 * KT, 2 * TILE_B, bits_next);
   }
 
   const int r = row0 + l31;
@@ -159,26 +158,24 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
     const int t = t0 + u, there = TILE_B - here;
     unsigned long long bits2 = ~0ULL;
     if (MASKED) {
-      km.next();
-      bits2 = km.bits[0];
+      bits2 = km.next();
       km.load((t + 3) * KT);
       if (wave == 0) write_start(start0 + (here ? 256 : 0), bits2, lane);
     }
-    if (u + 2 <= last) st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t + 2) * KT, here, bits2);
-    st.template one<KT, MASKED>(p, st.vbase, st.v_step, (t + 1) * KT, 2 * TILE_B + there, bits_next);
+    if (u + 2 <= last) st.template one<MASKED>(p, st.kbase, st.k_step, (t + 2) * KT, here, bits2);
+    st.template one<MASKED>(p, st.vbase, st.v_step, (t + 1) * KT, 2 * TILE_B + there, bits_next);
     if (MASKED) bits_next = bits2;
   };
 
   if (t0 < t1) {
     if (MASKED) {
       if (pm.row) pm.load(t0 * KT);
-      km.next();
-      bits_next = km.bits[0];
+      bits_next = km.next();
       km.load((t0 + 2) * KT);
     }
     tile_barrier();
     if (last > 0) {
-      st.template one<KT, MASKED>(p, st.kbase, st.k_step, (t0 + 1) * KT, TILE_B, bits_next);
+      st.template one<MASKED>(p, st.kbase, st.k_step, (t0 + 1) * KT, TILE_B, bits_next);
       if (MASKED && wave == 0) write_start(start0 + 256, bits_next, lane);
     }
     if (row0 >= p.R) {          // no rows: this wavefront only helps to stage the tiles
@@ -232,7 +229,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
     if (p.lse && h == 0)
       p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (row.m + log2f(lt)) * 0.6931471805599453f;
   } else {
-    const long long at = ((long long)w.slot * p.parts + w.part) * 128 + wave * 32 + l31;
+    const long long at = ((long long)w.slot * p.parts + w.part) * p.tile_rows + wave * 32 + l31;
     char* dst = (char*)(p.part + at * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -248,156 +245,15 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP 
   }
 }
 
-// At most 32 rows (a query token, class queries): the wavefronts take the same rows and each its own 32 keys of a tile of
-// 128; their parts are joined in LDS at the end.  Memory-bound: nothing is pipelined but the tiles.  Blocks that the masks
-// close for every row are skipped.
-template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_fwd_few_kernel(const AttnDev p) {
-  typedef AttnTile<T, DP> Tile;
-  typedef AttnRead<T, DP> Rd;
-  constexpr int KT = 128, KS = DP / 16, DB = DP / 32;
-  constexpr int TILE_B = KT * Tile::PITCH;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];   // 2 x (K tile, V tile)
-
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  const AttnWork w = attn_work(p);
-  if (w.n < 0) return;
-  const int n = w.n, hk = w.hk;
-
-  int k_end = p.Lk;
-  if (p.causal) k_end = max(0, min(k_end, div_g(p, p.R - 1) + p.off + 1));
-  const int all_steps = (k_end + KT - 1) / KT;
-  const int per = (all_steps + w.parts - 1) / w.parts;
-  const int t0 = min(w.part * per, all_steps), t1 = min(t0 + per, all_steps);
-
-  const bool row_ok = l31 < p.R;
-  const int rr = row_ok ? l31 : 0;
-  const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
-  AttnFrag<T> qf[KS];
-  {
-    const char* src = p.q.p + ((long long)n * p.q.n + (long long)tok * p.q.l + (long long)head * p.q.h) * (int)sizeof(T);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<T>(src, ks, h, p.D, row_ok);
-  }
-  const int lim = (p.causal ? min(p.Lk - 1, tok + p.off) : p.Lk - 1) - 4 * h;
-  const int ragged0 = p.causal ? min(p.Lk, p.off + 1) : p.Lk;      // (row 0 is token 0)
-
-  const AttnStage<T, DP> st(p, n, hk, wave, lane, smem);
-  AttnKeyMask<KT> km(MASKED && p.kmask ? p.kmask + n * p.km_n : nullptr, p.km_k, p.Lk, lane);
-  AttnPairMask pm(MASKED && p.mask ? p.mask + n * p.m_n + (long long)head * p.m_h + (long long)tok * p.m_q : nullptr, p.m_k, p.Lk, h);
-
-  AttnRow<T, DB> row;
-  if (t0 < t1) {
-    if (MASKED) {
-      km.load(t0 * KT);
-      km.next();
-      km.load((t0 + 1) * KT);
-      pm.load(t0 * KT + wave * 32);
-    }
-    st.template keys<KT, MASKED>(p, t0 * KT, 0, km.bits);
-  }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    tile_barrier();                       // tile t is here; every wavefront has left tile t - 1
-    const int key0 = t * KT + wave * 32;
-    unsigned word = 0, pair[4];
-    bool dead = false;
-    if (MASKED) {
-      word = km.word(wave * 32);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pair[g] = pm.w[g];
-      dead = word == 0;
-      if (pm.row && !dead) dead = !__any(row_ok && (pair[0] | pair[1] | pair[2] | pair[3]) != 0);
-    }
-    if (t + 1 < t1) {
-      if (MASKED) {
-        km.next();
-        km.load((t + 2) * KT);
-        pm.load((t + 1) * KT + wave * 32);
-      }
-      st.template keys<KT, MASKED>(p, (t + 1) * KT, buf ^ 1, km.bits);
-    }
-    if (dead) continue;
-    const char* kt = smem + buf * (2 * TILE_B) + wave * 32 * Tile::PITCH;
-    f32x16 s = zero16();
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) mma32(s, Rd::rows(kt, 0, ks, lane), qf[ks]);
-    if (key0 + 32 > ragged0) close_past(s, -INFINITY, lim - key0);
-    if (MASKED) {
-      close_word(s, -INFINITY, word, h);
-      if (pm.row) close_pairs(s, -INFINITY, pair);
-    }
-    AttnFrag<T> pf[2];
-    float sum = row.weigh(s, p.scale_log2, row.m, pf);
-    if (!row.fine(sum)) sum = row.raise(s, p.scale_log2, pf);
-    row.l += sum;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) mma32(row.o[db], Rd::cols(kt + TILE_B, j * 16, db * 32, lane), pf[j]);
-  }
-
-  // join the four wavefronts' parts: [wave][row][DP + 4] sums, then 4 x 32 maxima and sums
-  const float lt = pair_sum(row.l);
-  constexpr int LD = DP + 4;
-  float* const so = reinterpret_cast<float*>(smem);
-  float* const sm = so + 4 * 32 * LD;
-  tile_barrier();
-  if (h == 0) sm[wave * 32 + l31] = row.m;
-  tile_barrier();
-  float all = sm[l31];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) all = fmaxf(all, sm[i * 32 + l31]);
-  const float a = exp2_fast(row.m - (all == -INFINITY ? 0.f : all));
-  if (h == 0) sm[128 + wave * 32 + l31] = lt * a;
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + db * 32 + 2 * i + 4 * h) =
-          f32x4{row.o[db][i] * a, row.o[db][i + 1] * a, row.o[db][i + 2] * a, row.o[db][i + 3] * a};
-  tile_barrier();
-  for (int x = threadIdx.x; x < 32 * (DP / 4); x += ATTN_THREADS) {
-    const int rw = x / (DP / 4), d = x % (DP / 4) * 4;
-    if (rw >= p.R || d >= p.D) continue;
-    f32x4 v = *reinterpret_cast<const f32x4*>(so + rw * LD + d);
-    float sum = sm[128 + rw], top = sm[rw];
-#pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(so + (i * 32 + rw) * LD + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += y[e];
-      sum += sm[128 + i * 32 + rw];
-      top = fmaxf(top, sm[i * 32 + rw]);
-    }
-    if (w.parts == 1) {
-      const int tk = div_g(p, rw), hd = hk * p.G + rw - tk * p.G;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      store4<T>(p.out + ((long long)n * p.o.n + (long long)tk * p.o.l + (long long)hd * p.o.h) * (int)sizeof(T), d, v[0] * inv, v[1] * inv,
-                v[2] * inv, v[3] * inv);
-      if (p.lse && d == 0)
-        p.lse[((long long)n * p.Hq + hd) * p.Lq + tk] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    } else {
-      const long long at = ((long long)w.slot * p.parts + w.part) * p.R + rw;
-      store4<float>((char*)(p.part + at * p.D), d, v[0], v[1], v[2], v[3]);
-      if (d == 0) {
-        p.part_ml[2 * at] = top;
-        p.part_ml[2 * at + 1] = sum;
-      }
-    }
-  }
-}
-
 // Joins the parts of the tiles that were cut.  `lanes` = D / 4 rounded up to a power of two threads walk a row's channels of
 // every `groups`-th part; the groups of a row are joined in LDS in order.  tile_rows: rows of a tile in the partial results.
 template <typename T>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes, int groups, int tile_rows) {
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes, int groups) {
   __shared__ f32x4 so[ATTN_THREADS];
   __shared__ float sl[ATTN_THREADS], sm[ATTN_THREADS];
   const int c = threadIdx.x % lanes, g = threadIdx.x / lanes % groups, in = threadIdx.x / (lanes * groups);
   const long long line = (long long)blockIdx.x * (ATTN_THREADS / (lanes * groups)) + in;
-  const int slot = (int)(line / tile_rows), row = (int)(line - (long long)slot * tile_rows);
+  const int slot = (int)(line / p.tile_rows), row = (int)(line - (long long)slot * p.tile_rows);
   AttnWork w = {0, 0, 0, 0, 1, 0};
   int parts = 0;
   if (slot < p.rest) {
@@ -405,11 +261,11 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
     parts = attn_tile_parts(p, w.tile);
   }
   const bool ok = parts > 1;       // (a tile in one part is finished)
-  const long long first = ok ? (long long)slot * p.parts * tile_rows + row : 0;
+  const long long first = ok ? (long long)slot * p.parts * p.tile_rows + row : 0;
   // every group looks at its own parts' maxima first, so that the sums are scaled once
   float m = -INFINITY, l = 0.f;
   if (ok)
-    for (int s = g; s < parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * tile_rows)]);
+    for (int s = g; s < parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * p.tile_rows)]);
   sm[threadIdx.x] = m;
   __syncthreads();
   for (int i = 0; i < groups; ++i) m = fmaxf(m, sm[(in * groups + i) * lanes + c]);
@@ -417,7 +273,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (ok)
     for (int s = g; s < parts; s += groups) {
-      const long long at = first + (long long)s * tile_rows;
+      const long long at = first + (long long)s * p.tile_rows;
       const float a = exp2_fast(p.part_ml[2 * at] - ms);
       l = fmaf(p.part_ml[2 * at + 1], a, l);
       if (c * 4 < p.D) {
@@ -430,7 +286,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   sl[threadIdx.x] = l;
   __syncthreads();
   if (!ok || g != 0 || c * 4 >= p.D) return;
-  const int rr = w.tile * tile_rows + row;
+  const int rr = w.tile * 128 + row;
   if (rr >= p.R) return;
   for (int i = 1; i < groups; ++i) {
     const f32x4 x = so[threadIdx.x + i * lanes];
@@ -488,19 +344,6 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_row_stats_kernel(const Attn
 }
 
 // ------------------------------------------------------------------ host ----
-static int attn_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-static int attn_pitch(int D, int dtype) {
-  const int b = attn_dp(D) * dtype_size(dtype);
-  return b <= 64 ? 64 : b <= 128 ? 128 : b <= 256 ? 256 : 512;
-}
-
-// The wavefronts divide the keys instead of the rows where 32 rows hold the whole problem, except for fp32 heads over 64
-// channels, whose tiles of 128 keys do not fit into LDS twice, and for keys so far apart that 128 pass a buffer's range.
-bool attn_few(const AttnDev& p, int dtype) {
-  const long long far = (p.k.l > p.v.l ? p.k.l : p.v.l) * 128 * dtype_size(dtype);
-  return p.R <= 32 && attn_pitch(p.D, dtype) <= 256 && far < 0xf0000000LL;
-}
-
 long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps) {
   const long long all = (long long)p->tiles * p->N * p->Hk;
   const long long round = 256LL * per_cu;      // workgroups that run at once
@@ -579,7 +422,7 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   SEGK_REQUIRE(a->N > 0 && a->Lq > 0 && a->Lk >= 0 && a->Hq > 0 && a->Hk > 0 && a->Hq % a->Hk == 0,
                "attention: bad shape N=%d Lq=%d Lk=%d Hq=%d Hk=%d", a->N, a->Lq, a->Lk, a->Hq, a->Hk);
   SEGK_UNSUPPORTED(a->D > 0 && a->D <= 128 && a->D % 8 == 0, "attention: head size %d is not a multiple of 8 up to 128", a->D);
-  SEGK_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "attention: the scale must be positive and finite");
+  SEGK_REQUIRE(a->scale > 0.f && a->scale * LOG2E < INFINITY, "attention: the scale must be positive and finite");
   const int e8 = 16 / dtype_size(a->dtype);
   const int G = a->Hq / a->Hk;
   CHK_VIEW(q, "q", a->Lq, G);
@@ -605,6 +448,7 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   p->N = a->N, p->Lq = a->Lq, p->Lk = a->Lk, p->Hq = a->Hq, p->Hk = a->Hk, p->G = G, p->D = a->D;
   p->R = (int)R;
   p->Rp = round_up((int)R, 64);
+  p->tile_rows = R < 128 ? (int)R : 128;
   p->g_magic = G > 1 ? (unsigned)((0x100000000ULL + G - 1) / G) : 0;
   p->causal = a->causal != 0;
   p->off = a->Lk - a->Lq;
@@ -626,19 +470,17 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   return SEGK_OK;
 }
 
-template <typename T, int DP, bool FEW>
+template <typename T, int DP>
 static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
   static std::atomic<int> seen[2][ATTN_DEVICES];
   const bool masked = p->mask || p->kmask;
-  const int lds = 4 * (FEW ? 128 : 64) * AttnTile<T, DP>::PITCH + (masked && !FEW ? 512 : 0);
-  void (*kern)(const AttnDev);
-  if constexpr (FEW) kern = masked ? attn_fwd_few_kernel<T, DP, true> : attn_fwd_few_kernel<T, DP, false>;
-  else kern = masked ? attn_fwd_kernel<T, DP, true> : attn_fwd_kernel<T, DP, false>;
+  const int lds = 4 * 64 * AttnTile<T, DP>::PITCH + (masked ? 512 : 0);
+  void (*const kern)(const AttnDev) = masked ? attn_fwd_kernel<T, DP, true> : attn_fwd_kernel<T, DP, false>;
   const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
   if (per_cu < 0) return per_cu;
-  p->tiles = FEW ? 1 : ceil_div(p->R, 128);
+  p->tiles = ceil_div(p->R, 128);
   SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention: too many workgroups");
-  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, FEW ? 128 : 64), FEW ? 1 : 2);
+  const long long grid = attn_deal(p, per_cu, ceil_div(p->Lk, 64), 2);
   if (plan_only) return SEGK_OK;
   kern<<<(unsigned)grid, ATTN_THREADS, lds, st>>>(*p);
   SEGK_CHECK_LAUNCH("attention_fwd");
@@ -646,27 +488,17 @@ static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
 }
 
 template <typename T>
-static int dispatch_fwd(AttnDev* p, bool few, bool plan_only, hipStream_t st) {
-  switch (attn_dp(p->D)) {
-    case 32: return few ? launch_fwd<T, 32, true>(p, plan_only, st) : launch_fwd<T, 32, false>(p, plan_only, st);
-    case 64: return few ? launch_fwd<T, 64, true>(p, plan_only, st) : launch_fwd<T, 64, false>(p, plan_only, st);
-    case 96:
-      if constexpr (sizeof(T) == 2)
-        if (few) return launch_fwd<T, 96, true>(p, plan_only, st);
-      return launch_fwd<T, 96, false>(p, plan_only, st);
-    default:
-      if constexpr (sizeof(T) == 2)
-        if (few) return launch_fwd<T, 128, true>(p, plan_only, st);
-      return launch_fwd<T, 128, false>(p, plan_only, st);
-  }
+static int dispatch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
+  if (p->D <= 32) return launch_fwd<T, 32>(p, plan_only, st);
+  if (p->D <= 64) return launch_fwd<T, 64>(p, plan_only, st);
+  if (p->D <= 96) return launch_fwd<T, 96>(p, plan_only, st);
+  return launch_fwd<T, 128>(p, plan_only, st);
 }
 
-// The deal of a forward pass, and the floats of its partial results.  Launches unless plan_only.
+// The deal of a forward pass.  Launches unless plan_only.
 static int run_fwd(AttnDev* p, int dtype, bool plan_only, hipStream_t st) {
-  const bool few = attn_few(*p, dtype);
-  return dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, few, plan_only, st) : dispatch_fwd<float>(p, few, plan_only, st);
+  return dtype == SEGK_BF16 ? dispatch_fwd<bf16_t>(p, plan_only, st) : dispatch_fwd<float>(p, plan_only, st);
 }
-static int fwd_tile_rows(const AttnDev& p, int dtype) { return attn_few(p, dtype) ? p.R : 128; }
 
 // Floats of the backward pass's workspace: row statistics, then the partial results of whichever pass is running.
 static int bwd_floats(AttnDev p, int dtype, long long* floats) {
@@ -680,7 +512,7 @@ static int bwd_floats(AttnDev p, int dtype, long long* floats) {
   if (p.dq && p.Lk > 0) {
     const int rc = attn_dq(&p, dtype, true, nullptr);
     if (rc != SEGK_OK) return rc;
-    const long long x = attn_part_floats(p, fwd_tile_rows(p, dtype), p.D);
+    const long long x = attn_part_floats(p, p.tile_rows, p.D);
     if (x > part) part = x;
   }
   *floats = stats + part;
@@ -700,7 +532,7 @@ extern "C" long long segk_attention_workspace(const segk_attention_args* a, int 
     rc = bwd_floats(p, a->dtype, &floats);
   } else {
     rc = run_fwd(&p, a->dtype, true, nullptr);
-    floats = attn_part_floats(p, fwd_tile_rows(p, a->dtype), p.D + 2);
+    floats = attn_part_floats(p, p.tile_rows, p.D + 2);
   }
   return rc != SEGK_OK ? rc : floats * 4;
 }
@@ -721,13 +553,12 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
   hipStream_t st = (hipStream_t)stream;
   rc = run_fwd(&p, a->dtype, true, st);
   if (rc != SEGK_OK) return rc;
-  const int tile_rows = fwd_tile_rows(p, a->dtype);
-  const long long floats = attn_part_floats(p, tile_rows, p.D + 2);
+  const long long floats = attn_part_floats(p, p.tile_rows, p.D + 2);
   if (floats > 0) {
     rc = take_workspace(a, floats * 4, "attention_fwd");
     if (rc != SEGK_OK) return rc;
     p.part = (float*)a->workspace;
-    p.part_ml = p.part + attn_part_floats(p, tile_rows, p.D);
+    p.part_ml = p.part + attn_part_floats(p, p.tile_rows, p.D);
   }
   rc = run_fwd(&p, a->dtype, false, st);
   if (rc != SEGK_OK || p.parts == 1) return rc;
@@ -735,8 +566,8 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
   int groups = 1;
   while (groups * 4 < p.parts && groups * lanes < ATTN_THREADS) groups *= 2;     // about four parts a thread
   const int lines = ATTN_THREADS / (lanes * groups);
-  const unsigned grid = (unsigned)ceil_div((long long)p.rest * tile_rows, lines);   // (rest is less than a round of workgroups)
-  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes, groups, tile_rows)));
+  const unsigned grid = (unsigned)ceil_div((long long)p.rest * p.tile_rows, lines);   // (rest is less than a round of workgroups)
+  SEGK_DISPATCH_DTYPE(a->dtype, T, (attn_join_kernel<T><<<grid, ATTN_THREADS, 0, st>>>(p, lanes, groups)));
   SEGK_CHECK_LAUNCH("attention_fwd join");
   return SEGK_OK;
 }
