@@ -1348,11 +1348,12 @@ def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
     key / value head h // (Hq // Hk)) -> [N, Lq, Hq, D].  Views are read in place when their channels are contiguous and
     their rows 16-byte aligned (slices of one projection's output are), copied otherwise.
       mask      bool, broadcastable to [N, Hq, Lq, Lk], True = open.  A closed pair has probability zero; its key and value
-                are still read and must be finite.
+                are still read and must be finite (so under causal).
       key_mask  bool [N, Lk], True = open (e.g. the pixels that are not padding).  A closed key is not read.
       causal    key j is open to token i for j <= i + Lk - Lq
       scale     of the scores, positive; default D ** -0.5
-    A query without an open key gives zeros, and no gradient.  Differentiable once with respect to q, k and v."""
+    A query without an open key gives zeros, and no gradient.  Sums are kept relative to a running reference that the
+    probabilities pass by up to 2^30: values beyond 1e25 may overflow.  Differentiable once with respect to q, k and v."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes [N, L, heads, D] tensors, got %s, %s, %s"
                          % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))

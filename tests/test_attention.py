@@ -369,6 +369,68 @@ def test_far_offsets():
     check(dict(zip(("out", "dq", "dk", "dv"), (out.detach(),) + grads)), res, tol, "far")
 
 
+# Sizes at which the work is dealt out in other ways: a last round of workgroups that is cut up (of queries, of keys; rounds
+# are 256 times 1 to 5 workgroups), parts of equal length under the diagonal, images dealt out in turns, groups of more heads
+# than a tile has rows, one token against a long cache.
+DEALT = [
+    (1, 600, 4100, 104, 104, 128, "", "plain"),
+    (1, 2100, 600, 104, 104, 128, "", "plain"),
+    (1, 600, 4100, 104, 104, 120, "pair", "plain"),
+    (1, 2100, 600, 104, 104, 128, "key", "plain"),
+    (1, 700, 1900, 8, 2, 64, "causal", "plain"),
+    (1, 1900, 700, 2, 2, 128, "causal", "heads_first"),
+    (8, 150, 300, 2, 1, 64, "causal key", "plain"),
+    (4, 300, 700, 8, 4, 64, "key", "fused"),
+    (6, 700, 300, 4, 4, 32, "key", "plain"),
+    (2, 150, 333, 4, 4, 128, "pair key", "plain"),
+    (1, 7, 200, 40, 1, 64, "", "plain"),
+    (2, 5, 130, 200, 2, 32, "causal key", "plain"),
+    (1, 1, 70001, 8, 2, 64, "key", "plain"),
+    (2, 2, 33333, 4, 4, 128, "causal", "tokens_first"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", DEALT, ids=[str(c) for c in DEALT])
+def test_ways_of_dealing_out(case, dt):
+    from segk import functional as SF
+    N, Lq, Lk, Hq, Hk, D, kind, layout = case
+    q, k, v, dout, gen = make(N, Lq, Lk, Hq, Hk, D, dt, layout, 31)
+    mask, key, causal = make_masks(kind, N, Hq, Lq, Lk, gen, "cuda")
+    res, tol = reference(q, k, v, dout, mask, key, causal, D ** -0.5, dt)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = SF.attention(*leaves, mask, key, causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    check(dict(zip(("out", "dq", "dk", "dv"), (out.detach(),) + grads)), res, tol, str(case))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls on two streams that run side by side, each with its own workspace, against the same calls one after the other."""
+    from segk import functional as SF
+    sets = []
+    for seed, (Lq, Lk, kind) in ((1, (2, 9000, "key")), (2, (500, 700, "causal"))):
+        q, k, v, dout, gen = make(2, Lq, Lk, 4, 2, 64, BF, "plain", seed)
+        mask, key, causal = make_masks(kind, 2, 4, Lq, Lk, gen, "cuda")
+        sets.append(([t.requires_grad_(True) for t in (q, k, v)], dout, key, causal))
+
+    def step(leaves, dout, key, causal):
+        out = SF.attention(*leaves, None, key, causal)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(8):
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(step(*s))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2])), i
+
+
 # ------------------------------------------------------------- refusals ----
 def _meta(*shape, dt=F32):
     return torch.zeros(*shape, dtype=dt)

@@ -145,6 +145,22 @@ def test_forward_and_gradients(case, dt):
             close(grads[2 + i], dw, tw, "weight gradient %d" % i)
 
 
+# Numbers of tokens at which a group of lanes takes one, some or all of a token's heads (10 and 23 of them).
+SHARES = [
+    (1, 500, 7, 3, 64, (16, 16), False, "int32", True, 1e-6),
+    (1, 3001, 7, 3, 96, (16, 16, 16), False, "int64", True, 1e-6),
+    (2, 6001, 7, 3, 64, (16, 16), True, "images", True, 1e-6),
+    (1, 1777, 20, 3, 128, (32, 32), False, "int32", True, 1e-6),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", SHARES, ids=[str(c) for c in SHARES])
+def test_shares_of_heads(case, dt):
+    test_forward_and_gradients(case, dt)
+
+
 @pytest.mark.gpu
 def test_default_sections_layouts_and_types():
     from segk import functional as SF
