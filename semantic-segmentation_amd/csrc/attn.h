@@ -183,6 +183,17 @@ __device__ __forceinline__ AttnFrag<float> pack_frag<float>(const f32x16& s, int
   return f;
 }
 
+// What pack_frag's rounding left over, as a second operand.
+__device__ __forceinline__ AttnFrag<bf16_t> pack_rest(const f32x16& s, int half, const AttnFrag<bf16_t>& f) {
+  f32x16 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = s[8 * half + 2 * j] - __uint_as_float(f.v[j] << 16);
+    x[2 * j + 1] = s[8 * half + 2 * j + 1] - __uint_as_float(f.v[j] & 0xffff0000u);
+  }
+  return pack_frag<bf16_t>(x, 0);
+}
+
 // 8 probabilities as an operand, and their sum added to `sum` (unrounded: lse is an fp32 statistic).
 template <typename T>
 __device__ __forceinline__ AttnFrag<T> pack_sum(const float* x, float& sum);

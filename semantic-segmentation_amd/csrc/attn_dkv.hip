@@ -259,6 +259,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_dkv_sum_kernel(const AttnDe
   const int key = w.tile * 128 + row, parts = attn_tile_parts(p, w.tile);
   if (key >= p.Lk || parts == 1) return;     // (a tile in one part is finished)
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int s = 0; s < parts; ++s) {
     const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (((long long)slot * p.parts + s) * 256 + (line & 255)) * p.D + d);
 #pragma unroll
