@@ -295,10 +295,11 @@ int segk_dot_partial_rows(long long M);
  *   s_j = scale * q_i . k_j over the open keys j,  out_i = sum_j softmax(s)_j v_j,  lse_i = log sum_j exp(s_j).
  * Key j is open to token i when mask and key_mask (bytes, non-zero = open; NULL = all) say so and, with causal != 0,
  * j <= i + Lk - Lq.  A row without an open key gives out = 0, lse = -inf and no gradient.  A key that key_mask closes is
- * not read; a pair that only `mask` closes has probability zero, its key and value are read.
+ * not read; a pair that only `mask` or `causal` closes has probability zero, its key and value are read.  Sums are kept
+ * relative to a reference that terms pass by up to 2^30: values beyond 1e25 may overflow.
  * Operands: [N][L][heads][D] by element strides with unit stride over D, 16-byte aligned, strides multiples of 16 bytes
  * (0: broadcast); D a multiple of 8 up to 128.  bf16 operands: fp32 scores, statistics and sums, probabilities rounded to
- * bf16 for their products; fp32 operands: exact-fp32 products throughout. */
+ * bf16 for their products (the score gradients of dq: as two bf16 operands); fp32 operands: exact-fp32 products. */
 typedef struct {
   void* p;
   long long n, l, h; /* elements between images, tokens, heads */

@@ -2,6 +2,8 @@
 //   dv_j = sum_i p_ij dout_i,   ds_ij = p_ij (dout_i . v_j - delta_i),   dk_j = scale sum_i ds_ij q_i.
 // A workgroup owns 128 keys and walks over the packed rows (tokens x heads of the group): shared heads add up in its
 // registers, nothing is added atomically, every sum has a fixed order.
+// bf16: P and dS are rounded to operands of their products, as the probabilities of the forward pass are: rms error against 64
+// bits 0.0023 of the gradient's size, 0.0017 of it the final rounding.
 #include <type_traits>
 
 #include "attn.h"
@@ -17,8 +19,14 @@ constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 // of dV^T = dO^T P and dK^T = Q^T dS as they lie.  K of the wavefront's keys stays in registers; Q and dO tiles of QT rows
 // are staged through LDS and read both along rows and along columns.
 // V lies in LDS, too: at 128 channels the registers it would take leave one wavefront to a SIMD instead of two, which cover
-// each other's exponentials (2.49 -> 1.13 ms at 4225 tokens, 32 heads over 8, bf16); at 64 channels 165 -> 159 us; at
+// each other's exponentials (2.49 -> 1.13 ms in the first case below); at 64 channels 165 -> 159 us (the second); at
 // 32 it costs 1.5 % (class queries, 47.7 -> 48.5 us), which is not worth a second form.
+// The bounds are what fits without spills (32 channels with 4 wavefronts to a SIMD instead of 3: 49 -> 64 us).
+// Matrix-bound on long maps: 4 images of 4225 tokens, 16 heads over 4 of 128 channels: 1.05 to 1.13 ms for four products,
+// 1060 TFLOP/s, matrix cores busy 56 % of the cycles.  16 images of 961 tokens under key masks, 16 heads of 64 channels:
+// 155 us; a third of the tiles is padding and ends at once, so that 1.4 of 2 wavefronts to a SIMD are there on average.  A
+// pipelined form (three blocks in flight, K and V in registers) took 155 us there, too, and 1.45 ms instead of 1.13 at 128
+// channels.
 // MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
 template <typename T, int DP, int MASKS>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {

@@ -9,6 +9,8 @@ Data flow (all intermediate activations pixel-major [pixels, channels], dtype = 
   UpsampleFunction pixel-major logits -> NCHW fp32 at input size                            (modeling/deeplab.py:252)
   CrossEntropyFunction fused log-softmax + NLL with ignore index                            (utils/loss.py:23-35)
   SyncBNFunction   stand-alone batch norm for the feeder's layers                           (sync_batchnorm/batchnorm.py:48-78)
+  attention, qk_norm_rotary  the many-headed attention of transformer heads over the same maps, and the norm and position
+                   rotation of its queries and keys ([N, L, heads, D] tensors)
 
 Every conv->BN->ReLU(->dropout) unit is: implicit-GEMM conv that also emits per-tile sum / sum-of-squares,
 a tiny reduce (+ all-reduce across ranks), coefficient kernel, one fused apply pass.  Backward mirrors it:
