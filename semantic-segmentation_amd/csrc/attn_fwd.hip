@@ -57,7 +57,8 @@ struct AttnRow {
 // the scores of block b + 1 and the values of block b - 1 on the matrix cores while the exponentials of block b run on the
 // vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
 // tiles; K runs one tile ahead of V.  The bounds are what fits without spills: 3 wavefronts to a SIMD where a row of a tile
-// has at most 128 bytes, 1 for fp32 heads over 96 channels, else 2.
+// has at most 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089 tokens, 8 heads of 96
+// channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.
 // Matrix-bound on long maps: 2 images of 16641 tokens, 8 heads over 2 of 128 channels, bf16: 2.01 ms, 1130 TFLOP/s (a large
 // library product reaches 1164 here); the matrix cores are busy 60 % of the cycles, at 1.8 GHz under this load.
 // 16 images of 1089 tokens, 16 heads of 64 channels: 100 us, 778 TFLOP/s: half as many products to an exponential.
@@ -65,7 +66,7 @@ struct AttnRow {
 // 2.4 TB/s.  Kernels that dealt the keys of a tile to the four wavefronts and joined them in LDS measured 6.7 us there, 24 us
 // against 23 for 21 class queries under masks, and 22 us against 19.5 in the gradient: not worth a second form.
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 512 ? 1 : DP * (int)sizeof(T) > 128 ? 2 : 3)) void attn_fwd_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384 : 512) ? 1 : DP * (int)sizeof(T) > 128 ? 2 : 3)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
