@@ -66,7 +66,8 @@ __device__ __forceinline__ int div_g(const AttnDev& p, int r) { return p.G == 1 
 // tiles is all rest.  The tiles of one problem stay on one XCD (blockIdx % 8 in launch order): they share keys and values
 // (rows, in the backward pass over keys) in its L2.  XCDs take runs of problems; under a key mask, whose images differ in
 // length, problems are dealt to them in turns where their number allows.  16 images of 961 keys, a third of them padding:
-// forward 90.5 -> 87, dq 108 -> 103 us; of equal images it costs 1.5 % (1089 tokens, 64 heads: 104.8 -> 106.2 us).
+// forward 90.5 -> 87, dq 108 -> 103 us; of equal images it costs 1.5 %
+// (16 of 1089 tokens, 16 heads of 64 channels: 104.8 -> 106.2 us).  Tiles in plain launch order: 107.4 and, padded, 93.
 struct AttnWork {
   int n, hk, tile;   // n < 0: nothing
   int part, parts;
