@@ -1326,9 +1326,11 @@ class AttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, key_mask, causal, scale):
         q, k, v = ops.attention_operand(q), ops.attention_operand(k), ops.attention_operand(v)
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, mask, key_mask)
-        ctx.how = (causal, scale)
+        want = any(ctx.needs_input_grad[:3])
+        lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=want)
+        if want:
+            ctx.save_for_backward(q, k, v, out, lse, mask, key_mask)
+            ctx.how = (causal, scale)
         return out
 
     @staticmethod
@@ -1360,12 +1362,9 @@ def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
         raise ValueError("attention takes [N, L, heads, D] tensors, got %s, %s, %s"
                          % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     scale = float(q.shape[3]) ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return AttentionFunction.apply(q, k, v, mask, key_mask, bool(causal), scale)
-    q, k, v = ops.attention_operand(q), ops.attention_operand(k), ops.attention_operand(v)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask)
-    return out
+    # (always through the Function, gradients wanted or not: torch.jit.trace records a Function, not a launch, and
+    # forward-mode differentiation is refused there)
+    return AttentionFunction.apply(q, k, v, mask, key_mask, bool(causal), scale)
 
 
 class QkNormRotaryFunction(torch.autograd.Function):
@@ -1374,9 +1373,10 @@ class QkNormRotaryFunction(torch.autograd.Function):
         q, k = ops.attention_operand(q), (None if k is None else ops.attention_operand(k))
         wq, wk = _fp32_weight(q_weight), _fp32_weight(k_weight)
         res = ops.qk_norm_rotary_fwd(q, k, wq, wk, positions, inv_freq, sections, eps, interleaved)
-        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
-        ctx.how = (sections, eps, interleaved)
-        ctx.weight_dtypes = (None if q_weight is None else q_weight.dtype, None if k_weight is None else k_weight.dtype)
+        if any(ctx.needs_input_grad[:4]):
+            ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
+            ctx.how = (sections, eps, interleaved)
+            ctx.weight_dtypes = (None if q_weight is None else q_weight.dtype, None if k_weight is None else k_weight.dtype)
         return res if k is not None else res[0]
 
     @staticmethod
@@ -1419,8 +1419,4 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None,
     for t, name in ((q, "q"), (k, "k")):
         if t is not None and t.dim() != 4:
             raise ValueError("%s must be [N, L, heads, D], got shape %s" % (name, tuple(t.shape)))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return QkNormRotaryFunction.apply(*tensors, *args)
-    res = ops.qk_norm_rotary_fwd(ops.attention_operand(q), None if k is None else ops.attention_operand(k),
-                                 _fp32_weight(q_weight), _fp32_weight(k_weight), *args)
-    return res if k is not None else res[0]
+    return QkNormRotaryFunction.apply(*tensors, *args)      # (always: see attention)
