@@ -372,6 +372,20 @@ __device__ __forceinline__ AttnFrag<float> load_frag<float>(const char* row, int
   return f;
 }
 
+// Zero, or NaN if one of the fragment's elements is not finite.
+__device__ __forceinline__ float probe_frag(const AttnFrag<bf16_t>& f) {
+  float x = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x = fmaf(__uint_as_float(f.v[e] << 16), 0.f, fmaf(__uint_as_float(f.v[e] & 0xffff0000u), 0.f, x));
+  return x;
+}
+__device__ __forceinline__ float probe_frag(const AttnFrag<float>& f) {
+  float x = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x = fmaf(f.v[e], 0.f, x);
+  return x;
+}
+
 // 4 consecutive channels of one row
 template <typename T>
 __device__ __forceinline__ void store4(char* row, int d, float a, float b, float c, float e);

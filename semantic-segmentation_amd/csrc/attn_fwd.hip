@@ -127,6 +127,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
   constexpr std::integral_constant<int, 1> one, yes;
 
   AttnRow<T, DB> row;
+  bool odd = false;          // the row's query is not finite
   f32x16 s[2];
   AttnFrag<T> pf[2][2];
 
@@ -194,6 +195,21 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
       tile_barrier();
       return;
     }
+    // A query that is not finite has a softmax of NaN over whatever keys are open to it.  Its scores do not tell (all -inf looks
+    // like a row without an open key; a closed key's -inf + query * 0 is NaN): it is taken as zeros, and its row becomes NaN
+    // below if it has met an open key.
+    {
+      float x = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) x += probe_frag(qf[ks]);
+      odd = !(pair_sum(x) == 0.f);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (unsigned e = 0; e < sizeof(qf[0].v) / sizeof(qf[0].v[0]); ++e) qf[ks].v[e] = odd ? 0 : qf[ks].v[e];
+      }
+    }
     scores(s[0], 0, 0, 0);
     block(t0 * KT, zero, yes, key_b, 0, no, 0);
     // The second block of tile u and the first of tile u + 1; two turns to a round of the loop, so that the buffers are
@@ -222,7 +238,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
     }
   }
 
-  const float lt = pair_sum(row.l);
+  float lt = pair_sum(row.l);
+  if (odd && lt != 0.f) lt = NAN;
   if (!row_ok) return;
   if (w.parts == 1) {
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
