@@ -866,25 +866,21 @@ def dot(a, b):
 
 
 # ------------------------------------------------------ multi-head attention ----
-def _launch_packed(name, args, t):
-    """call(name, packed arguments, stream) on the device of tensor t (a stream belongs to its device)."""
+def _launch_packed(name, args, t, sizing=None):
+    """call(name, packed arguments, stream) on the device of tensor t (a stream belongs to its device).  args end before the
+    workspace; sizing: the entry point that tells its bytes, and what follows its arguments (None: no workspace)."""
     index = t.get_device()
-    if index == torch.cuda.current_device():
-        call(name, args, _stream())
-    else:
+    if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            call(name, args, _stream())
+            return _launch_packed(name, args, t, sizing)
+    need = call(sizing[0], args + bytes(16), *sizing[1:]) if sizing else 0
+    ws = torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
+    call(name, args + WORKSPACE_ARGS.pack(ws.data_ptr() if need else 0, need), _stream())
 
 
 def _like(t):
     """A contiguous tensor of t's shape, type and device, unset."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
-def _with_workspace(args, need, t):
-    """(packed arguments with `need` bytes of workspace, the tensor that owns them)."""
-    ws = torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
-    return args + WORKSPACE_ARGS.pack(ws.data_ptr() if need else 0, need), ws
 
 
 def _attention_view(t, z=None):
@@ -975,8 +971,7 @@ def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, w
     if N == 0 or Lq == 0:
         return lse
     args = ATTENTION_ARGS.pack(*head, lse.data_ptr() if want_lse else 0, *masks, *_NO_VIEW, 0, 0, 0)
-    args, ws = _with_workspace(args, call("segk_attention_workspace", args + bytes(16), 0), q)
-    _launch_packed("segk_attention_fwd", args, q)
+    _launch_packed("segk_attention_fwd", args, q, ("segk_attention_workspace", 0))
     return lse
 
 
@@ -999,8 +994,7 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_m
         return dq, dk, dv
     args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), *masks, *_need_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
                                dk.data_ptr() if need_dkv else 0, dv.data_ptr() if need_dkv else 0)
-    args, ws = _with_workspace(args, call("segk_attention_workspace", args + bytes(16), 1), q)
-    _launch_packed("segk_attention_bwd", args, q)
+    _launch_packed("segk_attention_bwd", args, q, ("segk_attention_workspace", 1))
     return dq, dk, dv
 
 
@@ -1065,7 +1059,7 @@ def qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, sections=N
     if q.shape[0] > 0 and q.shape[1] > 0:
         args = QK_NORM_ROTARY_ARGS.pack(*head, q_out.data_ptr(), 0 if k is None else k_out.data_ptr(), *weights, *rest,
                                         *_NO_VIEW, *_NO_VIEW, 0, 0)
-        _launch_packed("segk_qk_norm_rotary", args + bytes(16), q)
+        _launch_packed("segk_qk_norm_rotary", args, q)
     return q_out, k_out
 
 
@@ -1089,9 +1083,7 @@ def qk_norm_rotary_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_
     args = QK_NORM_ROTARY_ARGS.pack(*head, dq.data_ptr(), 0 if k is None else dk.data_ptr(), *weights, *rest,
                                     *_need_view(dq_out, "dq"), *(_NO_VIEW if k is None else _need_view(dk_out, "dk")),
                                     0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr())
-    need = call("segk_qk_norm_rotary_bwd_workspace", args + bytes(16))
-    args, ws = _with_workspace(args, need, q)
-    _launch_packed("segk_qk_norm_rotary_bwd", args, q)
+    _launch_packed("segk_qk_norm_rotary_bwd", args, q, ("segk_qk_norm_rotary_bwd_workspace",))
     return dq, dk, dqw, dkw
 
 
