@@ -185,7 +185,6 @@ __device__ __forceinline__ AttnFrag<float> pack_frag<float>(const f32x16& s, int
 }
 
 // What pack_frag's rounding left over, as a second operand.
-__device__ __forceinline__ AttnFrag<float> pack_rest(const f32x16&, int, const AttnFrag<float>& f) { return f; }   // (not used)
 __device__ __forceinline__ AttnFrag<bf16_t> pack_rest(const f32x16& s, int half, const AttnFrag<bf16_t>& f) {
   f32x16 x;
 #pragma unroll

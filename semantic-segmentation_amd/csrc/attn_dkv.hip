@@ -28,8 +28,7 @@ constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 // pipelined form (three blocks in flight, K and V in registers) took 155 us there, too, and 1.45 ms instead of 1.13 at 128
 // channels.
 // MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
-// REST: P and dS as two operands each
-template <typename T, int DP, int MASKS, bool REST>
+template <typename T, int DP, int MASKS>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnPiece<T, DP> Piece;
@@ -205,13 +204,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP 
         const AttnFrag<T> pf = pack_frag<T>(s, j), sf = pack_frag<T>(dp, j);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const AttnFrag<T> gc = ln.cols(gt + (rb * 32 + j * 16) * Tile::PITCH, db), qc = ln.cols(qt + (rb * 32 + j * 16) * Tile::PITCH, db);
-          mma32(dv[db], gc, pf);
-          mma32(dk[db], qc, sf);
-          if constexpr (REST) {
-            mma32(dv[db], gc, pack_rest(s, j, pf));
-            mma32(dk[db], qc, pack_rest(dp, j, sf));
-          }
+          mma32(dv[db], ln.cols(gt + (rb * 32 + j * 16) * Tile::PITCH, db), pf);
+          mma32(dk[db], ln.cols(qt + (rb * 32 + j * 16) * Tile::PITCH, db), sf);
         }
       }
     }
@@ -288,14 +282,10 @@ template <typename T, int DP>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   constexpr int QT = dkv_rows<T, DP>();
   const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + 128 * AttnTile<T, DP>::PITCH;
-  static std::atomic<int> seen[2][3][ATTN_DEVICES];
+  static std::atomic<int> seen[3][ATTN_DEVICES];
   const int masks = p->mask ? 2 : p->kmask ? 1 : 0;
-  const bool rest = sizeof(T) == 2 && p->R <= 64;
-  auto kern = p->mask ? attn_dkv_kernel<T, DP, 2, false> : p->kmask ? attn_dkv_kernel<T, DP, 1, false> : attn_dkv_kernel<T, DP, 0, false>;
-  if constexpr (sizeof(T) == 2) {
-    if (rest) kern = p->mask ? attn_dkv_kernel<T, DP, 2, true> : p->kmask ? attn_dkv_kernel<T, DP, 1, true> : attn_dkv_kernel<T, DP, 0, true>;
-  }
-  const int per_cu = attn_occupancy((const void*)kern, lds, seen[rest][masks]);
+  auto kern = p->mask ? attn_dkv_kernel<T, DP, 2> : p->kmask ? attn_dkv_kernel<T, DP, 1> : attn_dkv_kernel<T, DP, 0>;
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masks]);
   if (per_cu < 0) return per_cu;
   p->tiles = ceil_div(p->Lk, 128);
   p->loop_rows = QT;
