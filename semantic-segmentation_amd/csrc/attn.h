@@ -38,6 +38,7 @@ struct AttnDev {
   AttnView q, k, v, o, dout;
   char *out, *dq, *dk, *dv;       // out: strides of `o`; gradients contiguous [N][L][heads][D]
   float* lse;                     // [N][Hq][Lq] natural log, or NULL
+  char* out_rest;                 // [N][Lq][Hq][D] what the rounding of out left over, or NULL
   const unsigned char* mask;      // element strides below; NULL = all open
   long long m_n, m_h, m_q, m_k;
   const unsigned char* kmask;     // [N][Lk]
@@ -54,7 +55,7 @@ struct AttnDev {
   int loop_rows;                  // what a tile's loop runs over: 0 keys by 64, else packed rows by this many
   int tile_rows;                  // rows of a tile that exist: 128, of a shorter problem all of it
   float* part;                    // partial results: [rest][parts][tile_rows][D] (keys: [rest][parts][dk, dv][128][D])
-  float* part_ml;                 // [rest][parts][tile_rows][2]: maxima and sums of the forward pass
+  float* part_ml;                 // [rest][parts][tile_rows][3]: maxima and both sums of the forward pass
   float *row_lse2, *minus_delta;    // [N][Hk][Rp]: log2-domain lse (+inf: no open key) and -rowsum(dout * out)
 };
 
@@ -219,6 +220,17 @@ __device__ __forceinline__ AttnFrag<float> pack_sum<float>(const float* x, float
     sum += x[j];
   }
   return f;
+}
+
+// The sum of an operand's 8 probabilities as rounded, added to `sum` (four two-term products with ones).
+__device__ __forceinline__ float sum_frag(const AttnFrag<bf16_t>& f, float sum) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned two = f.v[e];      // (a cast of f.v[e] itself takes element 0)
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+  }
+  return sum;
 }
 
 // ---- tiles in LDS -------------------------------------------------------------------------------
@@ -395,6 +407,19 @@ __device__ __forceinline__ void store4<bf16_t>(char* row, int d, float a, float 
 template <>
 __device__ __forceinline__ void store4<float>(char* row, int d, float a, float b, float c, float e) {
   *reinterpret_cast<f32x4*>(row + d * 4) = f32x4{a, b, c, e};
+}
+
+// out, 4 consecutive channels of one row (row, token and head give its place), and what its rounding left over
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnDev& p, int n, int tok, int head, int d, float a, float b, float c, float e) {
+  store4<T>(p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T), d, a, b, c, e);
+  if constexpr (sizeof(T) == 2) {
+    if (p.out_rest) {
+      const unsigned x = pack_bf16x2(a, b), y = pack_bf16x2(c, e);
+      store4<T>(p.out_rest + (((long long)n * p.Lq + tok) * p.Hq + head) * p.D * (int)sizeof(T), d, a - __uint_as_float(x << 16),
+                b - __uint_as_float(x & 0xffff0000u), c - __uint_as_float(y << 16), e - __uint_as_float(y & 0xffff0000u));
+    }
+  }
 }
 
 // ---- LDS-DMA ------------------------------------------------------------------------------------

@@ -14,15 +14,21 @@ namespace segk {
 //   neither overflows nor loses the largest terms.  m starts as the maximum of the first block that has an open key and is
 //   raised (accumulators rescaled) only when a block's sum passes 2^30, so that the common block needs no maximum.
 //   m = -inf makes the sum infinite or NaN, as do such scores: the raising path sorts those out, too.
-template <typename T, int DB>
+// Two sums: l of p, for lse (LSE: training), and in bf16 lr of p as rounded for its product, by which out is divided.  Out is then the exact
+// mean of v under weights off by their rounding; divided by l, the roundings of the few probabilities that carry a row would
+// not cancel in delta = rowsum(dout out), next to which ds is small.  rms error of dq, of its size, at scores of standard
+// deviation 1 / 3 / 5 / 8 (512 x 1024, 64 channels): divided by l, delta from out as rounded 0.0017 / 0.0027 / 0.0044 / 0.0054;
+// by lr, out's own rounding carried (out_rest) 0.0017 / 0.0018 / 0.0019 / 0.0019; the final rounding alone 0.0017.
+template <typename T, int DB, bool LSE>
 struct AttnRow {
+  static constexpr bool ROUNDED = sizeof(T) == 2, BOTH = ROUNDED && LSE;
   f32x16 o[DB];
-  float m, l;
-  __device__ __forceinline__ AttnRow() : m(-INFINITY), l(0.f) {
+  float m, l, lr;
+  __device__ __forceinline__ AttnRow() : m(-INFINITY), l(0.f), lr(0.f) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = zero16();
   }
-  // probabilities of a block as two operands; their sum
+  // probabilities of a block as two operands; their sum (the rounded ones' where it is the only one)
   __device__ __forceinline__ float weigh(const f32x16& s, float scale_log2, float ref, AttnFrag<T>* pf) const {
     float sum = 0.f;
 #pragma unroll
@@ -30,7 +36,13 @@ struct AttnRow {
       float e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[8 * j + i], scale_log2, -ref));
-      pf[j] = pack_sum<T>(e, sum);
+      if constexpr (ROUNDED && !LSE) {
+        float unused = 0.f;
+        pf[j] = pack_sum<T>(e, unused);
+        sum += sum_frag(pf[j], 0.f);
+      } else {
+        pf[j] = pack_sum<T>(e, sum);
+      }
     }
     return sum;
   }
@@ -45,28 +57,36 @@ struct AttnRow {
     const float alpha = exp2_fast(m - ms);
     m = nm;
     l *= alpha;
+    lr *= alpha;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
     return weigh(s, scale_log2, ms, pf);
   }
+  __device__ __forceinline__ void add(float sum, const AttnFrag<T>* pf) {
+    l += sum;
+    if constexpr (BOTH) lr += sum_frag(pf[0], 0.f) + sum_frag(pf[1], 0.f);
+  }
 };
 
 // Row tiles: 4 wavefronts of 32 rows, tiles of 64 keys shared through LDS.  A wavefront works on three blocks at a time:
 // the scores of block b + 1 and the values of block b - 1 on the matrix cores while the exponentials of block b run on the
 // vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
-// tiles; K runs one tile ahead of V.  The bounds are what fits without spills: 3 wavefronts to a SIMD where a row of a tile
-// has at most 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089 tokens, 8 heads of 96
-// channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.
-// Matrix-bound on long maps: 2 images of 16641 tokens, 8 heads over 2 of 128 channels, bf16: 2.01 ms, 1130 TFLOP/s (a large
-// library product reaches 1164 here); the matrix cores are busy 60 % of the cycles, at 1.8 GHz under this load.
-// 16 images of 1089 tokens, 16 heads of 64 channels: 100 us, 778 TFLOP/s: half as many products to an exponential.
+// tiles; K runs one tile ahead of V.  Wavefronts to a SIMD: 4 where a row of a tile has 64 bytes (class queries under masks, 32
+// channels: 22.3 us, with 3 26.5), 3 up to 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089
+// tokens, 8 heads of 96 channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.  At 32 and 64
+// channels under masks one register is spilled (64 channels, training, with 2 wavefronts and no spill: 115 us instead of 99).
+// Matrix-bound on long maps: 2 images of 16641 tokens, 8 heads over 2 of 128 channels, bf16: 2.06 to 2.12 ms, 1070 to 1100
+// TFLOP/s (a large library product reaches 1164 here); the matrix cores are busy 60 % of the cycles, at 1.8 GHz.
+// 16 images of 1089 tokens, 16 heads of 64 channels: 104 us, 747 TFLOP/s: half as many products to an exponential.
+// Training (LSE) costs the second sum and out_rest's 2 bytes an element: 16 images of 961 tokens under key masks, 16 heads of
+// 64 channels 87 -> 99 us (sum 4, out_rest 8), 4 images of 4225 tokens, 16 heads of 128 channels 551 -> 585 us (20 and 14).
 // Few rows (one token, class queries) take one tile, whose wavefronts without rows only stage: 16641 keys of 4 heads in 7 us,
 // 2.4 TB/s.  Kernels that dealt the keys of a tile to the four wavefronts and joined them in LDS measured 6.7 us there, 24 us
 // against 23 for 21 class queries under masks, and 22 us against 19.5 in the gradient: not worth a second form.
-template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384 : 512) ? 1 : DP * (int)sizeof(T) > 128 ? 2 : 3)) void attn_fwd_kernel(const AttnDev p) {
+template <typename T, int DP, bool MASKED, bool LSE>
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384 : 512) ? 1 : DP * (int)sizeof(T) > 128 ? 2 : DP * (int)sizeof(T) > 64 ? 3 : 4)) void attn_fwd_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   constexpr int KT = 64, KS = DP / 16, DB = DP / 32;
   constexpr int TILE_B = KT * Tile::PITCH;
@@ -126,7 +146,8 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
   constexpr std::integral_constant<int, 0> zero, no;
   constexpr std::integral_constant<int, 1> one, yes;
 
-  AttnRow<T, DB> row;
+  typedef AttnRow<T, DB, LSE> Row;
+  Row row;
   bool odd = false;          // the row's query is not finite
   f32x16 s[2];
   AttnFrag<T> pf[2][2];
@@ -160,7 +181,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
     pin(pf[odd][0]);
     pin(pf[odd][1]);
     if (__builtin_expect(!row.fine(sum), 0)) sum = row.raise(s[odd], p.scale_log2, pf[odd]);
-    row.l += sum;
+    row.add(sum, pf[odd]);
   };
   // at the barrier of turn u: K tile u + 1 and V tile u are here; every wavefront is done with K tile u and V tile u - 1
   auto stage = [&](int u, int here) __attribute__((always_inline)) {
@@ -238,23 +259,27 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
     }
   }
 
-  float lt = pair_sum(row.l);
-  if (odd && lt != 0.f) lt = NAN;
-  if (!row_ok) return;
+  float lt = pair_sum(row.l), lrt = Row::BOTH ? pair_sum(row.lr) : lt;
+  if (odd && lt != 0.f) lt = lrt = NAN;
+  // (the row's place is worked out again: carried through the loop it costs the registers that 64 channels under masks lack)
+  int out_row = l31;
+  asm volatile("" : "+v"(out_row));
+  out_row += row0;
+  if (out_row >= p.R) return;
+  const int out_tok = div_g(p, out_row), out_head = hk * p.G + out_row - out_tok * p.G;
   if (w.parts == 1) {
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    char* dst = p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T);
+    const float inv = lt == 0.f ? 0.f : 1.f / lrt;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int d = db * 32 + 2 * i + 4 * h;
-        if (d < p.D) store4<T>(dst, d, row.o[db][i] * inv, row.o[db][i + 1] * inv, row.o[db][i + 2] * inv, row.o[db][i + 3] * inv);
+        if (d < p.D) store_out<T>(p, n, out_tok, out_head, d, row.o[db][i] * inv, row.o[db][i + 1] * inv, row.o[db][i + 2] * inv, row.o[db][i + 3] * inv);
       }
-    if (p.lse && h == 0)
-      p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = lt == 0.f ? -INFINITY : (row.m + log2f(lt)) * 0.6931471805599453f;
+    if (LSE && p.lse && h == 0)
+      p.lse[((long long)n * p.Hq + out_head) * p.Lq + out_tok] = lt == 0.f ? -INFINITY : (row.m + log2f(lt)) * 0.6931471805599453f;
   } else {
-    const long long at = ((long long)w.slot * p.parts + w.part) * p.tile_rows + wave * 32 + l31;
+    const long long at = ((long long)w.slot * p.parts + w.part) * p.tile_rows + out_row - w.tile * 128;
     char* dst = (char*)(p.part + at * p.D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -264,8 +289,9 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
         if (d < p.D) store4<float>(dst, d, row.o[db][i], row.o[db][i + 1], row.o[db][i + 2], row.o[db][i + 3]);
       }
     if (h == 0) {
-      p.part_ml[2 * at] = row.m;
-      p.part_ml[2 * at + 1] = lt;
+      p.part_ml[3 * at] = row.m;
+      p.part_ml[3 * at + 1] = lt;
+      p.part_ml[3 * at + 2] = lrt;
     }
   }
 }
@@ -276,7 +302,7 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= (MASKED ? 384
 template <typename T>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p, int lanes, int groups) {
   __shared__ f32x4 so[ATTN_THREADS];
-  __shared__ float sl[ATTN_THREADS], sm[ATTN_THREADS];
+  __shared__ float sl[ATTN_THREADS], sr[ATTN_THREADS], sm[ATTN_THREADS];
   const int c = threadIdx.x % lanes, g = threadIdx.x / lanes % groups, in = threadIdx.x / (lanes * groups);
   const long long line = (long long)blockIdx.x * (ATTN_THREADS / (lanes * groups)) + in;
   const int slot = (int)(line / p.tile_rows), row = (int)(line - (long long)slot * p.tile_rows);
@@ -289,9 +315,9 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   const bool ok = parts > 1;       // (a tile in one part is finished)
   const long long first = ok ? (long long)slot * p.parts * p.tile_rows + row : 0;
   // every group looks at its own parts' maxima first, so that the sums are scaled once
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, lr = 0.f;
   if (ok)
-    for (int s = g; s < parts; s += groups) m = fmaxf(m, p.part_ml[2 * (first + (long long)s * p.tile_rows)]);
+    for (int s = g; s < parts; s += groups) m = fmaxf(m, p.part_ml[3 * (first + (long long)s * p.tile_rows)]);
   sm[threadIdx.x] = m;
   __syncthreads();
   for (int i = 0; i < groups; ++i) m = fmaxf(m, sm[(in * groups + i) * lanes + c]);
@@ -300,8 +326,9 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   if (ok)
     for (int s = g; s < parts; s += groups) {
       const long long at = first + (long long)s * p.tile_rows;
-      const float a = exp2_fast(p.part_ml[2 * at] - ms);
-      l = fmaf(p.part_ml[2 * at + 1], a, l);
+      const float a = exp2_fast(p.part_ml[3 * at] - ms);
+      l = fmaf(p.part_ml[3 * at + 1], a, l);
+      lr = fmaf(p.part_ml[3 * at + 2], a, lr);
       if (c * 4 < p.D) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * p.D + c * 4);
 #pragma unroll
@@ -310,6 +337,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
     }
   so[threadIdx.x] = o;
   sl[threadIdx.x] = l;
+  sr[threadIdx.x] = lr;
   __syncthreads();
   if (!ok || g != 0 || c * 4 >= p.D) return;
   const int rr = w.tile * 128 + row;
@@ -319,20 +347,19 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e];
     l += sl[threadIdx.x + i * lanes];
+    lr += sr[threadIdx.x + i * lanes];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / lr;
   const int n = w.n, tok = div_g(p, rr), head = w.hk * p.G + rr - tok * p.G;
-  store4<T>(p.out + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T), c * 4, o[0] * inv, o[1] * inv,
-            o[2] * inv, o[3] * inv);
+  store_out<T>(p, n, tok, head, c * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
   if (p.lse && c == 0)
     p.lse[((long long)n * p.Hq + head) * p.Lq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // Row statistics of the backward pass in packed row order: -rowsum(dout * out) and the base-2 lse (+inf where a row has no
 // open key and in the padding: its probabilities then come out as zeros).  D / 8 lanes (rounded up to a power of two)
-// share a row.  `out` is taken as rounded for the caller: the rounding it brings to delta is an rms error of 0.0002 to 0.0004
-// of dq's size, against 0.0017 of dq's own rounding (bf16); an exact copy of out would cost 4 bytes an element to write and
-// to read.  Memory-bound: 16 images of 961 tokens, 16 heads of 64 channels 13.7 us, 4.6 TB/s.
+// share a row.  bf16: out with what its rounding left over (see AttnRow); without that, as rounded for the caller.
+// Memory-bound: 16 images of 961 tokens, 16 heads of 64 channels 17 us, 5.5 TB/s (14 us without out_rest).
 template <typename T>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_row_stats_kernel(const AttnDev p, int lanes) {
   const int per = ATTN_THREADS / lanes;
@@ -346,17 +373,20 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_row_stats_kernel(const Attn
   float sum = 0.f, lse = INFINITY;
   if (rr < p.R) {
     const int tok = div_g(p, rr), head = hk * p.G + rr - tok * p.G;
-    const float x = p.lse[((long long)n * p.Hq + head) * p.Lq + tok];
-    lse = x == -INFINITY ? INFINITY : x * LOG2E;
+    const float ln = p.lse[((long long)n * p.Hq + head) * p.Lq + tok];
+    lse = ln == -INFINITY ? INFINITY : ln * LOG2E;
     // (a row without an open key has no gradient, whatever arrives for it: its dout is not looked at)
-    if (c * 8 < p.D && x != -INFINITY) {
+    if (c * 8 < p.D && ln != -INFINITY) {
       const AttnFrag<T> a = load_frag<T>(p.o.p + ((long long)n * p.o.n + (long long)tok * p.o.l + (long long)head * p.o.h) * (int)sizeof(T), c >> 1, c & 1, p.D, true);
+      AttnFrag<T> x = {};
+      if (sizeof(T) == 2 && p.out_rest)
+        x = load_frag<T>(p.out_rest + (((long long)n * p.Lq + tok) * p.Hq + head) * p.D * (int)sizeof(T), c >> 1, c & 1, p.D, true);
       const AttnFrag<T> b = load_frag<T>(p.dout.p + ((long long)n * p.dout.n + (long long)tok * p.dout.l + (long long)head * p.dout.h) * (int)sizeof(T), c >> 1, c & 1, p.D, true);
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sum = fmaf(__uint_as_float(a.v[e] << 16), __uint_as_float(b.v[e] << 16), sum);
-          sum = fmaf(__uint_as_float(a.v[e] & 0xffff0000u), __uint_as_float(b.v[e] & 0xffff0000u), sum);
+          sum = fmaf(__uint_as_float(a.v[e] << 16) + __uint_as_float(x.v[e] << 16), __uint_as_float(b.v[e] << 16), sum);
+          sum = fmaf(__uint_as_float(a.v[e] & 0xffff0000u) + __uint_as_float(x.v[e] & 0xffff0000u), __uint_as_float(b.v[e] & 0xffff0000u), sum);
         }
       } else {
 #pragma unroll
@@ -471,6 +501,9 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
   p->dout = {nullptr, 0, 0, 0};
   p->out = (char*)a->out.p;
   p->lse = a->lse;
+  SEGK_REQUIRE(!a->out_rest || (a->dtype == SEGK_BF16 && ((uintptr_t)a->out_rest & 15) == 0),
+               "attention: out_rest belongs to bf16 operands and must be 16-byte aligned");
+  p->out_rest = (char*)a->out_rest;
   p->mask = (const unsigned char*)a->mask;
   p->m_n = a->mask_n, p->m_h = a->mask_h, p->m_q = a->mask_q, p->m_k = a->mask_k;
   p->kmask = (const unsigned char*)a->key_mask;
@@ -502,11 +535,14 @@ int attn_check(const segk_attention_args* a, AttnDev* p, bool backward) {
 
 template <typename T, int DP>
 static int launch_fwd(AttnDev* p, bool plan_only, hipStream_t st) {
-  static std::atomic<int> seen[2][ATTN_DEVICES];
-  const bool masked = p->mask || p->kmask;
+  static std::atomic<int> seen[2][2][ATTN_DEVICES];
+  const bool masked = p->mask || p->kmask, lse = sizeof(T) == 4 || p->lse;     // (fp32: one form)
   const int lds = 4 * 64 * AttnTile<T, DP>::PITCH + (masked ? 512 : 0);
-  void (*const kern)(const AttnDev) = masked ? attn_fwd_kernel<T, DP, true> : attn_fwd_kernel<T, DP, false>;
-  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked]);
+  void (*kern)(const AttnDev) = masked ? attn_fwd_kernel<T, DP, true, true> : attn_fwd_kernel<T, DP, false, true>;
+  if constexpr (sizeof(T) == 2) {
+    if (!lse) kern = masked ? attn_fwd_kernel<T, DP, true, false> : attn_fwd_kernel<T, DP, false, false>;
+  }
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masked][lse]);
   if (per_cu < 0) return per_cu;
   p->tiles = ceil_div(p->R, 128);
   SEGK_UNSUPPORTED((long long)p->tiles * p->N * p->Hk < 0x40000000LL, "attention: too many workgroups");
@@ -562,7 +598,7 @@ extern "C" long long segk_attention_workspace(const segk_attention_args* a, int 
     rc = bwd_floats(p, a->dtype, &floats);
   } else {
     rc = run_fwd(&p, a->dtype, true, nullptr);
-    floats = attn_part_floats(p, p.tile_rows, p.D + 2);
+    floats = attn_part_floats(p, p.tile_rows, p.D + 3);
   }
   return rc != SEGK_OK ? rc : floats * 4;
 }
@@ -583,7 +619,7 @@ extern "C" int segk_attention_fwd(const segk_attention_args* a, segk_stream_t st
   hipStream_t st = (hipStream_t)stream;
   rc = run_fwd(&p, a->dtype, true, st);
   if (rc != SEGK_OK) return rc;
-  const long long floats = attn_part_floats(p, p.tile_rows, p.D + 2);
+  const long long floats = attn_part_floats(p, p.tile_rows, p.D + 3);
   if (floats > 0) {
     rc = take_workspace(a, floats * 4, "attention_fwd");
     if (rc != SEGK_OK) return rc;

@@ -66,7 +66,7 @@ class GemmTnArgs(ctypes.Structure):
 
 # segk_attention_args and segk_qk_norm_rotary_args, packed in one go (native alignment; a view is pointer and 3 strides);
 # the workspace pointer and its size are the last two fields of both.
-ATTENTION_ARGS = struct.Struct("@8if" + "P3q" * 4 + "PP4qP2q" + "P3q" + "3P")
+ATTENTION_ARGS = struct.Struct("@8if" + "P3q" * 4 + "3P4qP2q" + "P3q" + "3P")
 QK_NORM_ROTARY_ARGS = struct.Struct("@6i" + "P3q" * 2 + "5Pi3q5iP2if" + "P3q" * 2 + "2P")
 WORKSPACE_ARGS = struct.Struct("@Pq")
 

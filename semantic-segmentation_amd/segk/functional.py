@@ -1327,20 +1327,21 @@ class AttentionFunction(torch.autograd.Function):
         q, k, v = ops.attention_operand(q), ops.attention_operand(k), ops.attention_operand(v)
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         want = any(ctx.needs_input_grad[:3])
-        lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=want)
+        rest = torch.empty_like(out) if want and out.dtype is torch.bfloat16 else None
+        lse = ops.attention_fwd(q, k, v, out, scale, causal, mask, key_mask, want_lse=want, out_rest=rest)
         if want:
-            ctx.save_for_backward(q, k, v, out, lse, mask, key_mask)
+            ctx.save_for_backward(q, k, v, out, lse, mask, key_mask, rest)
             ctx.how = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, out, lse, mask, key_mask = ctx.saved_tensors
+        q, k, v, out, lse, mask, key_mask, rest = ctx.saved_tensors
         causal, scale = ctx.how
         need = ctx.needs_input_grad
         dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, ops.attention_operand(g), scale, causal, mask, key_mask,
-                                       need_dq=need[0], need_dkv=need[1] or need[2])
+                                       need_dq=need[0], need_dkv=need[1] or need[2], out_rest=rest)
         return dq, (dk if need[1] else None), (dv if need[2] else None), None, None, None, None
 
 

@@ -960,24 +960,40 @@ def _attention_args(q, k, v, out, scale, causal, mask, key_mask):
     return head + _need_view(out, "out", zq), m + km
 
 
-def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, want_lse=False):
+def _out_rest(out_rest, out):
+    if out_rest is None:
+        return 0
+    if out.dtype is not torch.bfloat16:
+        raise ValueError("out_rest belongs to bfloat16 operands")
+    _same_kind(out.get_device(), out.dtype, out_rest, "out_rest")
+    if out_rest.shape != out.shape or not out_rest.is_contiguous():
+        raise ValueError("out_rest must be contiguous %s, got %s" % (tuple(out.shape), tuple(out_rest.shape)))
+    return out_rest.data_ptr()
+
+
+def attention_fwd(q, k, v, out, scale, causal=False, mask=None, key_mask=None, want_lse=False, out_rest=None):
     """out = softmax(scale * q k^T) v per head.  q, out: [N, Lq, Hq, D]; k, v: [N, Lk, Hk, D], query head h reads head
     h // (Hq // Hk); any strides with unit stride over D and 16-byte aligned rows; D a multiple of 8 up to 128.
     mask: bool, broadcastable to [N, Hq, Lq, Lk], True = open; key_mask: bool [N, Lk]; causal: key j is open to token i
-    for j <= i + Lk - Lq.  -> lse [N, Hq, Lq] float32 (None unless wanted)."""
+    for j <= i + Lk - Lq.  out_rest: bfloat16 like out, contiguous, gets what out's rounding left over, for attention_bwd.
+    -> lse [N, Hq, Lq] float32 (None unless wanted)."""
     head, masks = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
+    rest = _out_rest(out_rest, out)
     N, Lq, Hq = head[0], head[1], head[3]
     lse = torch.empty((N, Hq, Lq), dtype=torch.float32, device=q.device) if want_lse else None
     if N == 0 or Lq == 0:
         return lse
-    args = ATTENTION_ARGS.pack(*head, lse.data_ptr() if want_lse else 0, *masks, *_NO_VIEW, 0, 0, 0)
+    args = ATTENTION_ARGS.pack(*head, lse.data_ptr() if want_lse else 0, rest, *masks, *_NO_VIEW, 0, 0, 0)
     _launch_packed("segk_attention_fwd", args, q, ("segk_attention_workspace", 0))
     return lse
 
 
-def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_mask=None, need_dq=True, need_dkv=True):
-    """Gradients (dq, dk, dv) of attention_fwd, contiguous, of the operands' dtype; None where not wanted."""
+def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_mask=None, need_dq=True, need_dkv=True,
+                  out_rest=None):
+    """Gradients (dq, dk, dv) of attention_fwd, contiguous, of the operands' dtype; None where not wanted.  out_rest: as the
+    forward pass left it, or None, at some cost in accuracy where few keys carry a row (include/segk.h)."""
     head, masks = _attention_args(q, k, v, out, scale, causal, mask, key_mask)
+    rest = _out_rest(out_rest, out)
     N, Lq, Lk, Hq = head[:4]
     index = q.get_device()
     _same_kind(index, q.dtype, dout, "dout")
@@ -992,7 +1008,7 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=False, mask=None, key_m
     dv = new(k) if need_dkv else None
     if not some or not (need_dq or need_dkv):
         return dq, dk, dv
-    args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), *masks, *_need_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
+    args = ATTENTION_ARGS.pack(*head, lse.data_ptr(), rest, *masks, *_need_view(dout, "dout"), dq.data_ptr() if need_dq else 0,
                                dk.data_ptr() if need_dkv else 0, dv.data_ptr() if need_dkv else 0)
     _launch_packed("segk_attention_bwd", args, q, ("segk_attention_workspace", 1))
     return dq, dk, dv
