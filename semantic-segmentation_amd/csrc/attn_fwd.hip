@@ -1,5 +1,6 @@
-// Multi-head attention, forward: out = softmax(scale q k^T) v per head in one pass over the keys, with a running maximum
-// and sum per row (fp32, base-2 exponents), and the host side of the attention entry points.
+// Multi-head attention, forward: out = softmax(scale q k^T) v per head in one pass over the keys, with a running reference
+// and sums per row (fp32, base-2 exponents), and the host side of the attention entry points.
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -11,12 +12,15 @@ namespace segk {
 // Scores are computed transposed (S^T = K Q^T, a lane owns one query), so the running statistics are one
 // register and S^T is the operand of O^T = V^T P^T as it lies (attn.h).  Keys in blocks of 32.
 //   p = exp2(s scale log2(e) - m) for a reference m that need not be the maximum: in floating point any m serves that
-//   neither overflows nor loses the largest terms.  m starts as the maximum of the first block that has an open key and is
-//   raised (accumulators rescaled) only when a block's sum passes 2^30, so that the common block needs no maximum.
-//   m = -inf makes the sum infinite or NaN, as do such scores: the raising path sorts those out, too.
-// Two sums: l of p, for lse (LSE: training), and in bf16 lr of p as rounded for its product, by which out is divided.  Out is then the exact
-// mean of v under weights off by their rounding; divided by l, the roundings of the few probabilities that carry a row would
-// not cancel in delta = rowsum(dout out), next to which ds is small.  rms error of dq, of its size, at scores of standard
+//   neither overflows nor loses the largest terms.  m starts as the lowest finite number, to which closed scores (-inf) still
+//   add nothing and any score adds infinity, and is raised to a block's maximum (accumulators rescaled) only when a block's
+//   sum passes 2^30: at the first open key, then hardly ever, so that the common block needs no maximum and a row without open
+//   keys none at all.  (m = -inf would raise all of a wavefront's rows in every block until each has met an open key: 21 class
+//   queries, one in ten of them empty, 16 images of 4225 keys 22.6 us instead of 20.2, 4 images of 16641 keys 25.2 and 21.4.)
+//   Scores of +inf and NaN end up there, too.
+// Two sums: l of p, for lse (LSE: training), and in bf16 lr of p as rounded for its product, by which out is divided.  Out is
+// then the exact mean of v under weights off by their rounding; divided by l, the roundings of the few probabilities that carry
+// a row would not cancel in delta = rowsum(dout out), next to which ds is small.  rms error of dq, of its size, at scores of standard
 // deviation 1 / 3 / 5 / 8 (512 x 1024, 64 channels): divided by l, delta from out as rounded 0.0017 / 0.0027 / 0.0044 / 0.0054;
 // by lr, out's own rounding carried (out_rest) 0.0017 / 0.0018 / 0.0019 / 0.0019; the final rounding alone 0.0017.
 template <typename T, int DB, bool LSE>
@@ -24,7 +28,7 @@ struct AttnRow {
   static constexpr bool ROUNDED = sizeof(T) == 2, BOTH = ROUNDED && LSE;
   f32x16 o[DB];
   float m, l, lr;
-  __device__ __forceinline__ AttnRow() : m(-INFINITY), l(0.f), lr(0.f) {
+  __device__ __forceinline__ AttnRow() : m(-FLT_MAX), l(0.f), lr(0.f) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = zero16();
   }
@@ -53,8 +57,7 @@ struct AttnRow {
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
     const float nm = fmaxf(m, pair_max(mx) * scale_log2);
-    const float ms = nm == -INFINITY ? 0.f : nm;
-    const float alpha = exp2_fast(m - ms);
+    const float alpha = exp2_fast(m - nm);
     m = nm;
     l *= alpha;
     lr *= alpha;
@@ -62,7 +65,7 @@ struct AttnRow {
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-    return weigh(s, scale_log2, ms, pf);
+    return weigh(s, scale_log2, nm, pf);
   }
   __device__ __forceinline__ void add(float sum, const AttnFrag<T>* pf) {
     l += sum;
@@ -74,7 +77,7 @@ struct AttnRow {
 // the scores of block b + 1 and the values of block b - 1 on the matrix cores while the exponentials of block b run on the
 // vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
 // tiles; K runs one tile ahead of V.  Wavefronts to a SIMD: 4 where a row of a tile has 64 bytes (class queries under masks, 32
-// channels: 22.3 us, with 3 26.5), 3 up to 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089
+// channels: 26.5 -> 22.3 us against 3, 20.2 now), 3 up to 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089
 // tokens, 8 heads of 96 channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.  At 32 and 64
 // channels under masks one register is spilled (64 channels, training, with 2 wavefronts and no spill: 115 us instead of 99).
 // Matrix-bound on long maps: 2 images of 16641 tokens, 8 heads over 2 of 128 channels, bf16: 2.06 to 2.12 ms, 1070 to 1100
@@ -321,12 +324,11 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnDev p
   sm[threadIdx.x] = m;
   __syncthreads();
   for (int i = 0; i < groups; ++i) m = fmaxf(m, sm[(in * groups + i) * lanes + c]);
-  const float ms = m == -INFINITY ? 0.f : m;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (ok)
     for (int s = g; s < parts; s += groups) {
       const long long at = first + (long long)s * p.tile_rows;
-      const float a = exp2_fast(p.part_ml[3 * at] - ms);
+      const float a = exp2_fast(p.part_ml[3 * at] - m);
       l = fmaf(p.part_ml[3 * at + 1], a, l);
       lr = fmaf(p.part_ml[3 * at + 2], a, lr);
       if (c * 4 < p.D) {

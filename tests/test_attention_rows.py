@@ -85,3 +85,39 @@ def test_queries_that_are_not_finite_stay_visible(dt, masked, lk):
             assert torch.isnan(out[0, t, h]).all() and torch.isnan(lse[0, h, t])
             out[0, t, h] = want[0, t, h]
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("lk", [500, 9000])
+def test_an_empty_row_does_not_change_its_neighbours(dt, lk):
+    """Not by a bit: a row without an open key needs no new reference for its exponents, which the rows beside it would share."""
+    from segk import functional as SF
+    q, k, v, _, gen = make(1, 40, lk, 1, 1, 64, dt, "plain", 47)
+    mask = torch.rand(1, 1, 40, lk, generator=gen).cuda() < 0.9
+    mask[..., 0] = True
+    want = SF.attention(q, k, v, mask)
+    for row in (0, 7, 39):
+        less = mask.clone()
+        less[0, 0, row] = False
+        got = SF.attention(q, k, v, less)
+        assert not got[0, row].any()
+        got[0, row] = want[0, row]
+        same = torch.equal(got, want)
+        assert same
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("lk", [1, 70, 5000])
+def test_scores_far_below_zero(dt, lk):
+    """-1e30 and less, where one key lies so far above the others that the result is its value."""
+    from segk import functional as SF
+    _, _, v, _, _ = make(1, 33, lk, 1, 1, 32, dt, "plain", 53)
+    for top in (0, lk // 2, lk - 1):
+        q = torch.full((1, 33, 1, 32), 2.0 ** 50, device="cuda", dtype=dt)
+        k = torch.full((1, lk, 1, 32), -2.0 ** 52, device="cuda", dtype=dt)
+        k[0, top] = -2.0 ** 51
+        out = SF.attention(q, k, v, scale=1.0)
+        same = torch.equal(out, v[:, top:top + 1].expand_as(out))
+        assert same
