@@ -75,8 +75,10 @@ struct AttnWork {
   int slot;          // number among the tiles that are cut
 };
 __device__ __forceinline__ void attn_decode(const AttnDev& p, int problem, int tile, AttnWork* w) {
-  // (under the diagonal the last tiles are the longest: they start first)
-  w->tile = p.causal ? p.tiles - 1 - tile : tile;
+  // Under the diagonal the longest tiles start first, of rows the last ones, of keys the first: keys of 2 images of 4225 tokens,
+  // 16 heads of 64 channels 242 -> 202 us, 8 images, 8 heads over 4 of 128 channels 779 -> 730 us against the other order.  (Cut into
+  // equal parts they take the same time either way.)
+  w->tile = p.causal && !p.loop_rows ? p.tiles - 1 - tile : tile;
   w->hk = problem % p.Hk;
   w->n = problem / p.Hk;
 }
