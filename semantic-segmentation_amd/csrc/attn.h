@@ -74,11 +74,15 @@ struct AttnWork {
   int part, parts;
   int slot;          // number among the tiles that are cut
 };
-__device__ __forceinline__ void attn_decode(const AttnDev& p, int problem, int tile, AttnWork* w) {
+// Tile number `tile` of a problem in launch order.
+__device__ __forceinline__ int attn_tile(const AttnDev& p, int tile) {
   // Under the diagonal the longest tiles start first, of rows the last ones, of keys the first: keys of 2 images of 4225 tokens,
-  // 16 heads of 64 channels 242 -> 202 us, 8 images, 8 heads over 4 of 128 channels 779 -> 730 us against the other order.  (Cut into
-  // equal parts they take the same time either way.)
-  w->tile = p.causal && !p.loop_rows ? p.tiles - 1 - tile : tile;
+  // 16 heads of 64 channels 242 -> 202 us, 8 images, 8 heads over 4 of 128 channels 779 -> 730 us against the other order.
+  // (Cut into equal parts they take the same time either way.)
+  return p.causal && !p.loop_rows ? p.tiles - 1 - tile : tile;
+}
+__device__ __forceinline__ void attn_decode(const AttnDev& p, int problem, int tile, AttnWork* w) {
+  w->tile = attn_tile(p, tile);
   w->hk = problem % p.Hk;
   w->n = problem / p.Hk;
 }
@@ -117,19 +121,32 @@ __device__ __forceinline__ AttnWork attn_work(const AttnDev& p) {
     return w;
   }
   int u = x * p.rest_x + i - whole_x;
-  if (p.even_steps) {          // few tiles of different lengths: every part has about as many steps
+  if (p.even_steps) {          // tiles of different lengths: every part has about as many steps
     const int head = u / p.even_units;
     if (head >= p.N * p.Hk) return w;
     u -= head * p.even_units;
-    for (int t = 0; t < p.tiles; ++t) {
-      attn_decode_tile(p, head * p.tiles + t, &w);
-      w.parts = attn_tile_parts(p, w.tile);
-      w.slot = head * p.tiles + t;
-      w.part = u;
-      if (u < w.parts) return w;
-      u -= w.parts;
+    // Lane t counts the parts of tile t; the tile of part u is the first whose running sum passes it.  (One tile after the
+    // other: 0.3 us a tile, 1 image of 2048 tokens, 8 heads over 2 of 64 channels 36 us instead of 18.)
+    const int lane = (int)threadIdx.x & 63;
+    for (int t0 = 0; t0 < p.tiles; t0 += 64) {
+      const int mine = t0 + lane < p.tiles ? attn_tile_parts(p, attn_tile(p, t0 + lane)) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const int x = __shfl_up(sum, o, 64);
+        sum += lane >= o ? x : 0;
+      }
+      const int all = __builtin_amdgcn_readlane(sum, 63);
+      if (u < all) {
+        const int t = __builtin_ctzll(__ballot(sum > u));
+        w.parts = __builtin_amdgcn_readlane(mine, t);
+        w.part = u - __builtin_amdgcn_readlane(sum, t) + w.parts;
+        w.slot = head * p.tiles + t0 + t;
+        attn_decode_tile(p, w.slot, &w);
+        return w;
+      }
+      u -= all;
     }
-    w.n = -1;
     return w;
   }
   if (u >= p.rest * p.parts) return w;

@@ -408,10 +408,15 @@ long long attn_deal(AttnDev* p, int per_cu, int steps, int min_steps) {
   const long long all = (long long)p->tiles * p->N * p->Hk;
   const long long round = 256LL * per_cu;      // workgroups that run at once
   p->even_steps = p->even_units = 0;
-  if (p->causal && p->tiles > 1 && all < round && p->tiles <= 64) {
-    // Few tiles of different lengths: parts of equal length, a round of them.  fp32, 2 images of 1089 tokens, 8 heads of 64
-    // channels: forward 51 -> 46 us, keys 89 -> 78, queries 72 -> 55 against equal numbers of parts.  Parts of half the
-    // length gain 5 us in the forward kernel and lose them in the join; parts of twice the length take 59, 98 and 81 us.
+  if (p->causal && p->tiles > 1 && all < round) {
+    // Fewer tiles than a round, of different lengths: parts of equal length, a round of them.  Against equal numbers of parts:
+    // fp32, 2 images of 1089 tokens, 8 heads of 64 channels: forward 51.8 -> 50.8 us, keys 92 -> 71, queries 73 -> 55; bf16, one
+    // image: 2048 tokens, 8 heads over 2 of 64 channels 20.1 -> 18.4, 29.2 -> 25.9, 25.0 -> 20.3; 16641 tokens, 2 heads of 64
+    // channels 147 -> 116, 290 -> 220, 238 -> 179 (and 4 us more to join); 4225 tokens, 8 heads over 2 of 128 channels (264 tiles
+    // of 512: equal numbers leave one part) 107 -> 66, 142 -> 138, 174 -> 100.  It loses a little where equal numbers fill the
+    // round just so: 4096 tokens, 8 heads over 2 of 64 channels 34 -> 40, 72 -> 68, 52 -> 51.
+    // Parts of half the length gain 5 us in the first forward kernel and lose them in the join; parts of twice the length take 59,
+    // 98 and 81 us there.
     long long sum = 0;
     for (int t = 0; t < p->tiles; ++t) sum += attn_causal_steps(*p, t);
     long long per = (sum * p->N * p->Hk + round - 1) / round;

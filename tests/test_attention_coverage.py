@@ -167,6 +167,8 @@ KEYS = [
     (8, 150, 300, 2, 1, 64, "causal key"),
     (4, 300, 700, 8, 4, 64, "key"),
     (2, 1089, 1089, 4, 4, 64, "causal"),
+    (1, 1500, 1500, 8, 1, 64, "causal"),       # 94 tiles of rows
+    (1, 40, 9000, 2, 2, 32, "causal"),         # 71 tiles of keys
 ]
 ROWS = [
     (1, 1, 70, 1, 1, 8, ""),
@@ -181,6 +183,9 @@ ROWS = [
     (6, 700, 300, 4, 4, 32, "key"),
     (2, 300, 70, 6, 2, 40, "causal"),
     (2, 1089, 1089, 4, 4, 64, "causal"),
+    (1, 1500, 1500, 8, 1, 64, "causal"),
+    (1, 40, 9000, 2, 2, 32, "causal"),
+    (1, 9000, 40, 2, 2, 32, "causal"),
 ]
 
 
