@@ -21,7 +21,11 @@ constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 // V lies in LDS, too: at 128 channels the registers it would take leave one wavefront to a SIMD instead of two, which cover
 // each other's exponentials (2.49 -> 1.13 ms in the first case below); at 64 channels 165 -> 159 us (the second); at
 // 32 it costs 1.5 % (class queries, 47.7 -> 48.5 us), which is not worth a second form.
-// The bounds are what fits without spills (32 channels with 4 wavefronts to a SIMD instead of 3: 49 -> 64 us).
+// Wavefronts to a SIMD: what is fastest.  Registers spilled: 4 with a pair mask at 32 channels (3 wavefronts 49 us for class
+// queries, 2 without spills 58, 4 wavefronts 64), 8 with a key mask at 128 channels (2 wavefronts 97 us for 4 images of 1089
+// tokens, 1 129 us), 2 in fp32 with a pair mask at 64 channels (2 wavefronts 334 us, 1 388 us).  With a pair mask at 128 channels
+// 2 wavefronts would spill 66: 4 images of 4225 tokens, 8 heads 1660 us, 1 wavefront 1366 us; 8 images of 1089 tokens, 16 heads
+// over 4 587 and 375 us.
 // Matrix-bound on long maps: 4 images of 4225 tokens, 16 heads over 4 of 128 channels: 1.05 to 1.13 ms for four products,
 // 1060 TFLOP/s, matrix cores busy 56 % of the cycles.  16 images of 961 tokens under key masks, 16 heads of 64 channels:
 // 155 us; a third of the tiles is padding and ends at once, so that 1.4 of 2 wavefronts to a SIMD are there on average.  A
@@ -29,7 +33,7 @@ constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 // channels.
 // MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
 template <typename T, int DP, int MASKS>
-__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
+__global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 || (MASKS == 2 && DP >= 128) ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnPiece<T, DP> Piece;
   constexpr int QT = dkv_rows<T, DP>();

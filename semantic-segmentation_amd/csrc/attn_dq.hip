@@ -15,6 +15,8 @@ namespace segk {
 // rounding's alone.  It costs a fourth product in three: 100 -> 120 us (16 images of 961 tokens, 16 heads of 64 channels).
 // Matrix-bound on long maps: 4 images of 4225 tokens, 16 heads over 4 of 128 channels: 0.96 ms, 1220 TFLOP/s with the fourth
 // product, matrix cores busy 65 % of the cycles.
+// Wavefronts to a SIMD: what is fastest.  At 64 channels under masks 3 of them spill 8 registers: 16 images of 961 tokens, 16
+// heads 121 us, 2 without spills 136 us.
 // What a row needs: its statistics and its query and output gradient in registers (zeros for a row that has no open key,
 // whatever its memory holds).
 template <typename T, int DP>
