@@ -299,7 +299,8 @@ int segk_dot_partial_rows(long long M);
  * relative to a reference that terms pass by up to 2^30: values beyond 1e25 may overflow.
  * Operands: [N][L][heads][D] by element strides with unit stride over D, 16-byte aligned, strides multiples of 16 bytes
  * (0: broadcast); D a multiple of 8 up to 128.  bf16 operands: fp32 scores, statistics and sums, probabilities rounded to
- * bf16 for their products (the score gradients of dq: as two bf16 operands) and out divided by the sum of the rounded ones;
+ * bf16 for their products (the score gradients of dq, and up to 64 rows - tokens times heads of a group - both factors of dk and
+ * dv: as two bf16 operands) and out divided by the sum of the rounded ones;
  * fp32 operands: exact-fp32 products.  Without out_rest the backward pass takes rowsum(dout * out) from out as rounded, which
  * costs accuracy where few keys carry a row (dq's rms error 0.0043 of its size instead of 0.0019 at scores of standard
  * deviation 8). */

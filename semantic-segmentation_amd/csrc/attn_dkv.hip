@@ -3,7 +3,13 @@
 // A workgroup owns 128 keys and walks over the packed rows (tokens x heads of the group): shared heads add up in its
 // registers, nothing is added atomically, every sum has a fixed order.
 // bf16: P and dS are rounded to operands of their products, as the probabilities of the forward pass are: rms error against 64
-// bits 0.0023 of the gradient's size, 0.0017 of it the final rounding.
+// bits 0.0023 of the gradient's size, 0.0017 of it the final rounding.  Up to 64 rows they go in as two operands each, the rounded
+// value and what the rounding left over: 0.0017.  A key's gradient is then a sum of few terms, often one, whose roundings nothing
+// evens out (0.0024 and more for dk of class queries whose windows hold few keys, where plain fp32 has 0.0016), and the products
+// are not what such a kernel waits for.
+// Time of the two more products, 8 images of 4225 keys, 8 heads of 32 (pair mask) / 64 / 64 (key mask) / 128 channels:
+//   21 rows 26.5 -> 28.0, 40 -> 42, 37 -> 40, 77 -> 78 us     64 rows 32 -> 35, 45 -> 47, 39 -> 45, 89 -> 92
+//   256 rows 77 -> 87, 66 -> 78, 60 -> 83, 142 -> 156         1024 rows 254 -> 298, 170 -> 226, 145 -> 217, 354 -> 430
 #include <type_traits>
 
 #include "attn.h"
@@ -32,7 +38,8 @@ constexpr int dkv_rows() { return AttnTile<T, DP>::PITCH < 128 ? 64 : 32; }
 // pipelined form (three blocks in flight, K and V in registers) took 155 us there, too, and 1.45 ms instead of 1.13 at 128
 // channels.
 // MASKS: 0 none, 1 a key mask, 2 a pair mask (and perhaps a key mask)
-template <typename T, int DP, int MASKS>
+// REST: P and dS as two operands each (see above)
+template <typename T, int DP, int MASKS, bool REST>
 __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 || (MASKS == 2 && DP >= 128) ? 1 : DP * (int)sizeof(T) > 64 ? 2 : 3)) void attn_dkv_kernel(const AttnDev p) {
   typedef AttnTile<T, DP> Tile;
   typedef AttnPiece<T, DP> Piece;
@@ -208,8 +215,13 @@ __global__ __launch_bounds__(ATTN_THREADS, (DP * (int)sizeof(T) >= 384 || (MASKS
         const AttnFrag<T> pf = pack_frag<T>(s, j), sf = pack_frag<T>(dp, j);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          mma32(dv[db], ln.cols(gt + (rb * 32 + j * 16) * Tile::PITCH, db), pf);
-          mma32(dk[db], ln.cols(qt + (rb * 32 + j * 16) * Tile::PITCH, db), sf);
+          const AttnFrag<T> gc = ln.cols(gt + (rb * 32 + j * 16) * Tile::PITCH, db), qc = ln.cols(qt + (rb * 32 + j * 16) * Tile::PITCH, db);
+          mma32(dv[db], gc, pf);
+          mma32(dk[db], qc, sf);
+          if constexpr (REST) {
+            mma32(dv[db], gc, pack_rest(s, j, pf));
+            mma32(dk[db], qc, pack_rest(dp, j, sf));
+          }
         }
       }
     }
@@ -286,10 +298,14 @@ template <typename T, int DP>
 static int launch(AttnDev* p, bool plan_only, hipStream_t st) {
   constexpr int QT = dkv_rows<T, DP>();
   const int lds = 2 * (2 * QT * AttnTile<T, DP>::PITCH + 512) + 128 * AttnTile<T, DP>::PITCH;
-  static std::atomic<int> seen[3][ATTN_DEVICES];
+  static std::atomic<int> seen[2][3][ATTN_DEVICES];
   const int masks = p->mask ? 2 : p->kmask ? 1 : 0;
-  auto kern = p->mask ? attn_dkv_kernel<T, DP, 2> : p->kmask ? attn_dkv_kernel<T, DP, 1> : attn_dkv_kernel<T, DP, 0>;
-  const int per_cu = attn_occupancy((const void*)kern, lds, seen[masks]);
+  const bool rest = sizeof(T) == 2 && p->R <= 64;
+  auto kern = p->mask ? attn_dkv_kernel<T, DP, 2, false> : p->kmask ? attn_dkv_kernel<T, DP, 1, false> : attn_dkv_kernel<T, DP, 0, false>;
+  if constexpr (sizeof(T) == 2) {
+    if (rest) kern = p->mask ? attn_dkv_kernel<T, DP, 2, true> : p->kmask ? attn_dkv_kernel<T, DP, 1, true> : attn_dkv_kernel<T, DP, 0, true>;
+  }
+  const int per_cu = attn_occupancy((const void*)kern, lds, seen[rest][masks]);
   if (per_cu < 0) return per_cu;
   p->tiles = ceil_div(p->Lk, 128);
   p->loop_rows = QT;
