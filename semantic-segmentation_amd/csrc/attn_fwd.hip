@@ -20,9 +20,9 @@ namespace segk {
 //   Scores of +inf and NaN end up there, too.
 // Two sums: l of p, for lse (LSE: training), and in bf16 lr of p as rounded for its product, by which out is divided.  Out is
 // then the exact mean of v under weights off by their rounding; divided by l, the roundings of the few probabilities that carry
-// a row would not cancel in delta = rowsum(dout out), next to which ds is small.  rms error of dq, of its size, at scores of standard
-// deviation 1 / 3 / 5 / 8 (512 x 1024, 64 channels): divided by l, delta from out as rounded 0.0017 / 0.0027 / 0.0044 / 0.0054;
-// by lr, out's own rounding carried (out_rest) 0.0017 / 0.0018 / 0.0019 / 0.0019; the final rounding alone 0.0017.
+// a row would not cancel in delta = rowsum(dout out), next to which ds is small.  rms error of dq, of its size, at scores of
+// standard deviation 1 / 3 / 5 / 8 (512 x 1024, 64 channels): divided by l, delta from out as rounded 0.0017 / 0.0027 / 0.0044 /
+// 0.0054; by lr, out's own rounding carried (out_rest) 0.0017 / 0.0018 / 0.0019 / 0.0019; the final rounding alone 0.0017.
 template <typename T, int DB, bool LSE>
 struct AttnRow {
   static constexpr bool ROUNDED = sizeof(T) == 2, BOTH = ROUNDED && LSE;
@@ -77,9 +77,9 @@ struct AttnRow {
 // the scores of block b + 1 and the values of block b - 1 on the matrix cores while the exponentials of block b run on the
 // vector unit: one wavefront keeps both busy, as independent instructions of one basic block.  LDS holds two K and two V
 // tiles; K runs one tile ahead of V.  Wavefronts to a SIMD: 4 where a row of a tile has 64 bytes (class queries under masks, 32
-// channels: 26.5 -> 22.3 us against 3, 20.2 now), 3 up to 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8 images of 1089
-// tokens, 8 heads of 96 channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.  At 32 and 64
-// channels under masks one register is spilled (64 channels, training, with 2 wavefronts and no spill: 115 us instead of 99).
+// channels: 26.5 -> 22.3 us against 3, 20.2 now), 3 up to 128 bytes, 1 for fp32 heads over 96 channels (under masks over 64: 8
+// images of 1089 tokens, 8 heads of 96 channels, key mask 573 -> 459 us; without a mask 2 take 410 and 1 takes 417), else 2.  At 32
+// and 64 channels under masks one register is spilled (64 channels, training, with 2 wavefronts and no spill: 115 us instead of 99).
 // Matrix-bound on long maps: 2 images of 16641 tokens, 8 heads over 2 of 128 channels, bf16: 2.06 to 2.12 ms, 1070 to 1100
 // TFLOP/s (a large library product reaches 1164 here); the matrix cores are busy 60 % of the cycles, at 1.8 GHz.
 // 16 images of 1089 tokens, 16 heads of 64 channels: 104 us, 747 TFLOP/s: half as many products to an exponential.

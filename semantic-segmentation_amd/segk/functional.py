@@ -1352,13 +1352,15 @@ def attention(q, k, v, mask=None, key_mask=None, causal=False, scale=None):
     q [N, Lq, Hq, D]; k, v [N, Lk, Hk, D] (float32 or bfloat16, D a multiple of 8 up to 128; query head h reads
     key / value head h // (Hq // Hk)) -> [N, Lq, Hq, D].  Views are read in place when their channels are contiguous and
     their rows 16-byte aligned (slices of one projection's output are), copied otherwise.
-      mask      bool, broadcastable to [N, Hq, Lq, Lk], True = open.  A closed pair has probability zero; its key and value
-                are still read and must be finite (so under causal).
+      mask      bool, four dimensions that broadcast to [N, Hq, Lq, Lk], True = open.  A closed pair has probability zero;
+                its key and value are still read and must be finite (so under causal).
       key_mask  bool [N, Lk], True = open (e.g. the pixels that are not padding).  A closed key is not read.
       causal    key j is open to token i for j <= i + Lk - Lq
       scale     of the scores, positive; default D ** -0.5
     A query without an open key gives zeros, and no gradient.  Sums are kept relative to a running reference that the
-    probabilities pass by up to 2^30: values beyond 1e25 may overflow.  Differentiable once with respect to q, k and v."""
+    probabilities pass by up to 2^30: values beyond 1e25 may overflow.  Differentiable once with respect to q, k and v;
+    bfloat16 keeps what out's rounding left over for that, 2 bytes an element.  torch.jit.trace records the call, forward-mode
+    differentiation raises."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes [N, L, heads, D] tensors, got %s, %s, %s"
                          % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -1412,7 +1414,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None,
       inv_freq     float32, one frequency per rotated pair; a multiple of 4 pairs, at most D / 2
       sections     how many of the pairs, in order, turn by each axis; default: equal shares
       interleaved  pairs are channels (2c, 2c + 1) instead of (c, c + pairs); channels past the pairs stay as normalised
-    Angles are formed in 64 bits.  Differentiable once with respect to q, k and the weights."""
+    Angles are formed in 64 bits.  Differentiable once with respect to q, k and the weights; torch.jit.trace records the call,
+    forward-mode differentiation raises."""
     args = (positions, inv_freq, None if sections is None else tuple(map(int, sections)), eps, interleaved)
     tensors = (q, k, q_weight, k_weight)
     if positions.requires_grad or inv_freq.requires_grad:
